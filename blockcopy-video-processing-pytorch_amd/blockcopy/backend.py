@@ -178,6 +178,10 @@ def load_library(path: str = None) -> ctypes.CDLL:
         "bc_pn_set_stamps": [p],
         "bc_pn_probs": [p, p, p, p, i, p],
         "bc_pn_features_nhwc": [p, i, i, i, i, p, p, p, p, p],
+        "bc_linear_fwd": [p] * 6 + [ctypes.c_longlong, i, i] + [ctypes.c_longlong] * 3 + [i, i, i, p, ctypes.c_longlong, p],
+        "bc_linear_bwd": [p] * 7 + [ctypes.c_longlong, i, i] + [ctypes.c_longlong] * 3 + [i, i, i, p, ctypes.c_longlong, p],
+        "bc_norm_residual_fwd": [p] * 10 + [ctypes.c_longlong, i] + [ctypes.c_longlong] * 3 + [ctypes.c_float, ctypes.c_float, i, i, i, i, p],
+        "bc_norm_residual_bwd": [p] * 16 + [ctypes.c_longlong, i] + [ctypes.c_longlong] * 5 + [ctypes.c_float, i, i, i, i, p, ctypes.c_longlong, p],
         "bc_dyn_set": [p, i],
         "bc_tune_set": [ctypes.c_char_p, i],
         "bc_tune_get": [ctypes.c_char_p, ctypes.POINTER(i)],
@@ -192,7 +196,9 @@ def load_library(path: str = None) -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = i
-    for name, argtypes in {"bc_pn_conv_partials": [i, i, i, i], "bc_pn_wgrad_workspace": [i] * 6, "bc_pn_bn_bwd_partials": [ctypes.c_longlong]}.items():
+    for name, argtypes in {"bc_pn_conv_partials": [i, i, i, i], "bc_pn_wgrad_workspace": [i] * 6, "bc_pn_bn_bwd_partials": [ctypes.c_longlong],
+                           "bc_linear_fwd_workspace": [ctypes.c_longlong, i, i, i], "bc_linear_bwd_workspace": [ctypes.c_longlong, i, i, i, i],
+                           "bc_norm_residual_bwd_workspace": [ctypes.c_longlong, i, ctypes.c_longlong, i]}.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = ctypes.c_longlong
@@ -1015,6 +1021,102 @@ class HipBackend:
                                                            ptr(bias), scale.data_ptr(), shift.data_ptr(), ws.data_ptr(), ws.numel(), self._stream()),
                         "group_norm_affine_nhwc")
         return scale, shift
+
+    # -- channel operators on rows of features (blockcopy/utils/channel_ops.py; csrc/linear.hip, csrc/norm_residual.hip).  Every matrix is
+    #    (rows, features) with unit feature stride; workspaces come from the caching allocator on the current stream, so a captured call owns
+    #    its workspace inside the graph's pool
+    @staticmethod
+    def _rows_ok(t, shape, dtype, device):
+        return t is None or (t.dim() == 2 and tuple(t.shape) == tuple(shape) and t.dtype == dtype and t.device == device
+                             and (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]))
+
+    @staticmethod
+    def _ld(t):
+        return 0 if t is None else max(t.stride(0), t.shape[1])      # (the stride of a single row may be anything)
+
+    def linear_fwd(self, x, weight, bias=None, act: int = 0, residual=None, keep_z: bool = False):
+        """(y, z): y = act(z) + residual with z = x weight^T + bias; z is handed back (x's dtype) if ``keep_z``."""
+        M, K = x.shape
+        N = weight.shape[0]
+        assert x.is_cuda and x.dtype in _DTYPE_CODE, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
+        assert self._rows_ok(x, (M, K), x.dtype, x.device) and self._rows_ok(weight, (N, K), x.dtype, x.device) and self._rows_ok(residual, (M, N), x.dtype, x.device)
+        assert bias is None or (bias.shape == (N,) and bias.is_contiguous() and bias.dtype in (x.dtype, torch.float32) and bias.device == x.device)
+        code = _DTYPE_CODE[x.dtype]
+        ptr = lambda t: t.data_ptr() if t is not None else None
+        with torch.cuda.device_of(x):
+            y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+            z = torch.empty_like(y) if keep_z else None
+            need = self.lib.bc_linear_fwd_workspace(M, N, K, code)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+            self._check(self.lib.bc_linear_fwd(ptr(y), ptr(z), ptr(x), ptr(weight), ptr(bias), ptr(residual), M, N, K, self._ld(x), self._ld(weight), self._ld(residual),
+                                               int(act), code, int(bias is not None and bias.dtype == torch.float32), ptr(ws), need, self._stream()), "linear_fwd")
+        return y, z
+
+    def linear_bwd(self, gy, z, x, weight, act: int, want, bias_dtype=None):
+        """(dx, dw, db) of ``linear_fwd`` for the gradient ``gy`` of y; ``want`` = three truth values, None in the place of the others."""
+        M, N = gy.shape
+        K = weight.shape[1] if weight is not None else x.shape[1]
+        dt, dev = gy.dtype, gy.device
+        assert gy.is_cuda and dt in _DTYPE_CODE
+        assert all(self._rows_ok(t, s, dt, dev) for t, s in ((gy, (M, N)), (z, (M, N)), (x, (M, K)), (weight, (N, K)))) and (z is None or z.is_contiguous())
+        dx = torch.empty((M, K), dtype=dt, device=dev) if want[0] else None
+        dw = torch.empty((N, K), dtype=dt, device=dev) if want[1] else None
+        db = torch.empty((N,), dtype=bias_dtype or dt, device=dev) if want[2] else None
+        if M == 0:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+        code = _DTYPE_CODE[dt]
+        ptr = lambda t: t.data_ptr() if t is not None else None
+        with torch.cuda.device_of(gy):
+            need = self.lib.bc_linear_bwd_workspace(M, N, K, int(act), code)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            self._check(self.lib.bc_linear_bwd(ptr(dx), ptr(dw), ptr(db), ptr(gy), ptr(z), ptr(x), ptr(weight), M, N, K, self._ld(gy), self._ld(x), self._ld(weight),
+                                               int(act), code, int(db is not None and db.dtype == torch.float32), ptr(ws), need, self._stream()), "linear_bwd")
+        return dx, dw, db
+
+    @staticmethod
+    def _norm_params_ok(params, C, dtype, device, groups=None):
+        kinds = {p.dtype for p in params if p is not None}
+        assert len(kinds) <= 1 and kinds <= {dtype, torch.float32}, "norm parameters and gate must share one dtype: the rows' or float32"
+        for k, p in enumerate(params):
+            assert p is None or (p.is_contiguous() and p.device == device and p.numel() == (C * groups if groups and k == 2 else C))
+        return int(kinds == {torch.float32})
+
+    def norm_residual_fwd(self, h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind: int, in_kind: int, residual_scale: float, eps: float,
+                          rows_per_gate: int = 0, keep_stats: bool = False):
+        """(h_new, u, stats): h_new = residual_scale * h + gate * N_out(y), u = N_in(h_new) (blockcopy/utils/channel_ops.py); None for what is not asked for."""
+        M, C = h.shape
+        assert h.is_cuda and h.dtype in _DTYPE_CODE, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
+        assert self._rows_ok(h, (M, C), h.dtype, h.device) and self._rows_ok(y, (M, C), h.dtype, h.device)
+        pf32 = self._norm_params_ok((out_weight, out_bias, gate, in_weight, in_bias), C, h.dtype, h.device, M // rows_per_gate if rows_per_gate else None)
+        ptr = lambda t: t.data_ptr() if t is not None else None
+        with torch.cuda.device_of(h):
+            ho = torch.empty((M, C), dtype=h.dtype, device=h.device) if y is not None else None
+            u = torch.empty((M, C), dtype=h.dtype, device=h.device) if in_kind else None
+            stats = torch.empty((M, 4), dtype=torch.float32, device=h.device) if keep_stats else None
+            self._check(self.lib.bc_norm_residual_fwd(ptr(ho), ptr(u), ptr(stats), ptr(h), ptr(y), ptr(out_weight), ptr(out_bias), ptr(gate), ptr(in_weight), ptr(in_bias),
+                                                      M, C, self._ld(h), self._ld(y), int(rows_per_gate), float(residual_scale), float(eps), int(out_kind), int(in_kind),
+                                                      _DTYPE_CODE[h.dtype], pf32, self._stream()), "norm_residual_fwd")
+        return ho, u, stats
+
+    def norm_residual_bwd(self, gh, gu, stats, h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind: int, in_kind: int, residual_scale: float,
+                          rows_per_gate: int, want):
+        """Gradients (dh, dy, d out_weight, d out_bias, d gate, d in_weight, d in_bias) of ``norm_residual_fwd``; ``want`` = seven truth values."""
+        M, C = h.shape
+        dt, dev = h.dtype, h.device
+        assert all(self._rows_ok(t, (M, C), dt, dev) for t in (gh, gu, h, y)) and stats.is_contiguous() and M > 0
+        params = (out_weight, out_bias, gate, in_weight, in_bias)
+        pf32 = self._norm_params_ok(params, C, dt, dev, M // rows_per_gate if rows_per_gate else None)
+        ptr = lambda t: t.data_ptr() if t is not None else None
+        with torch.cuda.device_of(h):
+            dh = torch.empty((M, C), dtype=dt, device=dev) if want[0] else None
+            dy = torch.empty((M, C), dtype=dt, device=dev) if want[1] else None
+            dp = [torch.empty_like(t) if w and t is not None else None for t, w in zip(params, want[2:])]
+            need = self.lib.bc_norm_residual_bwd_workspace(M, C, int(rows_per_gate), _DTYPE_CODE[dt]) if any(t is not None for t in dp) else 0
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            self._check(self.lib.bc_norm_residual_bwd(ptr(dh), ptr(dy), *map(ptr, dp), ptr(gh), ptr(gu), ptr(stats), ptr(h), ptr(y), ptr(out_weight), ptr(out_bias), ptr(gate),
+                                                      ptr(in_weight), M, C, self._ld(h), self._ld(y), self._ld(gh), self._ld(gu), int(rows_per_gate), float(residual_scale),
+                                                      int(out_kind), int(in_kind), _DTYPE_CODE[dt], pf32, ptr(ws), need, self._stream()), "norm_residual_bwd")
+        return (dh, dy, *dp)
 
     # -- network-input stage: window gather from the frame-state map + 7x7 / stride 2 stem conv (csrc/stem7x7.inc)
     @staticmethod

@@ -8,12 +8,18 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = [os.path.join(HERE, "csrc", "blockcopy_hip.hip")]
-EXTRA_SRC = [os.path.join(HERE, "csrc", "policy_net.hip")]      # translation units of their own (the RL policy's CNN: forward / backward / optimizer)
+# translation units of their own: the RL policy's CNN (forward / backward / optimizer), the channel operators (products, norms; forward / backward)
+EXTRA_SRC = [os.path.join(HERE, "csrc", f) for f in ("policy_net.hip", "linear.hip", "norm_residual.hip")]
 HDR = [os.path.join(os.path.dirname(HERE), "include", "blockcopy_hip.h")] + [os.path.join(HERE, "csrc", f) for f in
                                                                              ("conv3x3_mfma.inc", "conv3x3_v2.inc", "conv3x3_wino.inc", "conv3x3_wino32.inc", "conv3x3_wino4.inc", "stem7x7.inc", "head1x1.inc", "pred3x3.inc", "gemm1x1.inc", "spp.inc")]
+NO_PACKED_SRC = ("linear.hip", "norm_residual.hip")
 OUT = os.path.join(HERE, "lib", "libblockcopy_hip.so")
 OBJ_DIR = os.path.join(HERE, "lib", "obj")
 ARCH = "gfx950"
+# hipcc -O3 turns pairs of ordinary float operations into packed fp32 instructions, some forms of which have returned wrong results on
+# this hardware now and then; the scalar instructions round identically (the host pass warns that it does not know the feature: harmless).
+# For the units of NO_PACKED_SRC; the conv units write such instructions themselves and would not compile under it
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # the one source is compiled as 7 translation units (-DBC_PART=n, see ConvV2Args in csrc/blockcopy_hip.hip): part 0 = everything
 # but the decompositions of the fused conv kernel, parts 1..6 = one (dtype, kernel size) slice of them each, part 7 = its Winograd form,
 # part 8 = the wide-tile Winograd form, part 9 = the dilation-2 form of the direct kernel, part 10 = the Winograd F(4x4,3x3) form
@@ -53,7 +59,9 @@ def build_hip_library(force: bool = False, verbose: bool = False) -> str:
         if fresh(objs[n], ([EXTRA_SRC[n - len(PARTS)], HDR[0]] if n >= len(PARTS) else SRC + HDR) + [os.path.abspath(__file__)]):
             return
         if n >= len(PARTS):
-            subprocess.check_call([hipcc()] + flags + ["-c", "-o", objs[n], EXTRA_SRC[n - len(PARTS)]])
+            src = EXTRA_SRC[n - len(PARTS)]
+            unit = NO_PACKED_FP32 if os.path.basename(src) in NO_PACKED_SRC else []
+            subprocess.check_call([hipcc()] + flags + unit + ["-c", "-o", objs[n], src])
         else:
             subprocess.check_call([hipcc()] + flags + [f"-DBC_PART={PARTS[n]}", "-c", "-o", objs[n]] + SRC)
 

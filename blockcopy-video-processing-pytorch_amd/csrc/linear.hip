@@ -1,0 +1,610 @@
+// linear.hip -- rows x weights products with the whole epilogue in the kernel, and their gradients.  Part of libblockcopy_hip.so.
+//
+//   forward     z[m][n] = sum_k x[m][k] w[n][k] + bias[n]          y[m][n] = act(z[m][n]) + residual[m][n]
+//   backward    dz = dy * act'(z)     dx[m][k] = sum_n dz[m][n] w[n][k]     dw[n][k] = sum_m dz[m][n] x[m][k]     db[n] = sum_m dz[m][n]
+//
+// A row is one pixel of a channels-last map (or one token), its features are the map's channels; bc_conv1x1_nhwc is the inference form of the
+// same product for packed channel counts, with per-channel affine records around it.  The three products are ONE kernel (k_lin_gemm) over
+// operands that either run along the summed index (KC) or across it (MC).  Sums, pre-activations and epilogue are fp32; z and dz are
+// rounded to the tensors' type once where they are stored.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/blockcopy_hip.h"
+
+#define BC_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 *lds_s16x4_ptr;
+
+enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };      // the dtype codes of the C ABI
+
+// V elements make 16 bytes; BK summed indexes make the 128 bytes of one staged row
+template <int DT> struct LinT { typedef float S; static constexpr int V = 4, BK = 32; };
+template <> struct LinT<DT_F16> { typedef _Float16 S; static constexpr int V = 8, BK = 64; };
+template <> struct LinT<DT_BF16> { typedef __bf16 S; static constexpr int V = 8, BK = 64; };
+
+inline int lin_status()
+{
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? BC_OK : (int)e;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ activations
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4, ACT_COUNT = 5 };
+
+// gelu_tanh is z * (1 + tanh(u)) / 2 = z * sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3): one exponential, nothing cancels
+constexpr float GELU_A = 0.7978845608028654f, GELU_B = 0.044715f;
+
+__device__ __forceinline__ float lin_act(float z, int act)
+{
+    switch (act) {
+    case ACT_RELU: return z > 0.f || z != z ? z : 0.f;
+    case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case ACT_GELU_TANH: return z / (1.f + expf(-2.f * GELU_A * (z + GELU_B * z * z * z)));
+    case ACT_SILU: return z / (1.f + expf(-z));
+    default: return z;
+    }
+}
+
+// act'(z).  Beyond +-64 every derivative is 0 or 1 to the last bit; the clamp keeps 0 * infinity out of the products (NaN passes through)
+__device__ __forceinline__ float lin_dact(float z, int act)
+{
+    const float c = z > 64.f ? 64.f : (z < -64.f ? -64.f : z);
+    switch (act) {
+    case ACT_RELU: return z != z ? z : (z > 0.f ? 1.f : 0.f);
+    case ACT_GELU: return 0.5f * (1.f + erff(c * 0.70710678118654752f)) + c * expf(-0.5f * c * c) * 0.3989422804014327f;
+    case ACT_GELU_TANH: {
+        const float u = 2.f * GELU_A * (c + GELU_B * c * c * c), s = 1.f / (1.f + expf(-u));
+        return s + c * s * (1.f - s) * 2.f * GELU_A * (1.f + 3.f * GELU_B * c * c);
+    }
+    case ACT_SILU: {
+        const float s = 1.f / (1.f + expf(-c));
+        return s * (1.f + c * (1.f - s));
+    }
+    default: return 1.f;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ the product
+struct LinOperand {
+    const void *p;
+    long long ld;       // elements between consecutive rows of memory
+};
+
+struct LinEpi {
+    void *y, *z;                // z: the pre-activations in the tensors' type (NULL: not kept)
+    const void *bias, *res;
+    long long ldr;
+    int bias_f32, act, vec;     // vec: four consecutive outputs may move as one vector
+};
+
+struct LinArgs {
+    LinOperand a, b;            // a: the operand of the output's columns (n), b: of its rows (m)
+    int M, N, K;
+    int kspan;                  // summed indexes of one slice (a multiple of BK): slice s takes [s kspan, (s + 1) kspan)
+    int vec_a, vec_b;           // 16-byte vectors never straddle a row's end and are aligned
+    unsigned tiles_m, tiles_n;
+    float *part;                // [slices][M][N] sums of the slices, or NULL: one slice, epilogue in place
+    LinEpi ep;
+};
+
+template <int DT> __device__ __forceinline__ void lin_mma(f32x4 &d, const uint4 &a, const uint4 &b)
+{
+    if constexpr (DT == DT_F16)
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
+    else if constexpr (DT == DT_BF16)
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), d, 0, 0, 0);
+    else {      // fp32: exact products, four k-steps of the 16 x 16 x 4 instruction; lane group g holds k = 4 g + j for step j on both sides
+        const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j], fb[j], d, 0, 0, 0);
+    }
+}
+
+// One staged operand tile: R rows (output rows or columns) x BK summed indexes = R * 8 vectors of 16 bytes.
+//   KC (memory runs along the summed index): image [row][8 vectors], vector c of row r at c ^ (r & 7): the 16 rows x 4 vectors that one
+//      fragment read touches cover all banks
+//   MC (memory runs across it): image [k][R / V vectors], vectors exchanged by lin_swz(k); 16-bit fragments are transposed by the LDS read
+//      itself (ds_read_b64_tr_b16: a group of 16 lanes addresses 4 k x 16 rows and lane i receives row i's four k), fp32 ones read word by word
+template <int DT, int R> __device__ __forceinline__ int lin_swz(int k)
+{
+    if constexpr (DT == DT_F32) return ((k >> 2) & 3) * 4;
+    else return ((k & 3) * 2 + ((k >> 3) & 1) * 8) & (R / 8 - 1);
+}
+
+template <int DT, bool MC, int R> __device__ __forceinline__ uint4 lin_frag(const uint4 *img, int row0, int ks, int lane)
+{
+    constexpr int V = LinT<DT>::V, CPR = R / V;
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (!MC) {
+        const int row = row0 + r;
+        return img[row * 8 + ((ks * 4 + g) ^ (row & 7))];
+    } else if constexpr (DT == DT_F32) {
+        const float *f = (const float *)img;
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = ks * 16 + 4 * g + j;
+            v[j] = f[k * R + ((((row0 + r) >> 2) ^ lin_swz<DT, R>(k)) << 2) + (r & 3)];
+        }
+        return uint4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    } else {
+        const int k = ks * 32 + 8 * g + (r >> 2), c = (row0 >> 3) + ((r & 3) >> 1);
+        const short *s = (const short *)img + ((k * CPR + (c ^ lin_swz<DT, R>(k))) * 8 + (r & 1) * 4);
+        const short *t = (const short *)img + (((k + 4) * CPR + (c ^ lin_swz<DT, R>(k + 4))) * 8 + (r & 1) * 4);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)s), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)t);
+        const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+        return uint4{a.x, a.y, b.x, b.y};
+    }
+}
+
+// 16 bytes of an operand starting at (row, k); elements outside the matrix (or the slice, k >= kend) are zero
+template <int DT, bool MC> __device__ __forceinline__ uint4 lin_fetch(const LinOperand &o, int vec, int rows, int kend, int row, int k)
+{
+    constexpr int V = LinT<DT>::V;
+    typedef typename LinT<DT>::S S;
+    const int run = MC ? row : k, run_end = MC ? rows : kend;       // the index that memory runs along
+    if (MC ? k >= kend : row >= rows) return uint4{0u, 0u, 0u, 0u};
+    const S *p = (const S *)o.p + (MC ? (size_t)k * o.ld + row : (size_t)row * o.ld + k);
+    if (vec && run + V <= run_end) return *(const uint4 *)p;
+    union { S s[V]; uint4 v; } u;
+    u.v = uint4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (run + e < run_end) u.s[e] = p[e];
+    return u.v;
+}
+
+template <int DT> __device__ __forceinline__ float lin_bias(const LinEpi &ep, int n)
+{
+    typedef typename LinT<DT>::S S;
+    return ep.bias ? (ep.bias_f32 ? ((const float *)ep.bias)[n] : (float)((const S *)ep.bias)[n]) : 0.f;
+}
+
+// four consecutive outputs (m, n .. n + 3) out of fp32 sums
+template <int DT> __device__ __forceinline__ void lin_store4(const LinEpi &ep, int N, int m, int n, const float *v)
+{
+    typedef typename LinT<DT>::S S;
+    typedef S S4 __attribute__((ext_vector_type(4)));
+    const size_t at = (size_t)m * N + n;
+    S4 y, z, r;
+    if (ep.vec) {
+        if (ep.res) r = *(const S4 *)((const S *)ep.res + (size_t)m * ep.ldr + n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float t = v[e] + lin_bias<DT>(ep, n + e);
+            z[e] = (S)t;
+            y[e] = (S)(lin_act(t, ep.act) + (ep.res ? (float)r[e] : 0.f));
+        }
+        if (ep.z) *(S4 *)((S *)ep.z + at) = z;
+        *(S4 *)((S *)ep.y + at) = y;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < N) {
+            const float t = v[e] + lin_bias<DT>(ep, n + e);
+            if (ep.z) ((S *)ep.z)[at + e] = (S)t;
+            ((S *)ep.y)[at + e] = (S)(lin_act(t, ep.act) + (ep.res ? (float)((const S *)ep.res)[(size_t)m * ep.ldr + n + e] : 0.f));
+        }
+}
+
+// out[m][n] = sum_k A(n, k) B(m, k).  A workgroup of WM x WN waves owns a BM x BN tile; the column operand is the matrix instruction's first
+// one, so a lane ends up with four consecutive columns of one row.  Operands go through registers into a double-buffered LDS image: the
+// loads of step t + 1 are requested before the products of step t and stored behind them, one barrier per step.
+template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC>
+__global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
+{
+    constexpr int V = LinT<DT>::V, BK = LinT<DT>::BK, NT = 64 * WM * WN;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int NA = BN * 8 / NT, NB = BM * 8 / NT;       // vectors per thread and step
+    constexpr int IMG = (BM + BN) * 8;
+    extern __shared__ uint4 lin_lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    // tiles in bands of 8 tile rows: neighbouring workgroups share operands
+    const unsigned band = 8 * g.tiles_n, b0 = blockIdx.x / band, in = blockIdx.x % band;
+    const unsigned rows_in_band = g.tiles_m - b0 * 8 < 8 ? g.tiles_m - b0 * 8 : 8;
+    const int m0 = (int)(b0 * 8 + in % rows_in_band) * BM, n0 = (int)(in / rows_in_band) * BN;
+    const int kbeg = (int)blockIdx.y * g.kspan, kend = g.K - kbeg < g.kspan ? g.K : kbeg + g.kspan;
+
+    uint4 ra[NA], rb[NB];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int v = tid + NT * i;
+            if constexpr (AMC) ra[i] = lin_fetch<DT, true>(g.a, g.vec_a, g.N, kend, n0 + v % (BN / V) * V, k0 + v / (BN / V));
+            else ra[i] = lin_fetch<DT, false>(g.a, g.vec_a, g.N, kend, n0 + (v >> 3), k0 + (v & 7) * V);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int v = tid + NT * i;
+            if constexpr (BMC) rb[i] = lin_fetch<DT, true>(g.b, g.vec_b, g.M, kend, m0 + v % (BM / V) * V, k0 + v / (BM / V));
+            else rb[i] = lin_fetch<DT, false>(g.b, g.vec_b, g.M, kend, m0 + (v >> 3), k0 + (v & 7) * V);
+        }
+    };
+    auto stage = [&](uint4 *img) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int v = tid + NT * i;
+            if constexpr (AMC) img[(v / (BN / V)) * (BN / V) + ((v % (BN / V)) ^ lin_swz<DT, BN>(v / (BN / V)))] = ra[i];
+            else img[(v & ~7) + ((v & 7) ^ ((v >> 3) & 7))] = ra[i];
+        }
+        img += BN * 8;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int v = tid + NT * i;
+            if constexpr (BMC) img[(v / (BM / V)) * (BM / V) + ((v % (BM / V)) ^ lin_swz<DT, BM>(v / (BM / V)))] = rb[i];
+            else img[(v & ~7) + ((v & 7) ^ ((v >> 3) & 7))] = rb[i];
+        }
+    };
+
+    f32x4 acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    fetch(kbeg);
+    stage(lin_lds);
+    __syncthreads();
+    int cur = 0;
+    for (int k0 = kbeg; k0 < kend; k0 += BK) {
+        const bool more = k0 + BK < kend;
+        if (more) fetch(k0 + BK);
+        const uint4 *ia = lin_lds + cur * IMG, *ib = ia + BN * 8;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            uint4 fa[FN], fb[FM];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) fa[i] = lin_frag<DT, AMC, BN>(ia, wn * (BN / WN) + 16 * i, ks, lane);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) fb[j] = lin_frag<DT, BMC, BM>(ib, wm * (BM / WM) + 16 * j, ks, lane);
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FM; ++j) lin_mma<DT>(acc[i][j], fa[i], fb[j]);
+        }
+        if (more) stage(lin_lds + (cur ^ 1) * IMG);
+        __syncthreads();
+        cur ^= 1;
+    }
+
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int m = m0 + wm * (BM / WM) + 16 * j + (lane & 15);
+        if (m >= g.M) continue;
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            const int n = n0 + wn * (BN / WN) + 16 * i + 4 * (lane >> 4);
+            if (n >= g.N) continue;
+            const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+            if (g.part) {
+                float *p = g.part + ((size_t)blockIdx.y * g.M + m) * g.N + n;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < g.N) p[e] = v[e];
+            } else
+                lin_store4<DT>(g.ep, g.N, m, n, v);
+        }
+    }
+}
+
+// sums of the slices in their order (run-to-run identical), then the epilogue: one thread per four outputs of a row
+template <int DT> __global__ __launch_bounds__(256) void k_lin_join(const float *part, int slices, int M, int N, LinEpi ep)
+{
+    const unsigned quads = ((unsigned)N + 3) / 4;
+    const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t m = id / quads;
+    if (m >= (size_t)M) return;
+    const int n = (int)(id % quads) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < slices; ++s) {
+        const float *p = part + ((size_t)s * M + m) * N + n;
+        if (ep.vec) {
+            const f32x4 q = *(const f32x4 *)p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += q[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < N) v[e] += p[e];
+        }
+    }
+    lin_store4<DT>(ep, N, (int)m, n, v);
+}
+
+// dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.
+struct DactArgs {
+    const void *gy, *z;         // z NULL: no activation, dz = gy is not stored
+    void *dz;
+    float *part;                // [gridDim.y][N], or NULL: no sums asked for
+    long long ldg;
+    int M, N, span, act, tpr_log;
+};
+
+template <int DT, int W> __global__ __launch_bounds__(256) void k_lin_dact(const DactArgs a)
+{
+    typedef typename LinT<DT>::S S;
+    typedef S SW __attribute__((ext_vector_type(W)));
+    __shared__ float red[256 * W];
+    const int tpr = 1 << a.tpr_log, tid = threadIdx.x, c = tid & (tpr - 1), r = tid >> a.tpr_log, rows = 256 >> a.tpr_log;
+    const int n = ((int)blockIdx.x * tpr + c) * W;
+    const int m1 = a.M - (int)blockIdx.y * a.span < a.span ? a.M : ((int)blockIdx.y + 1) * a.span;
+    float sum[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) sum[e] = 0.f;
+    if (n < a.N)
+        for (int m = (int)blockIdx.y * a.span + r; m < m1; m += rows) {
+            const SW gy = *(const SW *)((const S *)a.gy + (size_t)m * a.ldg + n);
+            SW d;
+            if (a.z) {
+                const SW z = *(const SW *)((const S *)a.z + (size_t)m * a.N + n);
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    const float t = (float)gy[e] * lin_dact((float)z[e], a.act);
+                    sum[e] += t;
+                    d[e] = (S)t;
+                }
+                *(SW *)((S *)a.dz + (size_t)m * a.N + n) = d;
+            } else {
+#pragma unroll
+                for (int e = 0; e < W; ++e) sum[e] += (float)gy[e];
+            }
+        }
+    if (!a.part) return;
+#pragma unroll
+    for (int e = 0; e < W; ++e) red[tid * W + e] = sum[e];
+    __syncthreads();
+    if (r == 0 && n < a.N)
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+            float s = 0.f;
+            for (int q = 0; q < rows; ++q) s += red[((q << a.tpr_log) + c) * W + e];
+            a.part[(size_t)blockIdx.y * a.N + n + e] = s;
+        }
+}
+
+template <int DT> __global__ __launch_bounds__(256) void k_lin_colsum(void *db, int db_f32, const float *part, int P, int N)
+{
+    typedef typename LinT<DT>::S S;
+    const int n = (int)blockIdx.x * 256 + threadIdx.x;
+    if (n >= N) return;
+    float s = 0.f;
+    for (int p = 0; p < P; ++p) s += part[(size_t)p * N + n];
+    if (db_f32) ((float *)db)[n] = s;
+    else ((S *)db)[n] = (S)s;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ host side
+constexpr int LIN_CUS = 256;
+
+struct LinPlan { int slices, kspan; unsigned tm, tn; };
+
+inline int lin_bk(int dtype) { return dtype == DT_F32 ? 32 : 64; }
+inline long long lin_round(long long v, long long to) { return (v + to - 1) / to * to; }
+
+LinPlan lin_plan(int dtype, long long M, long long N, long long K)
+{
+    LinPlan p;
+    const int bk = lin_bk(dtype);
+    p.tm = (unsigned)((M + 127) / 128);
+    p.tn = (unsigned)((N + 127) / 128);
+    const long long tiles = (long long)p.tm * p.tn, steps = (K + bk - 1) / bk;
+    long long s = tiles >= LIN_CUS ? 1 : 2 * LIN_CUS / tiles;
+    s = s < steps / 4 ? s : steps / 4;
+    if (s < 1) s = 1;
+    const long long per = (steps + s - 1) / s;
+    p.kspan = (int)(per * bk);
+    p.slices = (int)((steps + per - 1) / per);
+    if (p.slices < 1) p.slices = 1;
+    return p;
+}
+
+inline long long lin_part_bytes(const LinPlan &p, long long M, long long N) { return p.slices > 1 ? lin_round(4ll * p.slices * M * N, 256) : 0; }
+
+template <int DT, bool AMC, bool BMC> int lin_run(LinArgs &g, const LinPlan &p, void *ws, hipStream_t st)
+{
+    constexpr int BM = 128, BN = 128;
+    g.kspan = p.kspan;
+    g.tiles_m = p.tm;
+    g.tiles_n = p.tn;
+    g.part = p.slices > 1 ? (float *)ws : nullptr;
+    const size_t lds = 2 * (BM + BN) * 8 * sizeof(uint4);
+    static const hipError_t attr = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, 2, 2, AMC, BMC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (attr != hipSuccess) return (int)attr;
+    k_lin_gemm<DT, BM, BN, 2, 2, AMC, BMC><<<dim3(p.tm * p.tn, p.slices), 256, lds, st>>>(g);
+    if (p.slices > 1) {
+        const long long threads = (long long)g.M * ((g.N + 3) / 4);
+        k_lin_join<DT><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(g.part, p.slices, g.M, g.N, g.ep);
+    }
+    return lin_status();
+}
+
+template <bool AMC, bool BMC> int lin_product(int dtype, LinArgs &g, const LinPlan &p, void *ws, hipStream_t st)
+{
+    switch (dtype) {
+    case DT_F32: return lin_run<DT_F32, AMC, BMC>(g, p, ws, st);
+    case DT_F16: return lin_run<DT_F16, AMC, BMC>(g, p, ws, st);
+    default: return lin_run<DT_BF16, AMC, BMC>(g, p, ws, st);
+    }
+}
+
+inline int lin_esize(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+// 16-byte vectors of a matrix with rows of `run` elements, `ld` apart
+inline int lin_vec(const void *p, long long ld, int dtype)
+{
+    const int e = lin_esize(dtype);
+    return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0;
+}
+inline int lin_vec4(const void *p, long long ld, int dtype) { return !p || ((uintptr_t)p % (4 * lin_esize(dtype)) == 0 && ld % 4 == 0); }
+inline bool lin_aligned(const void *p, int dtype) { return (uintptr_t)p % lin_esize(dtype) == 0; }
+
+int lin_sizes(long long M, int N, int K, int dtype)
+{
+    if (dtype < 0 || dtype > 2) return BC_ERR_ELEM;
+    if (M < 0 || N < 1 || K < 1) return BC_ERR_SHAPE;
+    if (M > 0x7fffff00ll || N > 0x7fffff00 || K > 0x7fffff00) return BC_ERR_RANGE;
+    if (((M + 127) / 128) * (((long long)N + 127) / 128) > 0x7fffff00ll || ((M + 127) / 128) * (((long long)K + 127) / 128) > 0x7fffff00ll ||
+        (((long long)N + 127) / 128) * (((long long)K + 127) / 128) > 0x7fffff00ll)
+        return BC_ERR_RANGE;
+    return BC_OK;
+}
+
+struct DactPlan { int W, tpr_log, span; unsigned gx, gy; };
+
+DactPlan lin_dact_plan(long long M, int N, int V, bool vec)
+{
+    DactPlan p;
+    p.W = vec ? V : 1;
+    const int units = (N + p.W - 1) / p.W;
+    p.tpr_log = 0;
+    while (p.tpr_log < 8 && (1 << p.tpr_log) < units) ++p.tpr_log;
+    const int rows = 256 >> p.tpr_log;
+    p.gx = (unsigned)((units + (1 << p.tpr_log) - 1) >> p.tpr_log);
+    long long chunks = 4 * LIN_CUS / p.gx > 0 ? 4 * LIN_CUS / p.gx : 1;
+    const long long most = (M + 4 * rows - 1) / (4 * rows);
+    if (chunks > most) chunks = most;
+    if (chunks < 1) chunks = 1;
+    p.span = (int)((M + chunks - 1) / chunks);
+    if (p.span < 1) p.span = 1;
+    p.gy = (unsigned)((M + p.span - 1) / p.span);
+    return p;
+}
+
+template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, void *db, int db_f32, hipStream_t st)
+{
+    DactArgs a = a0;
+    a.span = p.span;
+    a.tpr_log = p.tpr_log;
+    if (p.W > 1) k_lin_dact<DT, LinT<DT>::V><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
+    else k_lin_dact<DT, 1><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
+    if (db) k_lin_colsum<DT><<<(a.N + 255) / 256, 256, 0, st>>>(db, db_f32, a.part, (int)p.gy, a.N);
+    return lin_status();
+}
+
+}  // namespace
+
+BC_EXPORT long long bc_linear_fwd_workspace(long long M, int N, int K, int dtype)
+{
+    if (lin_sizes(M, N, K, dtype) != BC_OK || M == 0) return 0;
+    return lin_part_bytes(lin_plan(dtype, M, N, K), M, N);
+}
+
+BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, long long M, int N, int K, long long ldx,
+                            long long ldw, long long ldr, int act, int dtype, int bias_f32, void *workspace, long long workspace_bytes, void *stream)
+{
+    const int rc = lin_sizes(M, N, K, dtype);
+    if (rc != BC_OK) return rc;
+    if (act < 0 || act >= ACT_COUNT || ldx < K || ldw < K || (residual && ldr < N)) return BC_ERR_SHAPE;
+    if (M == 0) return BC_OK;
+    if (!y || !x || !w) return BC_ERR_NULL;
+    if (!lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(y, dtype) || !lin_aligned(z, dtype) || !lin_aligned(residual, dtype)) return BC_ERR_ALIGN;
+    const LinPlan p = lin_plan(dtype, M, N, K);
+    const long long need = lin_part_bytes(p, M, N);
+    if (need > 0 && !workspace) return BC_ERR_NULL;
+    if (workspace_bytes < need) return BC_ERR_SHAPE;
+    if (need > 0 && (uintptr_t)workspace % 16 != 0) return BC_ERR_ALIGN;
+    LinArgs g = {};
+    g.a = {w, ldw};
+    g.b = {x, ldx};
+    g.M = (int)M;
+    g.N = N;
+    g.K = K;
+    g.vec_a = lin_vec(w, ldw, dtype);
+    g.vec_b = lin_vec(x, ldx, dtype);
+    g.ep = {y, z, bias, residual, ldr, bias_f32, act, lin_vec4(y, N, dtype) && lin_vec4(z, N, dtype) && lin_vec4(residual, ldr, dtype)};
+    return lin_product<false, false>(dtype, g, p, workspace, (hipStream_t)stream);
+}
+
+// the workspace of a backward pass: dz (activations only), the column sums' partials, and the slices of one product at a time
+struct LinBwdSpace { long long dz, part, slices; };
+static LinBwdSpace lin_bwd_space(long long M, int N, int K, int act, int dtype)
+{
+    LinBwdSpace s;
+    s.dz = act != ACT_NONE ? lin_round(M * N * lin_esize(dtype), 256) : 0;
+    const DactPlan a = lin_dact_plan(M, N, dtype == DT_F32 ? 4 : 8, true), b = lin_dact_plan(M, N, 1, false);
+    s.part = lin_round(4ll * N * (a.gy > b.gy ? a.gy : b.gy), 256);
+    const long long x = lin_part_bytes(lin_plan(dtype, M, K, N), M, K), w = lin_part_bytes(lin_plan(dtype, N, K, M), N, K);
+    s.slices = x > w ? x : w;
+    return s;
+}
+
+BC_EXPORT long long bc_linear_bwd_workspace(long long M, int N, int K, int act, int dtype)
+{
+    if (lin_sizes(M, N, K, dtype) != BC_OK || M == 0 || act < 0 || act >= ACT_COUNT) return 0;
+    const LinBwdSpace s = lin_bwd_space(M, N, K, act, dtype);
+    return s.dz + s.part + s.slices;
+}
+
+BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const void *z, const void *x, const void *w, long long M, int N, int K, long long ldg,
+                            long long ldx, long long ldw, int act, int dtype, int bias_f32, void *workspace, long long workspace_bytes, void *stream)
+{
+    const int rc = lin_sizes(M, N, K, dtype);
+    if (rc != BC_OK) return rc;
+    if (act < 0 || act >= ACT_COUNT || ldg < N || (dw && ldx < K) || (dx && ldw < K)) return BC_ERR_SHAPE;
+    if (M == 0) return BC_ERR_SHAPE;        // (no rows: the caller's gradients are zeros, nothing to launch)
+    if (!gy || (act != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return BC_ERR_NULL;
+    if (!lin_aligned(gy, dtype) || !lin_aligned(z, dtype) || !lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(dx, dtype) || !lin_aligned(dw, dtype))
+        return BC_ERR_ALIGN;
+    const LinBwdSpace s = lin_bwd_space(M, N, K, act, dtype);
+    if (s.dz + s.part + s.slices > 0 && !workspace) return BC_ERR_NULL;
+    if (workspace_bytes < s.dz + s.part + s.slices) return BC_ERR_SHAPE;
+    if ((uintptr_t)workspace % 256 != 0) return BC_ERR_ALIGN;
+    hipStream_t st = (hipStream_t)stream;
+    char *wsp = (char *)workspace;
+    void *slices = wsp + s.dz + s.part;
+    const void *dz = gy;
+    long long ldz = ldg;
+    if (act != ACT_NONE || db) {
+        const int V = dtype == DT_F32 ? 4 : 8;
+        const bool vec = N % V == 0 && lin_vec(gy, ldg, dtype) && (!z || lin_vec(z, N, dtype));
+        const DactPlan p = lin_dact_plan(M, N, V, vec);
+        DactArgs a = {};
+        a.gy = gy;
+        a.z = act != ACT_NONE ? z : nullptr;
+        a.dz = act != ACT_NONE ? wsp : nullptr;
+        a.part = db ? (float *)(wsp + s.dz) : nullptr;
+        a.ldg = ldg;
+        a.M = (int)M;
+        a.N = N;
+        a.act = act;
+        const int r = dtype == DT_F32 ? lin_dact_run<DT_F32>(a, p, db, bias_f32, st) : dtype == DT_F16 ? lin_dact_run<DT_F16>(a, p, db, bias_f32, st)
+                                                                                                     : lin_dact_run<DT_BF16>(a, p, db, bias_f32, st);
+        if (r != BC_OK) return r;
+        if (act != ACT_NONE) { dz = wsp; ldz = N; }
+    }
+    if (dx) {       // dx[m][k] = sum_n dz[m][n] w[n][k]: the weight runs across the summed index
+        LinArgs g = {};
+        g.a = {w, ldw};
+        g.b = {dz, ldz};
+        g.M = (int)M;
+        g.N = K;
+        g.K = N;
+        g.vec_a = lin_vec(w, ldw, dtype);
+        g.vec_b = lin_vec(dz, ldz, dtype);
+        g.ep = {dx, nullptr, nullptr, nullptr, 0, 0, ACT_NONE, lin_vec4(dx, K, dtype)};
+        const int r = lin_product<true, false>(dtype, g, lin_plan(dtype, M, K, N), slices, st);
+        if (r != BC_OK) return r;
+    }
+    if (dw) {       // dw[n][k] = sum_m dz[m][n] x[m][k]: both run across it
+        LinArgs g = {};
+        g.a = {x, ldx};
+        g.b = {dz, ldz};
+        g.M = N;
+        g.N = K;
+        g.K = (int)M;
+        g.vec_a = lin_vec(x, ldx, dtype);
+        g.vec_b = lin_vec(dz, ldz, dtype);
+        g.ep = {dw, nullptr, nullptr, nullptr, 0, 0, ACT_NONE, lin_vec4(dw, K, dtype)};
+        const int r = lin_product<true, true>(dtype, g, lin_plan(dtype, N, K, M), slices, st);
+        if (r != BC_OK) return r;
+    }
+    return BC_OK;
+}

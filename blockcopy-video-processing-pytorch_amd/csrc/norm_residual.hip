@@ -1,0 +1,602 @@
+// norm_residual.hip -- what stands between two blocks of a residual network, in one pass over the rows, and its gradient.  Part of
+// libblockcopy_hip.so.
+//
+//   t  = N_out(y) * wo + bo                 the norm after a block (or y itself)
+//   h' = residual_scale * h + gate * t      the block's gate (per channel, or per sample and channel) and the residual stream
+//   u  = N_in(h') * wi + bi                 the norm before the next block (or nothing)
+//   N(x) = x / sqrt(mean(x^2) + eps)  (rms)   or   (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps)  (layer), over the C channels of a row
+//
+// A row is one pixel of a channels-last map (or one token).  All statistics and sums are fp32 and centred (two passes over registers);
+// u is formed from the unrounded h'.  Bound: memory -- forward reads h, y and writes h', u; backward reads h, y and the two gradients and
+// writes dh, dy.  It forms h' again out of h and y (the same bytes as reading it back, without its rounding).
+// Decomposition: a lane owns E channels of a row (16-byte vectors) and a row G lanes -- part of a wave, or up to 16 waves that exchange
+// their sums through the LDS.  Backward: a lane keeps the same channels for every row of its workgroup, so the five column sums (gate,
+// norm weights and biases) stay in registers, and go to a workspace once per workgroup; a second launch adds them in a fixed order.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/blockcopy_hip.h"
+
+#define BC_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
+enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
+
+template <int DT> struct NrT { typedef float S; static constexpr int V = 4; };
+template <> struct NrT<DT_F16> { typedef _Float16 S; static constexpr int V = 8; };
+template <> struct NrT<DT_BF16> { typedef __bf16 S; static constexpr int V = 8; };
+
+inline int nr_status()
+{
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? BC_OK : (int)e;
+}
+
+struct NormArgs {
+    const void *h, *y;                          // (M, C), rows ldh / ldy apart; y NULL: no block, h' = h (not stored)
+    const void *wo, *bo, *gate, *wi, *bi;       // NULL: ones / zeros; fp32 or the tensors' type (pf32)
+    void *ho, *u;
+    float *stats;                               // [M][4]: mean, 1 / deviation of y; mean, 1 / deviation of h' (backward)
+    const void *gh, *gu;                        // gradients of h' and u (NULL: zeros)
+    void *dh, *dy;
+    float *part;                                // [workgroups][5][C]: column sums of gate, wo, bo, wi, bi
+    long long ldh, ldy, ldgh, ldgu;
+    int M, C, g_log, rows_per_gate, span, chunks;
+    int out_kind, in_kind, pf32, need_dh, need_dy;
+    float alpha, eps;
+};
+
+// ---- sums over the G lanes of a row; every lane of the row gets the same bits
+template <int CTRL> __device__ __forceinline__ float nr_dpp(float v)
+{
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+
+__device__ __forceinline__ float nr_wave_sum(float v, int g_log)
+{
+    if (g_log > 0) v = nr_dpp<0xB1>(v);         // quad_perm 1 0 3 2
+    if (g_log > 1) v = nr_dpp<0x4E>(v);         // quad_perm 2 3 0 1
+    if (g_log > 2) v = nr_dpp<0x141>(v);        // row_half_mirror
+    if (g_log > 3) v = nr_dpp<0x140>(v);        // row_mirror
+    if (g_log > 4) v += __shfl_xor(v, 16);
+    if (g_log > 5) v += __shfl_xor(v, 32);
+    return v;
+}
+
+// WPR waves share a row: the waves' sums meet in `red` (two halves used in turn, so one barrier per exchange is enough)
+template <int WPR, int NW> struct NrSum {
+    float *red;         // [2][NW][2]
+    int turn, wave, g_log;
+    __device__ __forceinline__ void operator()(float &a, float &b, bool two)
+    {
+        a = nr_wave_sum(a, g_log);
+        if (two) b = nr_wave_sum(b, g_log);
+        if constexpr (WPR > 1) {
+            float *r = red + turn * (2 * NW);
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) {
+                r[2 * wave] = a;
+                r[2 * wave + 1] = b;
+            }
+            __syncthreads();
+            const float *q = r + 2 * (wave / WPR * WPR);
+            float sa = 0.f, sb = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) {
+                sa += q[2 * w];
+                sb += q[2 * w + 1];
+            }
+            a = sa;
+            b = sb;
+        }
+    }
+};
+
+// `cnt` of V elements at column `at` of row `base` (in elements).  With the base in scalar registers (whole waves share a row) a lane's address
+// is one 32-bit offset.  Rows of any width and start: the 16-byte accesses ask for the alignment of an element only (the hardware takes
+// unaligned vectors), the last vector of a row goes element by element.
+template <typename S, int V> __device__ __forceinline__ void nr_load(float *f, const void *q, size_t base, unsigned at, int cnt)
+{
+    typedef S SV __attribute__((ext_vector_type(V), aligned(sizeof(S))));
+    const S *p = (const S *)q + base + at;
+    if (cnt >= V) {
+        const SV v = *(const SV *)p;
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = (float)v[e];
+    } else
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = e < cnt ? (float)p[e] : 0.f;
+}
+
+template <typename S, int V> __device__ __forceinline__ void nr_store(void *q, size_t base, unsigned at, int cnt, const float *f)
+{
+    typedef S SV __attribute__((ext_vector_type(V), aligned(sizeof(S))));
+    S *p = (S *)q + base + at;
+    if (cnt >= V) {
+        SV v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = (S)f[e];
+        *(SV *)p = v;
+    } else
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (e < cnt) p[e] = (S)f[e];
+}
+
+// per-channel parameters; `none` where the pointer is NULL
+template <typename S, int V> __device__ __forceinline__ void nr_param(float *f, const void *p, int pf32, size_t base, unsigned at, int cnt, float none)
+{
+    if (!p) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = none;
+    } else if (pf32) {
+        if constexpr (V == 8) {
+            nr_load<float, 4>(f, p, base, at, cnt);
+            nr_load<float, 4>(f + 4, p, base, at + 4, cnt - 4);
+        } else
+            nr_load<float, V>(f, p, base, at, cnt);
+    } else
+        nr_load<S, V>(f, p, base, at, cnt);
+}
+
+// x[E] -> normalised in place (0 behind the row's end); mean and 1 / deviation returned.  E = NV vectors of V
+template <int V, int NV, class Sum> __device__ __forceinline__ void nr_normalise(float *x, int kind, const int *cnt, float inv_c, float eps, Sum &sum, float &mean, float &rstd)
+{
+    float none = 0.f;
+    mean = 0.f;
+    if (kind == NORM_LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV * V; ++i) s += x[i];
+        sum(s, none, false);
+        mean = s * inv_c;
+#pragma unroll
+        for (int i = 0; i < NV * V; ++i) x[i] = i % V < cnt[i / V] ? x[i] - mean : 0.f;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV * V; ++i) q += x[i] * x[i];
+    sum(q, none, false);
+    rstd = 1.f / sqrtf(q * inv_c + eps);
+#pragma unroll
+    for (int i = 0; i < NV * V; ++i) x[i] *= rstd;
+}
+
+template <int DT, int V, int NV, int WPR>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const NormArgs a)
+{
+    typedef typename NrT<DT>::S S;
+    constexpr int NT = WPR > 4 ? 64 * WPR : 256, NW = NT / 64, E = V * NV;
+    __shared__ float red[4 * NW];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int G = WPR > 1 ? 64 * WPR : 1 << a.g_log, lr = WPR > 1 ? tid % (64 * WPR) : tid & (G - 1), RPB = NT / G;
+    const int slot = WPR > 1 ? wave / WPR : tid >> a.g_log;       // (a scalar where whole waves share a row)
+    const float inv_c = 1.f / (float)a.C;
+    NrSum<WPR, NW> sum = {red, 0, wave, a.g_log};
+    unsigned col[NV];
+    int cnt[NV];        // how many of a vector's channels exist
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        col[i] = (i * G + lr) * V;
+        cnt[i] = a.C - (int)col[i];
+    }
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.M; r0 += (long long)gridDim.x * RPB) {      // (uniform: every wave meets every barrier)
+        const long long row = r0 + slot;
+        const bool live = row < a.M;
+        const size_t gate_at = a.rows_per_gate ? (size_t)(row / a.rows_per_gate) * a.C : 0;
+        float x[E], w[V], b[V], mean_y = 0.f, rstd_y = 0.f, mean_h = 0.f, rstd_h = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = 0.f;
+        if (a.y) {
+            if (live)
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (cnt[i] > 0) nr_load<S, V>(x + i * V, a.y, (size_t)row * a.ldy, col[i], cnt[i]);
+            if (a.out_kind != NORM_NONE) {
+                nr_normalise<V, NV>(x, a.out_kind, cnt, inv_c, a.eps, sum, mean_y, rstd_y);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (cnt[i] > 0) {
+                        nr_param<S, V>(w, a.wo, a.pf32, 0, col[i], cnt[i], 1.f);
+                        nr_param<S, V>(b, a.bo, a.pf32, 0, col[i], cnt[i], 0.f);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) x[i * V + e] = x[i * V + e] * w[e] + b[e];
+                    }
+            }
+            if (live)
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (cnt[i] > 0) {
+                        nr_load<S, V>(b, a.h, (size_t)row * a.ldh, col[i], cnt[i]);
+                        nr_param<S, V>(w, a.gate, a.pf32, gate_at, col[i], cnt[i], 1.f);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) x[i * V + e] = a.alpha * b[e] + w[e] * x[i * V + e];
+                        nr_store<S, V>(a.ho, (size_t)row * a.C, col[i], cnt[i], x + i * V);
+                    }
+        } else if (live)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (cnt[i] > 0) nr_load<S, V>(x + i * V, a.h, (size_t)row * a.ldh, col[i], cnt[i]);
+        if (a.in_kind != NORM_NONE) {
+            nr_normalise<V, NV>(x, a.in_kind, cnt, inv_c, a.eps, sum, mean_h, rstd_h);
+            if (live)
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (cnt[i] > 0) {
+                        nr_param<S, V>(w, a.wi, a.pf32, 0, col[i], cnt[i], 1.f);
+                        nr_param<S, V>(b, a.bi, a.pf32, 0, col[i], cnt[i], 0.f);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) x[i * V + e] = x[i * V + e] * w[e] + b[e];
+                        nr_store<S, V>(a.u, (size_t)row * a.C, col[i], cnt[i], x + i * V);
+                    }
+        }
+        if (a.stats && live && lr == 0) *(float4 *)(a.stats + 4 * row) = float4{mean_y, rstd_y, mean_h, rstd_h};
+    }
+}
+
+// the five column sums of a workgroup: its rows' lanes with the same channels meet in the LDS, in the order of the rows' slots
+template <int V, int NV, int NT> __device__ __forceinline__ void nr_put_sums(float *lds, float *dst, const float *acc, const unsigned *col, const int *cnt, int tid, int G, int RPB)
+{
+    if (RPB == 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (cnt[i] > 0)
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < cnt[i]) dst[col[i] + e] = acc[i * V + e];
+        return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV * V; ++i) lds[i * NT + tid] = acc[i];
+    __syncthreads();
+    if (tid < G)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (cnt[i] > 0)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    float s = 0.f;
+                    for (int r = 0; r < RPB; ++r) s += lds[(i * V + e) * NT + r * G + tid];
+                    if (e < cnt[i]) dst[col[i] + e] = s;
+                }
+}
+
+template <int DT, int V, int NV, int WPR>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(const NormArgs a)
+{
+    typedef typename NrT<DT>::S S;
+    constexpr int NT = WPR > 4 ? 64 * WPR : 256, NW = NT / 64, E = V * NV;
+    __shared__ float red[4 * NW];
+    __shared__ float meet[WPR > 2 ? 1 : NT * E];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int G = WPR > 1 ? 64 * WPR : 1 << a.g_log, lr = WPR > 1 ? tid % (64 * WPR) : tid & (G - 1), RPB = NT / G;
+    const int slot = WPR > 1 ? wave / WPR : tid >> a.g_log;       // (a scalar where whole waves share a row)
+    const float inv_c = 1.f / (float)a.C;
+    NrSum<WPR, NW> sum = {red, 0, wave, a.g_log};
+    unsigned col[NV];
+    int cnt[NV];        // how many of a vector's channels exist
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        col[i] = (i * G + lr) * V;
+        cnt[i] = a.C - (int)col[i];
+    }
+    // workgroup b: chunk b % chunks of the rows of gate group b / chunks
+    const int group = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x % a.chunks;
+    const int per_group = a.rows_per_gate ? a.rows_per_gate : a.M;
+    const long long base = (long long)group * per_group;
+    const int first = chunk * a.span, last = per_group - first < a.span ? per_group : first + a.span;
+    const size_t gate_at = a.rows_per_gate ? (size_t)group * a.C : 0;
+
+    float s_gate[E], s_wo[E], s_bo[E], s_wi[E], s_bi[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) s_gate[i] = s_wo[i] = s_bo[i] = s_wi[i] = s_bi[i] = 0.f;
+
+    for (int r0 = first; r0 < last; r0 += RPB) {
+        const bool live = r0 + slot < last;
+        const long long row = base + r0 + slot;
+        float n[E], g[E], p[E], w[V], b[V];      // normalised y; normalised h', then the gradient of h'; working row
+        float4 st = {0.f, 0.f, 0.f, 0.f};
+        if (live) st = *(const float4 *)(a.stats + 4 * row);
+#pragma unroll
+        for (int i = 0; i < E; ++i) n[i] = g[i] = p[i] = 0.f;
+        if (live)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (cnt[i] > 0) {
+                    if (a.gh) nr_load<S, V>(g + i * V, a.gh, (size_t)row * a.ldgh, col[i], cnt[i]);
+                    if (a.y) nr_load<S, V>(n + i * V, a.y, (size_t)row * a.ldy, col[i], cnt[i]);
+                }
+        if (a.out_kind != NORM_NONE)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) n[i * V + e] = live && e < cnt[i] ? (n[i * V + e] - st.x) * st.y : 0.f;
+        if (a.in_kind != NORM_NONE) {
+            float hn[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) hn[i] = 0.f;
+            if (live)
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (cnt[i] > 0) {
+                        nr_load<S, V>(hn + i * V, a.h, (size_t)row * a.ldh, col[i], cnt[i]);
+                        if (a.y) {
+                            float t[V];
+                            nr_param<S, V>(w, a.wo, a.pf32, 0, col[i], cnt[i], 1.f);
+                            nr_param<S, V>(b, a.bo, a.pf32, 0, col[i], cnt[i], 0.f);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) t[e] = n[i * V + e] * w[e] + b[e];
+                            nr_param<S, V>(w, a.gate, a.pf32, gate_at, col[i], cnt[i], 1.f);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) hn[i * V + e] = a.alpha * hn[i * V + e] + w[e] * t[e];
+                        }
+                        if (a.gu) nr_load<S, V>(p + i * V, a.gu, (size_t)row * a.ldgu, col[i], cnt[i]);
+                        nr_param<S, V>(w, a.wi, a.pf32, 0, col[i], cnt[i], 1.f);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const int k = i * V + e;
+                            hn[k] = e < cnt[i] ? (hn[k] - st.z) * st.w : 0.f;
+                            s_wi[k] += p[k] * hn[k];
+                            s_bi[k] += p[k];
+                            p[k] *= w[e];
+                        }
+                    }
+            float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                m1 += p[i] * hn[i];
+                m2 += p[i];
+            }
+            sum(m1, m2, a.in_kind == NORM_LAYER);
+            m1 *= inv_c;
+            m2 = a.in_kind == NORM_LAYER ? m2 * inv_c : 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) g[i] += st.w * (p[i] - m2 - hn[i] * m1);
+        }
+        if (a.need_dh && live)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (cnt[i] > 0) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) b[e] = a.alpha * g[i * V + e];
+                    nr_store<S, V>(a.dh, (size_t)row * a.C, col[i], cnt[i], b);
+                }
+        if (!a.y) continue;
+        float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (cnt[i] > 0 && live) {
+                float t[V];
+                nr_param<S, V>(w, a.wo, a.pf32, 0, col[i], cnt[i], 1.f);
+                nr_param<S, V>(b, a.bo, a.pf32, 0, col[i], cnt[i], 0.f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) t[e] = n[i * V + e] * w[e] + b[e];
+                nr_param<S, V>(b, a.gate, a.pf32, gate_at, col[i], cnt[i], 1.f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const int k = i * V + e;
+                    s_gate[k] += g[k] * t[e];
+                    const float q = g[k] * b[e];
+                    s_wo[k] += q * n[k];
+                    s_bo[k] += q;
+                    p[k] = q * w[e];
+                    m1 += p[k] * n[k];
+                    m2 += p[k];
+                }
+            }
+        if (a.out_kind != NORM_NONE) {
+            sum(m1, m2, a.out_kind == NORM_LAYER);
+            m1 *= inv_c;
+            m2 = a.out_kind == NORM_LAYER ? m2 * inv_c : 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) p[i] = st.y * (p[i] - m2 - n[i] * m1);
+        }
+        if (a.need_dy && live)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (cnt[i] > 0) nr_store<S, V>(a.dy, (size_t)row * a.C, col[i], cnt[i], p + i * V);
+    }
+    if (!a.part) return;
+    float *dst = a.part + (size_t)blockIdx.x * 5 * a.C;
+    if (a.y) {
+        nr_put_sums<V, NV, NT>(meet, dst, s_gate, col, cnt, tid, G, RPB);
+        nr_put_sums<V, NV, NT>(meet, dst + a.C, s_wo, col, cnt, tid, G, RPB);
+        nr_put_sums<V, NV, NT>(meet, dst + 2 * (size_t)a.C, s_bo, col, cnt, tid, G, RPB);
+    }
+    nr_put_sums<V, NV, NT>(meet, dst + 3 * (size_t)a.C, s_wi, col, cnt, tid, G, RPB);
+    nr_put_sums<V, NV, NT>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, tid, G, RPB);
+}
+
+// column sums of the workgroups: 16 columns x 16 runs of workgroups per launch block, joined in a fixed order.  blockIdx.y: which of the five
+// (the gate's sums run over its own group's workgroups, blockIdx.z)
+struct NormJoin {
+    const float *part;
+    void *out[5];
+    int C, blocks, chunks, groups, f32;
+};
+
+template <int DT> __global__ __launch_bounds__(256) void k_norm_join(const NormJoin a)
+{
+    typedef typename NrT<DT>::S S;
+    __shared__ float red[256];
+    const int which = blockIdx.y, c = (int)blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
+    if (!a.out[which] || (which > 0 && blockIdx.z > 0)) return;
+    const bool per_group = which == 0;
+    const int b0 = per_group ? (int)blockIdx.z * a.chunks : 0, nb = per_group ? a.chunks : a.blocks;
+    float s = 0.f;
+    if (c < a.C)
+        for (int b = run; b < nb; b += 16) s += a.part[((size_t)(b0 + b) * 5 + which) * a.C + c];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (run == 0 && c < a.C) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t += red[16 * r + threadIdx.x];
+        const size_t at = (per_group ? (size_t)blockIdx.z * a.C : 0) + c;
+        if (a.f32) ((float *)a.out[which])[at] = t;
+        else ((S *)a.out[which])[at] = (S)t;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ host side
+constexpr int NR_MAX_C = 16384;
+
+struct NormShape { int E, WPR, g_log; };
+
+// lanes per row so that a lane owns eight channels (sixteen beyond 8192)
+NormShape nr_shape(int C)
+{
+    NormShape s = {8, 1, 0};
+    while (s.WPR < 16 && 64 * s.WPR * s.E < C) s.WPR *= 2;
+    if (64 * s.WPR * s.E < C) s.E = 16;
+    while (s.g_log < 6 && (s.E << s.g_log) < C) ++s.g_log;
+    return s;
+}
+
+inline int nr_rows_per_block(const NormShape &s) { return s.WPR > 1 ? (s.WPR > 4 ? 1 : 4 / s.WPR) : 256 >> s.g_log; }
+
+template <int DT, int V, int NV> int nr_go(bool bwd, const NormArgs &a, int wpr, unsigned grid, hipStream_t st)
+{
+#define NR_GO(W)                                                                                       \
+    if (wpr == W) {                                                                                    \
+        if (bwd) k_norm_bwd<DT, V, NV, W><<<grid, W > 4 ? 64 * W : 256, 0, st>>>(a);                   \
+        else k_norm_fwd<DT, V, NV, W><<<grid, W > 4 ? 64 * W : 256, 0, st>>>(a);                       \
+        return nr_status();                                                                            \
+    }
+    if constexpr (V * NV == 8) {
+        NR_GO(1)
+        NR_GO(2)
+        NR_GO(4)
+        NR_GO(8)
+    }
+    NR_GO(16)
+#undef NR_GO
+    return BC_ERR_SHAPE;
+}
+
+template <int DT> int nr_launch(bool bwd, const NormArgs &a, const NormShape &s, unsigned grid, hipStream_t st)
+{
+    constexpr int V = NrT<DT>::V;
+    return s.E == 8 ? nr_go<DT, V, 8 / V>(bwd, a, s.WPR, grid, st) : nr_go<DT, V, 16 / V>(bwd, a, s.WPR, grid, st);
+}
+
+int nr_dispatch(int dtype, bool bwd, const NormArgs &a, const NormShape &s, unsigned grid, hipStream_t st)
+{
+    switch (dtype) {
+    case DT_F32: return nr_launch<DT_F32>(bwd, a, s, grid, st);
+    case DT_F16: return nr_launch<DT_F16>(bwd, a, s, grid, st);
+    default: return nr_launch<DT_BF16>(bwd, a, s, grid, st);
+    }
+}
+
+inline int nr_esize(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+
+int nr_check(long long M, int C, int dtype, int out_kind, int in_kind, long long rows_per_gate, const void *gate, const void *y)
+{
+    if (dtype < 0 || dtype > 2) return BC_ERR_ELEM;
+    if (M < 0 || C < 1 || C > NR_MAX_C || out_kind < 0 || out_kind > 2 || in_kind < 0 || in_kind > 2) return BC_ERR_SHAPE;
+    if (M > 0x7fffffffll) return BC_ERR_RANGE;
+    if (rows_per_gate < 0 || (rows_per_gate && (!gate || M % rows_per_gate))) return BC_ERR_SHAPE;
+    if (!y && (out_kind != NORM_NONE || gate || in_kind == NORM_NONE)) return BC_ERR_SHAPE;
+    return BC_OK;
+}
+
+// about two workgroups per CU, the rows of a gate group divided evenly among whole workgroups
+struct NormChunks { int chunks, span, groups; };
+NormChunks nr_chunks(long long M, long long rows_per_gate, int rows_per_block)
+{
+    NormChunks c;
+    const long long per = rows_per_gate ? rows_per_gate : M;
+    c.groups = (int)(M / per);
+    long long n = (512 + c.groups - 1) / c.groups;
+    const long long most = (per + rows_per_block - 1) / rows_per_block;
+    if (n > most) n = most;
+    long long span = (per + n - 1) / n;
+    span = (span + rows_per_block - 1) / rows_per_block * rows_per_block;
+    c.span = (int)span;
+    c.chunks = (int)((per + span - 1) / span);
+    return c;
+}
+
+}  // namespace
+
+BC_EXPORT int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const void *h, const void *y, const void *out_weight, const void *out_bias, const void *gate,
+                                   const void *in_weight, const void *in_bias, long long M, int C, long long ldh, long long ldy, long long rows_per_gate, float residual_scale,
+                                   float eps, int out_kind, int in_kind, int dtype, int params_f32, void *stream)
+{
+    const int rc = nr_check(M, C, dtype, out_kind, in_kind, rows_per_gate, gate, y);
+    if (rc != BC_OK) return rc;
+    if (ldh < C || (y && ldy < C)) return BC_ERR_SHAPE;
+    if (M == 0) return BC_OK;
+    if (!h || (y && !h_out) || (in_kind != NORM_NONE && !u)) return BC_ERR_NULL;
+    const int e = nr_esize(dtype), pe = params_f32 ? 4 : e;
+    const void *ts[] = {h, y, h_out, u}, *ps[] = {out_weight, out_bias, gate, in_weight, in_bias};
+    for (int i = 0; i < 4; ++i)
+        if (ts[i] && (uintptr_t)ts[i] % e) return BC_ERR_ALIGN;
+    for (int i = 0; i < 5; ++i)
+        if (ps[i] && (uintptr_t)ps[i] % pe) return BC_ERR_ALIGN;
+    if (stats && (uintptr_t)stats % 16) return BC_ERR_ALIGN;
+    NormArgs a = {};
+    a.h = h; a.y = y; a.wo = out_weight; a.bo = out_bias; a.gate = gate; a.wi = in_weight; a.bi = in_bias;
+    a.ho = h_out; a.u = u; a.stats = stats;
+    a.ldh = ldh; a.ldy = ldy; a.M = (int)M; a.C = C; a.rows_per_gate = (int)rows_per_gate;
+    a.out_kind = out_kind; a.in_kind = in_kind; a.pf32 = params_f32; a.alpha = residual_scale; a.eps = eps;
+    const NormShape s = nr_shape(C);
+    a.g_log = s.g_log;
+    const long long blocks = (M + nr_rows_per_block(s) - 1) / nr_rows_per_block(s);
+    return nr_dispatch(dtype, false, a, s, (unsigned)(blocks < 8192 ? blocks : 8192), (hipStream_t)stream);
+}
+
+BC_EXPORT long long bc_norm_residual_bwd_workspace(long long M, int C, long long rows_per_gate, int dtype)
+{
+    if (M < 1 || C < 1 || C > NR_MAX_C || dtype < 0 || dtype > 2 || rows_per_gate < 0 || (rows_per_gate && M % rows_per_gate)) return 0;
+    const NormChunks c = nr_chunks(M, rows_per_gate, nr_rows_per_block(nr_shape(C)));
+    return 20ll * C * c.chunks * c.groups;
+}
+
+BC_EXPORT int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void *d_out_bias, void *d_gate, void *d_in_weight, void *d_in_bias, const void *gh, const void *gu,
+                                   const float *stats, const void *h, const void *y, const void *out_weight, const void *out_bias, const void *gate, const void *in_weight,
+                                   long long M, int C, long long ldh, long long ldy, long long ldgh, long long ldgu, long long rows_per_gate, float residual_scale, int out_kind,
+                                   int in_kind, int dtype, int params_f32, void *workspace, long long workspace_bytes, void *stream)
+{
+    const int rc = nr_check(M, C, dtype, out_kind, in_kind, rows_per_gate, gate, y);
+    if (rc != BC_OK) return rc;
+    if (ldh < C || (y && ldy < C) || (gh && ldgh < C) || (gu && ldgu < C) || M == 0) return BC_ERR_SHAPE;
+    if (!h || !stats || (dy && !y)) return BC_ERR_NULL;
+    const int e = nr_esize(dtype), pe = params_f32 ? 4 : e;
+    const void *ts[] = {h, y, gh, gu, dh, dy}, *ps[] = {out_weight, out_bias, gate, in_weight, d_out_weight, d_out_bias, d_gate, d_in_weight, d_in_bias};
+    for (int i = 0; i < 6; ++i)
+        if (ts[i] && (uintptr_t)ts[i] % e) return BC_ERR_ALIGN;
+    for (int i = 0; i < 9; ++i)
+        if (ps[i] && (uintptr_t)ps[i] % pe) return BC_ERR_ALIGN;
+    if ((uintptr_t)stats % 16) return BC_ERR_ALIGN;
+    const NormShape s = nr_shape(C);
+    const NormChunks c = nr_chunks(M, rows_per_gate, nr_rows_per_block(s));
+    const bool sums = d_out_weight || d_out_bias || d_gate || d_in_weight || d_in_bias;
+    if (sums && !workspace) return BC_ERR_NULL;
+    if (sums && workspace_bytes < 20ll * C * c.chunks * c.groups) return BC_ERR_SHAPE;
+    if (sums && (uintptr_t)workspace % 4) return BC_ERR_ALIGN;
+    NormArgs a = {};
+    a.h = h; a.y = y; a.wo = out_weight; a.bo = out_bias; a.gate = gate; a.wi = in_weight;
+    a.stats = (float *)stats; a.gh = gh; a.gu = gu; a.dh = dh; a.dy = dy; a.part = sums ? (float *)workspace : nullptr;
+    a.ldh = ldh; a.ldy = ldy; a.ldgh = ldgh; a.ldgu = ldgu; a.M = (int)M; a.C = C; a.rows_per_gate = (int)rows_per_gate;
+    a.out_kind = out_kind; a.in_kind = in_kind; a.pf32 = params_f32; a.alpha = residual_scale;
+    a.need_dh = dh != nullptr; a.need_dy = dy != nullptr;
+    a.g_log = s.g_log; a.span = c.span; a.chunks = c.chunks;
+    const int r = nr_dispatch(dtype, true, a, s, (unsigned)(c.chunks * c.groups), (hipStream_t)stream);
+    if (r != BC_OK || !sums) return r;
+    NormJoin j = {};
+    j.part = (const float *)workspace;
+    j.out[0] = d_gate; j.out[1] = d_out_weight; j.out[2] = d_out_bias; j.out[3] = d_in_weight; j.out[4] = d_in_bias;
+    j.C = C; j.blocks = c.chunks * c.groups; j.chunks = c.chunks; j.groups = c.groups; j.f32 = params_f32;
+    const dim3 grid((unsigned)((C + 15) / 16), 5, (unsigned)c.groups);
+    switch (dtype) {
+    case DT_F32: k_norm_join<DT_F32><<<grid, 256, 0, (hipStream_t)stream>>>(j); break;
+    case DT_F16: k_norm_join<DT_F16><<<grid, 256, 0, (hipStream_t)stream>>>(j); break;
+    default: k_norm_join<DT_BF16><<<grid, 256, 0, (hipStream_t)stream>>>(j);
+    }
+    return nr_status();
+}

@@ -605,6 +605,44 @@ int bc_pn_set_stamps(void *buf);
 int bc_pn_features_nhwc(float *out, int N, int h, int w, int Cpad, const void *const *ptrs, const long long *strides, const int *dims,
                         const float *scales, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * B3. Channel operators: products and norms over rows of features (a row = one pixel of a channels-last map, or one token).  Additions for
+ * models built of them, forward and backward; blockcopy/utils/channel_ops.py is the torch side (csrc/linear.hip, csrc/norm_residual.hip).
+ * dtype BC_F32 / BC_F16 / BC_BF16 of every matrix; matrices are row-major with unit feature stride and ld* elements between rows (outputs and
+ * z contiguous); pointers aligned to an element.  Sums, statistics and activations in fp32; results run-to-run identical (no atomics).
+ * M = 0 forward: nothing is launched; backward: BC_ERR_SHAPE (the gradients are zeros, the caller's own).
+ * Workspaces: at least the bytes the query returns for the same sizes, 256-byte aligned, free again when the call's work on `stream` is done.
+ * ------------------------------------------------------------------------------------------- */
+
+/* y[m][n] = act(z[m][n]) + residual[m][n],  z[m][n] = sum_k x[m][k] w[n][k] + bias[n].  x (M, K), w (N, K), y and residual (M, N); bias, residual and
+ * z may be NULL; bias in fp32 (bias_f32) or dtype; act 0 none, 1 relu, 2 gelu (erf), 3 gelu (tanh), 4 silu.  z: the pre-activations rounded to dtype,
+ * which the backward pass of an activation needs. */
+int bc_linear_fwd(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, long long M, int N, int K, long long ldx,
+                  long long ldw, long long ldr, int act, int dtype, int bias_f32, void *workspace, long long workspace_bytes, void *stream);
+long long bc_linear_fwd_workspace(long long M, int N, int K, int dtype);
+/* gradients for gy = d loss / d y (the residual's gradient is gy itself): dz = gy * act'(z), dx (M, K) = dz w, dw (N, K) = dz^T x, db (N) = column sums
+ * of dz (fp32 sums, taken before dz is rounded to dtype; stored in fp32 if bias_f32).  dx, dw, db may each be NULL; z only with an activation,
+ * w only for dx, x only for dw. */
+int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const void *z, const void *x, const void *w, long long M, int N, int K, long long ldg,
+                  long long ldx, long long ldw, int act, int dtype, int bias_f32, void *workspace, long long workspace_bytes, void *stream);
+long long bc_linear_bwd_workspace(long long M, int N, int K, int act, int dtype);
+
+/* h_out = residual_scale * h + gate * t,  t = N_out(y) * out_weight + out_bias;  u = N_in(h_out) * in_weight + in_bias, over the C <= 16384 features of a
+ * row.  N (kinds): 0 none, 1 x / sqrt(mean(x^2) + eps), 2 (x - mean) / sqrt(mean((x - mean)^2) + eps).  y NULL: no block yet (out_kind 0, no gate; h_out is h,
+ * not stored).  in_kind 0: no u.  Parameters NULL = ones / zeros, all fp32 (params_f32) or all dtype; gate (C), or (M / rows_per_gate, C) with
+ * rows_per_gate > 0: row m takes gate row m / rows_per_gate.  u is formed from h_out before its rounding.  stats (M, 4) fp32, 16-byte aligned:
+ * {mean, 1 / deviation} of y and of h_out for the backward pass (NULL: not kept). */
+int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const void *h, const void *y, const void *out_weight, const void *out_bias, const void *gate,
+                         const void *in_weight, const void *in_bias, long long M, int C, long long ldh, long long ldy, long long rows_per_gate, float residual_scale,
+                         float eps, int out_kind, int in_kind, int dtype, int params_f32, void *stream);
+/* gradients of the above out of gh, gu = d loss / d h_out, d u (NULL: zeros), the forward's inputs and its stats; every output may be NULL, parameter
+ * gradients have their parameter's shape and type.  workspace: only if a parameter's gradient is asked for. */
+int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void *d_out_bias, void *d_gate, void *d_in_weight, void *d_in_bias, const void *gh, const void *gu,
+                         const float *stats, const void *h, const void *y, const void *out_weight, const void *out_bias, const void *gate, const void *in_weight,
+                         long long M, int C, long long ldh, long long ldy, long long ldgh, long long ldgu, long long rows_per_gate, float residual_scale, int out_kind,
+                         int in_kind, int dtype, int params_f32, void *workspace, long long workspace_bytes, void *stream);
+long long bc_norm_residual_bwd_workspace(long long M, int C, long long rows_per_gate, int dtype);
+
 /* tuning / A-B knob (measurement infrastructure; defaults are the shipped behaviour): key in
  *   "conv_impl"      1 = first-generation fused conv kernel, 2 = CU-balanced kernel (default)
  *   "conv2_cfg"      -1 = choose the decomposition per launch (default), 0..15 = force one (BC_ERR_SHAPE at launch if it does not fit)
