@@ -81,14 +81,13 @@ struct LinEpi {
     void *y, *z;                // z: the pre-activations in the tensors' type (NULL: not kept)
     const void *bias, *res;
     long long ldr;
-    int bias_f32, act, vec;     // vec: four consecutive outputs may move as one vector
+    int bias_f32, act;
 };
 
 struct LinArgs {
     LinOperand a, b;            // a: the operand of the output's columns (n), b: of its rows (m)
     int M, N, K;
     int kspan;                  // summed indexes of one slice (a multiple of BK): slice s takes [s kspan, (s + 1) kspan)
-    int vec_a, vec_b;           // 16-byte vectors never straddle a row's end and are aligned
     unsigned tiles_m, tiles_n;
     float *part;                // [slices][M][N] sums of the slices, or NULL: one slice, epilogue in place
     LinEpi ep;
@@ -144,64 +143,104 @@ template <int DT, bool MC, int R> __device__ __forceinline__ uint4 lin_frag(cons
     }
 }
 
-// 16 bytes of an operand starting at (row, k); elements outside the matrix (or the slice, k >= kend) are zero
-template <int DT, bool MC> __device__ __forceinline__ uint4 lin_fetch(const LinOperand &o, int vec, int rows, int kend, int row, int k)
+// 16 bytes of an operand starting at (row, k); elements outside the matrix (or the slice, k >= kend) are zero.  The vector asks for the
+// alignment of an element only (the hardware takes unaligned vectors): rows may start anywhere
+template <int DT, bool MC> __device__ __forceinline__ uint4 lin_fetch(const LinOperand &o, int rows, int kend, int row, int k)
 {
     constexpr int V = LinT<DT>::V;
     typedef typename LinT<DT>::S S;
+    typedef S SV __attribute__((ext_vector_type(V), aligned(sizeof(S))));
     const int run = MC ? row : k, run_end = MC ? rows : kend;       // the index that memory runs along
-    if (MC ? k >= kend : row >= rows) return uint4{0u, 0u, 0u, 0u};
+    if ((MC ? k >= kend : row >= rows) || run >= run_end) return uint4{0u, 0u, 0u, 0u};
     const S *p = (const S *)o.p + (MC ? (size_t)k * o.ld + row : (size_t)row * o.ld + k);
-    if (vec && run + V <= run_end) return *(const uint4 *)p;
-    union { S s[V]; uint4 v; } u;
-    u.v = uint4{0u, 0u, 0u, 0u};
+    SV v;
+    if (run + V <= run_end) v = *(const SV *)p;
+    else
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-        if (run + e < run_end) u.s[e] = p[e];
-    return u.v;
+        for (int e = 0; e < V; ++e) v[e] = run + e < run_end ? p[e] : (S)0.f;
+    return __builtin_bit_cast(uint4, v);
 }
 
-template <int DT> __device__ __forceinline__ float lin_bias(const LinEpi &ep, int n)
+// W consecutive elements, of which `cnt` exist (the vector asks for the alignment of an element only)
+template <typename S, int W> __device__ __forceinline__ void lin_load(float *f, const S *p, int cnt)
 {
-    typedef typename LinT<DT>::S S;
-    return ep.bias ? (ep.bias_f32 ? ((const float *)ep.bias)[n] : (float)((const S *)ep.bias)[n]) : 0.f;
+    typedef S SW __attribute__((ext_vector_type(W), aligned(sizeof(S))));
+    if (cnt >= W) {
+        const SW v = *(const SW *)p;
+#pragma unroll
+        for (int e = 0; e < W; ++e) f[e] = (float)v[e];
+    } else
+#pragma unroll
+        for (int e = 0; e < W; ++e) f[e] = e < cnt ? (float)p[e] : 0.f;
 }
 
-// four consecutive outputs (m, n .. n + 3) out of fp32 sums
-template <int DT> __device__ __forceinline__ void lin_store4(const LinEpi &ep, int N, int m, int n, const float *v)
+template <typename S, int W> __device__ __forceinline__ void lin_save(S *p, const float *f, int cnt)
+{
+    typedef S SW __attribute__((ext_vector_type(W), aligned(sizeof(S))));
+    if (cnt >= W) {
+        SW v;
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] = (S)f[e];
+        *(SW *)p = v;
+    } else
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (e < cnt) p[e] = (S)f[e];
+}
+
+// 16 bytes' worth of consecutive outputs (m, n ..), cnt of them inside the matrix: sums v -> z, y
+template <int DT> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v)
 {
     typedef typename LinT<DT>::S S;
-    typedef S S4 __attribute__((ext_vector_type(4)));
+    constexpr int W = LinT<DT>::V;
+    const int cnt = N - n;
     const size_t at = (size_t)m * N + n;
-    S4 y, z, r;
-    if (ep.vec) {
-        if (ep.res) r = *(const S4 *)((const S *)ep.res + (size_t)m * ep.ldr + n);
+    float t[W];
+    if (ep.bias) {
+        if (ep.bias_f32) lin_load<float, W>(t, (const float *)ep.bias + n, cnt);
+        else lin_load<S, W>(t, (const S *)ep.bias + n, cnt);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float t = v[e] + lin_bias<DT>(ep, n + e);
-            z[e] = (S)t;
-            y[e] = (S)(lin_act(t, ep.act) + (ep.res ? (float)r[e] : 0.f));
-        }
-        if (ep.z) *(S4 *)((S *)ep.z + at) = z;
-        *(S4 *)((S *)ep.y + at) = y;
-        return;
+        for (int e = 0; e < W; ++e) v[e] += t[e];
     }
+    if (ep.z) lin_save<S, W>((S *)ep.z + at, v, cnt);
+    if (ep.act != ACT_NONE)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (n + e < N) {
-            const float t = v[e] + lin_bias<DT>(ep, n + e);
-            if (ep.z) ((S *)ep.z)[at + e] = (S)t;
-            ((S *)ep.y)[at + e] = (S)(lin_act(t, ep.act) + (ep.res ? (float)((const S *)ep.res)[(size_t)m * ep.ldr + n + e] : 0.f));
-        }
+        for (int e = 0; e < W; ++e) v[e] = lin_act(v[e], ep.act);
+    if (ep.res) {
+        lin_load<S, W>(t, (const S *)ep.res + (size_t)m * ep.ldr + n, cnt);
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] += t[e];
+    }
+    lin_save<S, W>((S *)ep.y + at, v, cnt);
+}
+
+// ---- direct copies global -> LDS.  A wave moves 64 x 16 bytes per instruction: lane l's bytes land at lds + 16 l, its source is base + off, so
+// an image's exchanged vector order is made by the lanes' source offsets.  The descriptor is a plain range of bytes (no stride, no limit:
+// every offset that is used lies inside the matrix).  Written in assembly because the compiler waits for all outstanding copies before any
+// LDS read once it sees one; the kernel waits itself (lin_arrived), and there is no register that a copy in flight could overwrite.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void lin_copy16(const void *base, unsigned off, unsigned lds)
+{
+    const unsigned long long b = (unsigned long long)base;
+    const i32x4 r = {(int)(unsigned)b, (int)(unsigned)(b >> 32) & 0xffff, -1, 0x00027000};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(off), "s"(r) : "memory", "m0");
+}
+
+// everything this wave copied is in the LDS and everything it read from there in registers, then all waves meet
+__device__ __forceinline__ void lin_meet()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
 }
 
 // out[m][n] = sum_k A(n, k) B(m, k).  A workgroup of WM x WN waves owns a BM x BN tile; the column operand is the matrix instruction's first
-// one, so a lane ends up with four consecutive columns of one row.  Operands go through registers into a double-buffered LDS image: the
-// loads of step t + 1 are requested before the products of step t and stored behind them, one barrier per step.
-template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC>
+// one, so a lane ends up with four consecutive columns of one row.  Two LDS images: while step t is multiplied, step t + 1 travels into the
+// other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel global -> LDS without registers (a partial last step
+// goes through registers, zero-filled); otherwise through registers, requested before the products and stored behind them.
+template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
 {
-    constexpr int V = LinT<DT>::V, BK = LinT<DT>::BK, NT = 64 * WM * WN;
+    constexpr int V = LinT<DT>::V, BK = LinT<DT>::BK, NT = 64 * WM * WN, ES = 16 / V;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int NA = BN * 8 / NT, NB = BM * 8 / NT;       // vectors per thread and step
     constexpr int IMG = (BM + BN) * 8;
@@ -219,14 +258,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
             const int v = tid + NT * i;
-            if constexpr (AMC) ra[i] = lin_fetch<DT, true>(g.a, g.vec_a, g.N, kend, n0 + v % (BN / V) * V, k0 + v / (BN / V));
-            else ra[i] = lin_fetch<DT, false>(g.a, g.vec_a, g.N, kend, n0 + (v >> 3), k0 + (v & 7) * V);
+            if constexpr (AMC) ra[i] = lin_fetch<DT, true>(g.a, g.N, kend, n0 + v % (BN / V) * V, k0 + v / (BN / V));
+            else ra[i] = lin_fetch<DT, false>(g.a, g.N, kend, n0 + (v >> 3), k0 + (v & 7) * V);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int v = tid + NT * i;
-            if constexpr (BMC) rb[i] = lin_fetch<DT, true>(g.b, g.vec_b, g.M, kend, m0 + v % (BM / V) * V, k0 + v / (BM / V));
-            else rb[i] = lin_fetch<DT, false>(g.b, g.vec_b, g.M, kend, m0 + (v >> 3), k0 + (v & 7) * V);
+            if constexpr (BMC) rb[i] = lin_fetch<DT, true>(g.b, g.M, kend, m0 + v % (BM / V) * V, k0 + v / (BM / V));
+            else rb[i] = lin_fetch<DT, false>(g.b, g.M, kend, m0 + (v >> 3), k0 + (v & 7) * V);
         }
     };
     auto stage = [&](uint4 *img) {
@@ -244,21 +283,54 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
             else img[(v & ~7) + ((v & 7) ^ ((v >> 3) & 7))] = rb[i];
         }
     };
+    // direct copies: byte offsets of this lane's sources from the tile's corner of the step.  Rows behind the matrix take its last row
+    // (vector) -- their sums are never stored
+    unsigned oa[NA], ob[NB];
+    const char *pa = nullptr, *pb = nullptr;
+    const size_t stepa = AMC ? (size_t)BK * g.a.ld * ES : 128, stepb = BMC ? (size_t)BK * g.b.ld * ES : 128;
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int v = tid + NT * i;
+            if constexpr (AMC) {
+                const int k = v / (BN / V), c = (v % (BN / V)) ^ lin_swz<DT, BN>(k), n = n0 + c * V + V <= g.N ? c * V : g.N - V - n0;
+                oa[i] = (unsigned)((long long)k * g.a.ld + n) * ES;
+            } else {
+                const int row = n0 + (v >> 3) < g.N ? v >> 3 : g.N - 1 - n0;
+                oa[i] = (unsigned)((long long)row * g.a.ld) * ES + (unsigned)((v & 7) ^ ((v >> 3) & 7)) * 16;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int v = tid + NT * i;
+            if constexpr (BMC) {
+                const int k = v / (BM / V), c = (v % (BM / V)) ^ lin_swz<DT, BM>(k), m = m0 + c * V + V <= g.M ? c * V : g.M - V - m0;
+                ob[i] = (unsigned)((long long)k * g.b.ld + m) * ES;
+            } else {
+                const int row = m0 + (v >> 3) < g.M ? v >> 3 : g.M - 1 - m0;
+                ob[i] = (unsigned)((long long)row * g.b.ld) * ES + (unsigned)((v & 7) ^ ((v >> 3) & 7)) * 16;
+            }
+        }
+        pa = (const char *)g.a.p + ((AMC ? (size_t)kbeg * g.a.ld + n0 : (size_t)n0 * g.a.ld + kbeg)) * ES;
+        pb = (const char *)g.b.p + ((BMC ? (size_t)kbeg * g.b.ld + m0 : (size_t)m0 * g.b.ld + kbeg)) * ES;
+    }
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lin_lds;
+    auto copy = [&](int img) {      // the next step's operands into image `img`
+#pragma unroll
+        for (int i = 0; i < NA; ++i) lin_copy16(pa, oa[i], lds0 + (img * IMG + wave * 64 + NT * i) * 16);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) lin_copy16(pb, ob[i], lds0 + (img * IMG + BN * 8 + wave * 64 + NT * i) * 16);
+        pa += stepa;
+        pb += stepb;
+    };
 
     f32x4 acc[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    fetch(kbeg);
-    stage(lin_lds);
-    __syncthreads();
-    int cur = 0;
-    for (int k0 = kbeg; k0 < kend; k0 += BK) {
-        const bool more = k0 + BK < kend;
-        if (more) fetch(k0 + BK);
-        const uint4 *ia = lin_lds + cur * IMG, *ib = ia + BN * 8;
+    auto multiply = [&](const uint4 *ia) {
+        const uint4 *ib = ia + BN * 8;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             uint4 fa[FN], fb[FM];
@@ -271,53 +343,85 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
 #pragma unroll
                 for (int j = 0; j < FM; ++j) lin_mma<DT>(acc[i][j], fa[i], fb[j]);
         }
-        if (more) stage(lin_lds + (cur ^ 1) * IMG);
+    };
+
+    if constexpr (DIRECT) {
+        const int full = (kend - kbeg) / BK;
+        if (full > 0) copy(0);
+        for (int t = 0; t < full; ++t) {
+            lin_meet();
+            if (t + 1 < full) copy((t + 1) & 1);
+            multiply(lin_lds + (t & 1) * IMG);
+        }
+        if (kbeg + full * BK < kend) {
+            fetch(kbeg + full * BK);
+            stage(lin_lds + (full & 1) * IMG);      // (last read two steps ago, before the previous barrier)
+            __syncthreads();
+            multiply(lin_lds + (full & 1) * IMG);
+        }
+    } else {
+        fetch(kbeg);
+        stage(lin_lds);
         __syncthreads();
-        cur ^= 1;
+        int cur = 0;
+        for (int k0 = kbeg; k0 < kend; k0 += BK) {
+            const bool more = k0 + BK < kend;
+            if (more) fetch(k0 + BK);
+            multiply(lin_lds + cur * IMG);
+            if (more) stage(lin_lds + (cur ^ 1) * IMG);
+            __syncthreads();
+            cur ^= 1;
+        }
     }
 
+    // the sums meet their epilogue through the LDS: a wave lays 64 x 64 of them (16-byte vector c of row r at c ^ (r & 15)) into its own part of
+    // the images and takes them back row by row, so that every access to memory is a whole 16-byte vector
+    static_assert(BN / WN == 64 && BM / WM % 64 == 0 && WM * WN * 1024 <= 2 * IMG, "a wave owns 64 columns");
+    uint4 *own = lin_lds + wave * 1024;
+    constexpr int PER_ROW = 64 / V, RPI = 64 / PER_ROW;         // lanes per row, rows per round
+    const int n = n0 + wn * 64 + (lane % PER_ROW) * V;
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const int m = m0 + wm * (BM / WM) + 16 * j + (lane & 15);
-        if (m >= g.M) continue;
+    for (int h = 0; h < FM / 4; ++h) {
+        lin_meet();         // (h = 0: all waves have read the last step; otherwise the wave's own vectors are out)
 #pragma unroll
-        for (int i = 0; i < FN; ++i) {
-            const int n = n0 + wn * (BN / WN) + 16 * i + 4 * (lane >> 4);
-            if (n >= g.N) continue;
-            const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-            if (g.part) {
-                float *p = g.part + ((size_t)blockIdx.y * g.M + m) * g.N + n;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < g.N) p[e] = v[e];
-            } else
-                lin_store4<DT>(g.ep, g.N, m, n, v);
+            for (int i = 0; i < FN; ++i) own[(16 * j + (lane & 15)) * 16 + ((4 * i + (lane >> 4)) ^ (lane & 15))] = __builtin_bit_cast(uint4, acc[i][4 * h + j]);
+        lin_meet();
+        for (int r0 = 0; r0 < 64; r0 += RPI) {
+            const int r = r0 + lane / PER_ROW, m = m0 + wm * (BM / WM) + 64 * h + r;
+            if (m >= g.M || n >= g.N) continue;
+            float v[V];
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {
+                const f32x4 f = __builtin_bit_cast(f32x4, own[r * 16 + (((lane % PER_ROW) * (V / 4) + q) ^ (r & 15))]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = f[e];
+            }
+            if (g.part) lin_save<float, V>(g.part + ((size_t)blockIdx.y * g.M + m) * g.N + n, v, g.N - n);
+            else lin_epilogue<DT>(g.ep, g.N, m, n, v);
         }
     }
 }
 
-// sums of the slices in their order (run-to-run identical), then the epilogue: one thread per four outputs of a row
+// sums of the slices in their order (run-to-run identical), then the epilogue: one thread per 16 bytes of outputs
 template <int DT> __global__ __launch_bounds__(256) void k_lin_join(const float *part, int slices, int M, int N, LinEpi ep)
 {
-    const unsigned quads = ((unsigned)N + 3) / 4;
+    constexpr int W = LinT<DT>::V;
+    const unsigned units = ((unsigned)N + W - 1) / W;
     const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const size_t m = id / quads;
+    const size_t m = id / units;
     if (m >= (size_t)M) return;
-    const int n = (int)(id % quads) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const int n = (int)(id % units) * W;
+    float v[W], t[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = 0.f;
     for (int s = 0; s < slices; ++s) {
-        const float *p = part + ((size_t)s * M + m) * N + n;
-        if (ep.vec) {
-            const f32x4 q = *(const f32x4 *)p;
+        lin_load<float, W>(t, part + ((size_t)s * M + m) * N + n, N - n);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += q[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < N) v[e] += p[e];
-        }
+        for (int e = 0; e < W; ++e) v[e] += t[e];
     }
-    lin_store4<DT>(ep, N, (int)m, n, v);
+    lin_epilogue<DT>(ep, N, (int)m, n, v);
 }
 
 // dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.
@@ -329,45 +433,40 @@ struct DactArgs {
     int M, N, span, act, tpr_log;
 };
 
-template <int DT, int W> __global__ __launch_bounds__(256) void k_lin_dact(const DactArgs a)
+template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactArgs a)
 {
     typedef typename LinT<DT>::S S;
-    typedef S SW __attribute__((ext_vector_type(W)));
+    constexpr int W = LinT<DT>::V;
     __shared__ float red[256 * W];
     const int tpr = 1 << a.tpr_log, tid = threadIdx.x, c = tid & (tpr - 1), r = tid >> a.tpr_log, rows = 256 >> a.tpr_log;
-    const int n = ((int)blockIdx.x * tpr + c) * W;
+    const int n = ((int)blockIdx.x * tpr + c) * W, cnt = a.N - n;
     const int m1 = a.M - (int)blockIdx.y * a.span < a.span ? a.M : ((int)blockIdx.y + 1) * a.span;
     float sum[W];
 #pragma unroll
     for (int e = 0; e < W; ++e) sum[e] = 0.f;
     if (n < a.N)
         for (int m = (int)blockIdx.y * a.span + r; m < m1; m += rows) {
-            const SW gy = *(const SW *)((const S *)a.gy + (size_t)m * a.ldg + n);
-            SW d;
+            float d[W], z[W];
+            lin_load<S, W>(d, (const S *)a.gy + (size_t)m * a.ldg + n, cnt);
             if (a.z) {
-                const SW z = *(const SW *)((const S *)a.z + (size_t)m * a.N + n);
+                lin_load<S, W>(z, (const S *)a.z + (size_t)m * a.N + n, cnt);
 #pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const float t = (float)gy[e] * lin_dact((float)z[e], a.act);
-                    sum[e] += t;
-                    d[e] = (S)t;
-                }
-                *(SW *)((S *)a.dz + (size_t)m * a.N + n) = d;
-            } else {
-#pragma unroll
-                for (int e = 0; e < W; ++e) sum[e] += (float)gy[e];
+                for (int e = 0; e < W; ++e) d[e] *= lin_dact(z[e], a.act);
+                lin_save<S, W>((S *)a.dz + (size_t)m * a.N + n, d, cnt);
             }
+#pragma unroll
+            for (int e = 0; e < W; ++e) sum[e] += d[e];
         }
     if (!a.part) return;
 #pragma unroll
-    for (int e = 0; e < W; ++e) red[tid * W + e] = sum[e];
+    for (int e = 0; e < W; ++e) red[e * 256 + tid] = sum[e];
     __syncthreads();
     if (r == 0 && n < a.N)
 #pragma unroll
         for (int e = 0; e < W; ++e) {
             float s = 0.f;
-            for (int q = 0; q < rows; ++q) s += red[((q << a.tpr_log) + c) * W + e];
-            a.part[(size_t)blockIdx.y * a.N + n + e] = s;
+            for (int q = 0; q < rows; ++q) s += red[e * 256 + (q << a.tpr_log) + c];
+            if (e < cnt) a.part[(size_t)blockIdx.y * a.N + n + e] = s;
         }
 }
 
@@ -385,7 +484,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_colsum(void *db, 
 // ------------------------------------------------------------------------------------------------------------------ host side
 constexpr int LIN_CUS = 256;
 
-struct LinPlan { int slices, kspan; unsigned tm, tn; };
+struct LinPlan { int slices, kspan, big; unsigned tm, tn; };
 
 inline int lin_bk(int dtype) { return dtype == DT_F32 ? 32 : 64; }
 inline long long lin_round(long long v, long long to) { return (v + to - 1) / to * to; }
@@ -394,8 +493,10 @@ LinPlan lin_plan(int dtype, long long M, long long N, long long K)
 {
     LinPlan p;
     const int bk = lin_bk(dtype);
-    p.tm = (unsigned)((M + 127) / 128);
-    p.tn = (unsigned)((N + 127) / 128);
+    p.big = ((M + 255) / 256) * ((N + 255) / 256) >= LIN_CUS;
+    const int edge = p.big ? 256 : 128;
+    p.tm = (unsigned)((M + edge - 1) / edge);
+    p.tn = (unsigned)((N + edge - 1) / edge);
     const long long tiles = (long long)p.tm * p.tn, steps = (K + bk - 1) / bk;
     long long s = tiles >= LIN_CUS ? 1 : 2 * LIN_CUS / tiles;
     s = s < steps / 4 ? s : steps / 4;
@@ -408,42 +509,55 @@ LinPlan lin_plan(int dtype, long long M, long long N, long long K)
 }
 
 inline long long lin_part_bytes(const LinPlan &p, long long M, long long N) { return p.slices > 1 ? lin_round(4ll * p.slices * M * N, 256) : 0; }
+inline int lin_esize(int dtype) { return dtype == DT_F32 ? 4 : 2; }
 
-template <int DT, bool AMC, bool BMC> int lin_run(LinArgs &g, const LinPlan &p, void *ws, hipStream_t st)
+// may an operand travel global -> LDS directly: aligned 16-byte vectors that never straddle a row's end, offsets inside a tile below 2^31
+inline bool lin_direct(const LinOperand &o, long long rows, bool mc, int dtype)
 {
-    constexpr int BM = 128, BN = 128;
+    const int e = lin_esize(dtype), v = 16 / e;
+    return (uintptr_t)o.p % 16 == 0 && o.ld % v == 0 && (!mc || rows % v == 0) && o.ld * e * 256 < 0x7fffffffll;
+}
+
+template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT> int lin_run(LinArgs &g, const LinPlan &p, hipStream_t st)
+{
+    const size_t lds = 2 * (BM + BN) * 8 * sizeof(uint4);
+    static const hipError_t attr = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (attr != hipSuccess) return (int)attr;
+    k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT><<<dim3(p.tm * p.tn, p.slices), 64 * WM * WN, lds, st>>>(g);
+    return lin_status();
+}
+
+template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *ws, hipStream_t st)
+{
+    g.part = p.slices > 1 ? (float *)ws : nullptr;
+    const bool direct = lin_direct(g.a, g.N, AMC, DT) && lin_direct(g.b, g.M, BMC, DT);
+    if (!direct && p.big) {     // (the register route has the small tile only)
+        p.tm = (unsigned)(((long long)g.M + 127) / 128);
+        p.tn = (unsigned)(((long long)g.N + 127) / 128);
+        p.big = 0;
+    }
     g.kspan = p.kspan;
     g.tiles_m = p.tm;
     g.tiles_n = p.tn;
-    g.part = p.slices > 1 ? (float *)ws : nullptr;
-    const size_t lds = 2 * (BM + BN) * 8 * sizeof(uint4);
-    static const hipError_t attr = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, 2, 2, AMC, BMC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (attr != hipSuccess) return (int)attr;
-    k_lin_gemm<DT, BM, BN, 2, 2, AMC, BMC><<<dim3(p.tm * p.tn, p.slices), 256, lds, st>>>(g);
-    if (p.slices > 1) {
-        const long long threads = (long long)g.M * ((g.N + 3) / 4);
-        k_lin_join<DT><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(g.part, p.slices, g.M, g.N, g.ep);
-    }
+    int r;
+    if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false>(g, p, st);
+    else if (p.big) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true>(g, p, st);
+    else r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true>(g, p, st);
+    if (r != BC_OK || p.slices == 1) return r;
+    const long long threads = (long long)g.M * ((g.N + LinT<DT>::V - 1) / LinT<DT>::V);
+    k_lin_join<DT><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(g.part, p.slices, g.M, g.N, g.ep);
     return lin_status();
 }
 
 template <bool AMC, bool BMC> int lin_product(int dtype, LinArgs &g, const LinPlan &p, void *ws, hipStream_t st)
 {
     switch (dtype) {
-    case DT_F32: return lin_run<DT_F32, AMC, BMC>(g, p, ws, st);
-    case DT_F16: return lin_run<DT_F16, AMC, BMC>(g, p, ws, st);
-    default: return lin_run<DT_BF16, AMC, BMC>(g, p, ws, st);
+    case DT_F32: return lin_pick<DT_F32, AMC, BMC>(g, p, ws, st);
+    case DT_F16: return lin_pick<DT_F16, AMC, BMC>(g, p, ws, st);
+    default: return lin_pick<DT_BF16, AMC, BMC>(g, p, ws, st);
     }
 }
 
-inline int lin_esize(int dtype) { return dtype == DT_F32 ? 4 : 2; }
-// 16-byte vectors of a matrix with rows of `run` elements, `ld` apart
-inline int lin_vec(const void *p, long long ld, int dtype)
-{
-    const int e = lin_esize(dtype);
-    return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0;
-}
-inline int lin_vec4(const void *p, long long ld, int dtype) { return !p || ((uintptr_t)p % (4 * lin_esize(dtype)) == 0 && ld % 4 == 0); }
 inline bool lin_aligned(const void *p, int dtype) { return (uintptr_t)p % lin_esize(dtype) == 0; }
 
 int lin_sizes(long long M, int N, int K, int dtype)
@@ -457,13 +571,12 @@ int lin_sizes(long long M, int N, int K, int dtype)
     return BC_OK;
 }
 
-struct DactPlan { int W, tpr_log, span; unsigned gx, gy; };
+struct DactPlan { int tpr_log, span; unsigned gx, gy; };
 
-DactPlan lin_dact_plan(long long M, int N, int V, bool vec)
+DactPlan lin_dact_plan(long long M, int N, int dtype)
 {
     DactPlan p;
-    p.W = vec ? V : 1;
-    const int units = (N + p.W - 1) / p.W;
+    const int W = 16 / lin_esize(dtype), units = (int)(((long long)N + W - 1) / W);
     p.tpr_log = 0;
     while (p.tpr_log < 8 && (1 << p.tpr_log) < units) ++p.tpr_log;
     const int rows = 256 >> p.tpr_log;
@@ -483,8 +596,7 @@ template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, void *
     DactArgs a = a0;
     a.span = p.span;
     a.tpr_log = p.tpr_log;
-    if (p.W > 1) k_lin_dact<DT, LinT<DT>::V><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
-    else k_lin_dact<DT, 1><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
+    k_lin_dact<DT><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
     if (db) k_lin_colsum<DT><<<(a.N + 255) / 256, 256, 0, st>>>(db, db_f32, a.part, (int)p.gy, a.N);
     return lin_status();
 }
@@ -517,9 +629,7 @@ BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, cons
     g.M = (int)M;
     g.N = N;
     g.K = K;
-    g.vec_a = lin_vec(w, ldw, dtype);
-    g.vec_b = lin_vec(x, ldx, dtype);
-    g.ep = {y, z, bias, residual, ldr, bias_f32, act, lin_vec4(y, N, dtype) && lin_vec4(z, N, dtype) && lin_vec4(residual, ldr, dtype)};
+    g.ep = {y, z, bias, residual, ldr, bias_f32, act};
     return lin_product<false, false>(dtype, g, p, workspace, (hipStream_t)stream);
 }
 
@@ -529,8 +639,7 @@ static LinBwdSpace lin_bwd_space(long long M, int N, int K, int act, int dtype)
 {
     LinBwdSpace s;
     s.dz = act != ACT_NONE ? lin_round(M * N * lin_esize(dtype), 256) : 0;
-    const DactPlan a = lin_dact_plan(M, N, dtype == DT_F32 ? 4 : 8, true), b = lin_dact_plan(M, N, 1, false);
-    s.part = lin_round(4ll * N * (a.gy > b.gy ? a.gy : b.gy), 256);
+    s.part = lin_round(4ll * N * lin_dact_plan(M, N, dtype).gy, 256);
     const long long x = lin_part_bytes(lin_plan(dtype, M, K, N), M, K), w = lin_part_bytes(lin_plan(dtype, N, K, M), N, K);
     s.slices = x > w ? x : w;
     return s;
@@ -563,9 +672,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
     const void *dz = gy;
     long long ldz = ldg;
     if (act != ACT_NONE || db) {
-        const int V = dtype == DT_F32 ? 4 : 8;
-        const bool vec = N % V == 0 && lin_vec(gy, ldg, dtype) && (!z || lin_vec(z, N, dtype));
-        const DactPlan p = lin_dact_plan(M, N, V, vec);
+        const DactPlan p = lin_dact_plan(M, N, dtype);
         DactArgs a = {};
         a.gy = gy;
         a.z = act != ACT_NONE ? z : nullptr;
@@ -587,9 +694,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
         g.M = (int)M;
         g.N = K;
         g.K = N;
-        g.vec_a = lin_vec(w, ldw, dtype);
-        g.vec_b = lin_vec(dz, ldz, dtype);
-        g.ep = {dx, nullptr, nullptr, nullptr, 0, 0, ACT_NONE, lin_vec4(dx, K, dtype)};
+                g.ep = {dx, nullptr, nullptr, nullptr, 0, 0, ACT_NONE};
         const int r = lin_product<true, false>(dtype, g, lin_plan(dtype, M, K, N), slices, st);
         if (r != BC_OK) return r;
     }
@@ -600,9 +705,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
         g.M = N;
         g.N = K;
         g.K = (int)M;
-        g.vec_a = lin_vec(x, ldx, dtype);
-        g.vec_b = lin_vec(dz, ldz, dtype);
-        g.ep = {dw, nullptr, nullptr, nullptr, 0, 0, ACT_NONE, lin_vec4(dw, K, dtype)};
+                g.ep = {dw, nullptr, nullptr, nullptr, 0, 0, ACT_NONE};
         const int r = lin_product<true, true>(dtype, g, lin_plan(dtype, N, K, M), slices, st);
         if (r != BC_OK) return r;
     }

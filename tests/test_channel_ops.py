@@ -323,6 +323,25 @@ def test_linear_whole_numbers_are_exact(dt, M, K, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("M,K,N", [(4100, 72, 4104), (4104, 4104, 72), (72, 4104, 4104), (4099, 136, 4101), (8200, 1032, 2056)])
+def test_linear_large_tiles_are_exact(dt, M, K, N):
+    """Enough work for the large tile in each of the three products (and, with odd sizes, what takes its place): whole numbers, exact results."""
+    import blockcopy
+
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    pick = lambda *s: torch.randint(-2, 3, s, generator=gen, device="cuda").to(DT[dt])
+    x, w, b, gy = pick(M, K).requires_grad_(True), pick(N, K).requires_grad_(True), pick(N).requires_grad_(True), pick(M, N)
+    y = blockcopy.linear_act(x, w, b, activation="relu")
+    d = lambda t: t.detach().double()
+    z = d(x) @ d(w).t() + d(b)
+    assert torch.equal(y, z.clamp_min(0).to(DT[dt]))
+    dz = d(gy) * (z > 0)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], gy)
+    assert torch.equal(gx, (dz @ d(w)).to(DT[dt])) and torch.equal(gw, (dz.t() @ d(x)).to(DT[dt])) and torch.equal(gb, dz.sum(0).to(DT[dt]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_linear_infinities_stay_in_their_rows(dt, M):
     """An infinity or NaN in a row of x reaches that row's outputs only, one in a row of w that column's; large finite pre-activations keep
