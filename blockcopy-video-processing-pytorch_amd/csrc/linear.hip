@@ -38,34 +38,63 @@ inline int lin_status()
 // ------------------------------------------------------------------------------------------------------------------ activations
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4, ACT_COUNT = 5 };
 
+// sigmoid(v) = 1 / (1 + e^-v).  fp32 tensors take the library's exponential and the rounded division; for 16-bit ones (result off by 2^-9 or 2^-11
+// anyway) the hardware's exp2 and reciprocal, each good to one unit in the last place of fp32: 4 instructions instead of about 25
+template <int DT> __device__ __forceinline__ float lin_sigmoid(float v)
+{
+    if constexpr (DT == DT_F32) return 1.f / (1.f + expf(-v));
+    else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2).  16-bit tensors: Abramowitz & Stegun 7.1.26, erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2) with
+// t = 1 / (1 + p x), off by at most 1.5e-7 -- 14 instructions, and the derivative needs the same exponential.  erff is about 40: an epilogue
+// of 256 x 256 outputs spent 17 us on it, more than eight steps of products
+template <int DT> __device__ __forceinline__ float lin_phi(float z, float &e)
+{
+    if constexpr (DT == DT_F32) {
+        e = expf(-0.5f * z * z);
+        return 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    } else {
+        e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+        const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.f));
+        const float q = 0.5f * t * e * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        return z < 0.f ? q : 1.f - q;
+    }
+}
+
 // gelu_tanh is z * (1 + tanh(u)) / 2 = z * sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3): one exponential, nothing cancels
 constexpr float GELU_A = 0.7978845608028654f, GELU_B = 0.044715f;
 
-__device__ __forceinline__ float lin_act(float z, int act)
+template <int DT> __device__ __forceinline__ float lin_act(float z, int act)
 {
+    float e;
     switch (act) {
     case ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-    case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case ACT_GELU_TANH: return z / (1.f + expf(-2.f * GELU_A * (z + GELU_B * z * z * z)));
-    case ACT_SILU: return z / (1.f + expf(-z));
+    case ACT_GELU: return z * lin_phi<DT>(z, e);
+    case ACT_GELU_TANH: return z * lin_sigmoid<DT>(2.f * GELU_A * z * fmaf(GELU_B * z, z, 1.f));
+    case ACT_SILU: return z * lin_sigmoid<DT>(z);
     default: return z;
     }
 }
 
 // act'(z).  Beyond +-64 every derivative is 0 or 1 to the last bit; the clamp keeps 0 * infinity out of the products (NaN passes through)
-__device__ __forceinline__ float lin_dact(float z, int act)
+template <int DT> __device__ __forceinline__ float lin_dact(float z, int act)
 {
     const float c = z > 64.f ? 64.f : (z < -64.f ? -64.f : z);
     switch (act) {
     case ACT_RELU: return z != z ? z : (z > 0.f ? 1.f : 0.f);
-    case ACT_GELU: return 0.5f * (1.f + erff(c * 0.70710678118654752f)) + c * expf(-0.5f * c * c) * 0.3989422804014327f;
+    case ACT_GELU: {
+        float e;
+        const float p = lin_phi<DT>(c, e);
+        return fmaf(c * e, 0.3989422804014327f, p);
+    }
     case ACT_GELU_TANH: {
-        const float u = 2.f * GELU_A * (c + GELU_B * c * c * c), s = 1.f / (1.f + expf(-u));
-        return s + c * s * (1.f - s) * 2.f * GELU_A * (1.f + 3.f * GELU_B * c * c);
+        const float s = lin_sigmoid<DT>(2.f * GELU_A * c * fmaf(GELU_B * c, c, 1.f));
+        return s + c * s * (1.f - s) * 2.f * GELU_A * fmaf(3.f * GELU_B * c, c, 1.f);
     }
     case ACT_SILU: {
-        const float s = 1.f / (1.f + expf(-c));
-        return s * (1.f + c * (1.f - s));
+        const float s = lin_sigmoid<DT>(c);
+        return s * fmaf(c, 1.f - s, 1.f);
     }
     default: return 1.f;
     }
@@ -205,7 +234,7 @@ template <int DT> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep,
     if (ep.z) lin_save<S, W>((S *)ep.z + at, v, cnt);
     if (ep.act != ACT_NONE)
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = lin_act(v[e], ep.act);
+        for (int e = 0; e < W; ++e) v[e] = lin_act<DT>(v[e], ep.act);
     if (ep.res) {
         lin_load<S, W>(t, (const S *)ep.res + (size_t)m * ep.ldr + n, cnt);
 #pragma unroll
@@ -374,27 +403,28 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
         }
     }
 
-    // the sums meet their epilogue through the LDS: a wave lays 64 x 64 of them (16-byte vector c of row r at c ^ (r & 15)) into its own part of
-    // the images and takes them back row by row, so that every access to memory is a whole 16-byte vector
-    static_assert(BN / WN == 64 && BM / WM % 64 == 0 && WM * WN * 1024 <= 2 * IMG, "a wave owns 64 columns");
-    uint4 *own = lin_lds + wave * 1024;
-    constexpr int PER_ROW = 64 / V, RPI = 64 / PER_ROW;         // lanes per row, rows per round
-    const int n = n0 + wn * 64 + (lane % PER_ROW) * V;
+    // the sums meet their epilogue through the LDS: a wave lays up to 64 rows of them (16-byte vector c of row r at c ^ (r & its mask)) into its
+    // own part of the images and takes them back row by row, so that every access to memory is a whole 16-byte vector
+    constexpr int CW = BN / WN, RH = BM / WM < 64 ? BM / WM : 64, CPR = CW / 4;      // columns of a wave, rows at a time, vectors per row
+    static_assert(WM * WN * RH * CPR <= 2 * IMG && (CPR & (CPR - 1)) == 0 && CPR <= 16 && BM / WM % RH == 0, "the images hold the waves' sums");
+    uint4 *own = lin_lds + wave * (RH * CPR);
+    constexpr int PER_ROW = CW / V, RPI = 64 / PER_ROW;         // lanes per row, rows per round
+    const int n = n0 + wn * CW + (lane % PER_ROW) * V;
 #pragma unroll
-    for (int h = 0; h < FM / 4; ++h) {
+    for (int h = 0; h < BM / WM / RH; ++h) {
         lin_meet();         // (h = 0: all waves have read the last step; otherwise the wave's own vectors are out)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < RH / 16; ++j)
 #pragma unroll
-            for (int i = 0; i < FN; ++i) own[(16 * j + (lane & 15)) * 16 + ((4 * i + (lane >> 4)) ^ (lane & 15))] = __builtin_bit_cast(uint4, acc[i][4 * h + j]);
+            for (int i = 0; i < FN; ++i) own[(16 * j + (lane & 15)) * CPR + ((4 * i + (lane >> 4)) ^ (lane & (CPR - 1)))] = __builtin_bit_cast(uint4, acc[i][RH / 16 * h + j]);
         lin_meet();
-        for (int r0 = 0; r0 < 64; r0 += RPI) {
-            const int r = r0 + lane / PER_ROW, m = m0 + wm * (BM / WM) + 64 * h + r;
+        for (int r0 = 0; r0 < RH; r0 += RPI) {
+            const int r = r0 + lane / PER_ROW, m = m0 + wm * (BM / WM) + RH * h + r;
             if (m >= g.M || n >= g.N) continue;
             float v[V];
 #pragma unroll
             for (int q = 0; q < V / 4; ++q) {
-                const f32x4 f = __builtin_bit_cast(f32x4, own[r * 16 + (((lane % PER_ROW) * (V / 4) + q) ^ (r & 15))]);
+                const f32x4 f = __builtin_bit_cast(f32x4, own[r * CPR + (((lane % PER_ROW) * (V / 4) + q) ^ (r & (CPR - 1)))]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[4 * q + e] = f[e];
             }
@@ -404,23 +434,37 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
     }
 }
 
-// sums of the slices in their order (run-to-run identical), then the epilogue: one thread per 16 bytes of outputs
+// sums of the slices, then the epilogue.  A workgroup takes 64 x 16 bytes of outputs, four waves a quarter of the slices each; the quarters are
+// added in their order (run-to-run identical)
 template <int DT> __global__ __launch_bounds__(256) void k_lin_join(const float *part, int slices, int M, int N, LinEpi ep)
 {
     constexpr int W = LinT<DT>::V;
+    __shared__ float red[3][W][64];
     const unsigned units = ((unsigned)N + W - 1) / W;
-    const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t id = (size_t)blockIdx.x * 64 + (threadIdx.x & 63);
     const size_t m = id / units;
-    if (m >= (size_t)M) return;
-    const int n = (int)(id % units) * W;
-    float v[W], t[W];
+    const int n = (int)(id % units) * W, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const bool live = m < (size_t)M;
+    float v[W];
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] = 0.f;
-    for (int s = 0; s < slices; ++s) {
-        lin_load<float, W>(t, part + ((size_t)s * M + m) * N + n, N - n);
+    if (live) {
+        const int s1 = slices * (wave + 1) / 4;
+#pragma unroll 4
+        for (int s = slices * wave / 4; s < s1; ++s) {
+            float t[W];
+            lin_load<float, W>(t, part + ((size_t)s * M + m) * N + n, N - n);
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += t[e];
+            for (int e = 0; e < W; ++e) v[e] += t[e];
+        }
+        if (wave)
+#pragma unroll
+            for (int e = 0; e < W; ++e) red[wave - 1][e][lane] = v[e];
     }
+    __syncthreads();
+    if (wave || !live) return;
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = ((v[e] + red[0][e][lane]) + red[1][e][lane]) + red[2][e][lane];
     lin_epilogue<DT>(ep, N, (int)m, n, v);
 }
 
@@ -451,7 +495,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
             if (a.z) {
                 lin_load<S, W>(z, (const S *)a.z + (size_t)m * a.N + n, cnt);
 #pragma unroll
-                for (int e = 0; e < W; ++e) d[e] *= lin_dact(z[e], a.act);
+                for (int e = 0; e < W; ++e) d[e] *= lin_dact<DT>(z[e], a.act);
                 lin_save<S, W>((S *)a.dz + (size_t)m * a.N + n, d, cnt);
             }
 #pragma unroll
@@ -470,13 +514,22 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
         }
 }
 
+// 16 columns x 16 runs of partial sums per workgroup, joined in order
 template <int DT> __global__ __launch_bounds__(256) void k_lin_colsum(void *db, int db_f32, const float *part, int P, int N)
 {
     typedef typename LinT<DT>::S S;
-    const int n = (int)blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+    __shared__ float red[256];
+    const int n = (int)blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
     float s = 0.f;
-    for (int p = 0; p < P; ++p) s += part[(size_t)p * N + n];
+    if (n < N)
+#pragma unroll 8
+        for (int p = run; p < P; p += 16) s += part[(size_t)p * N + n];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (run || n >= N) return;
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += red[16 * r + threadIdx.x];
     if (db_f32) ((float *)db)[n] = s;
     else ((S *)db)[n] = (S)s;
 }
@@ -484,19 +537,19 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_colsum(void *db, 
 // ------------------------------------------------------------------------------------------------------------------ host side
 constexpr int LIN_CUS = 256;
 
-struct LinPlan { int slices, kspan, big; unsigned tm, tn; };
+struct LinPlan { int slices, kspan, edge; unsigned tm, tn; };
 
 inline int lin_bk(int dtype) { return dtype == DT_F32 ? 32 : 64; }
 inline long long lin_round(long long v, long long to) { return (v + to - 1) / to * to; }
+inline long long lin_tiles(long long M, long long N, int edge) { return ((M + edge - 1) / edge) * ((N + edge - 1) / edge); }
 
 LinPlan lin_plan(int dtype, long long M, long long N, long long K)
 {
     LinPlan p;
     const int bk = lin_bk(dtype);
-    p.big = ((M + 255) / 256) * ((N + 255) / 256) >= LIN_CUS;
-    const int edge = p.big ? 256 : 128;
-    p.tm = (unsigned)((M + edge - 1) / edge);
-    p.tn = (unsigned)((N + edge - 1) / edge);
+    p.edge = dtype != DT_F32 && lin_tiles(M, N, 256) >= LIN_CUS ? 256 : lin_tiles(M, N, 128) >= 2 * LIN_CUS ? 128 : 64;
+    p.tm = (unsigned)((M + p.edge - 1) / p.edge);
+    p.tn = (unsigned)((N + p.edge - 1) / p.edge);
     const long long tiles = (long long)p.tm * p.tn, steps = (K + bk - 1) / bk;
     long long s = tiles >= LIN_CUS ? 1 : 2 * LIN_CUS / tiles;
     s = s < steps / 4 ? s : steps / 4;
@@ -531,21 +584,22 @@ template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *
 {
     g.part = p.slices > 1 ? (float *)ws : nullptr;
     const bool direct = lin_direct(g.a, g.N, AMC, DT) && lin_direct(g.b, g.M, BMC, DT);
-    if (!direct && p.big) {     // (the register route has the small tile only)
+    if (!direct && p.edge == 256) {     // (the register route has no large tile)
+        p.edge = 128;
         p.tm = (unsigned)(((long long)g.M + 127) / 128);
         p.tn = (unsigned)(((long long)g.N + 127) / 128);
-        p.big = 0;
     }
     g.kspan = p.kspan;
     g.tiles_m = p.tm;
     g.tiles_n = p.tn;
-    int r;
-    if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false>(g, p, st);
-    else if (p.big) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true>(g, p, st);
-    else r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true>(g, p, st);
+    int r = BC_OK;
+    if (!direct) r = p.edge == 128 ? lin_run<DT, 128, 128, 2, 2, AMC, BMC, false>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false>(g, p, st);
+    else if (p.edge == 128) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true>(g, p, st);
+    else if (p.edge == 64) r = lin_run<DT, 64, 64, 2, 2, AMC, BMC, true>(g, p, st);
+    else if constexpr (DT != DT_F32) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true>(g, p, st);
     if (r != BC_OK || p.slices == 1) return r;
-    const long long threads = (long long)g.M * ((g.N + LinT<DT>::V - 1) / LinT<DT>::V);
-    k_lin_join<DT><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(g.part, p.slices, g.M, g.N, g.ep);
+    const long long units = (long long)g.M * ((g.N + LinT<DT>::V - 1) / LinT<DT>::V);
+    k_lin_join<DT><<<(unsigned)((units + 63) / 64), 256, 0, st>>>(g.part, p.slices, g.M, g.N, g.ep);
     return lin_status();
 }
 
@@ -565,8 +619,8 @@ int lin_sizes(long long M, int N, int K, int dtype)
     if (dtype < 0 || dtype > 2) return BC_ERR_ELEM;
     if (M < 0 || N < 1 || K < 1) return BC_ERR_SHAPE;
     if (M > 0x7fffff00ll || N > 0x7fffff00 || K > 0x7fffff00) return BC_ERR_RANGE;
-    if (((M + 127) / 128) * (((long long)N + 127) / 128) > 0x7fffff00ll || ((M + 127) / 128) * (((long long)K + 127) / 128) > 0x7fffff00ll ||
-        (((long long)N + 127) / 128) * (((long long)K + 127) / 128) > 0x7fffff00ll)
+    if (((M + 63) / 64) * (((long long)N + 63) / 64) > 0x7fffff00ll || ((M + 63) / 64) * (((long long)K + 63) / 64) > 0x7fffff00ll ||
+        (((long long)N + 63) / 64) * (((long long)K + 63) / 64) > 0x7fffff00ll)
         return BC_ERR_RANGE;
     return BC_OK;
 }
@@ -597,7 +651,7 @@ template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, void *
     a.span = p.span;
     a.tpr_log = p.tpr_log;
     k_lin_dact<DT><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
-    if (db) k_lin_colsum<DT><<<(a.N + 255) / 256, 256, 0, st>>>(db, db_f32, a.part, (int)p.gy, a.N);
+    if (db) k_lin_colsum<DT><<<(a.N + 15) / 16, 256, 0, st>>>(db, db_f32, a.part, (int)p.gy, a.N);
     return lin_status();
 }
 
