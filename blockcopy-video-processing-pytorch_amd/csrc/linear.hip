@@ -24,10 +24,10 @@ typedef __attribute__((address_space(3))) s16x4 *lds_s16x4_ptr;
 
 enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };      // the dtype codes of the C ABI
 
-// V elements make 16 bytes; BK summed indexes make the 128 bytes of one staged row
-template <int DT> struct LinT { typedef float S; static constexpr int V = 4, BK = 32; };
-template <> struct LinT<DT_F16> { typedef _Float16 S; static constexpr int V = 8, BK = 64; };
-template <> struct LinT<DT_BF16> { typedef __bf16 S; static constexpr int V = 8, BK = 64; };
+// V elements make 16 bytes
+template <int DT> struct LinT { typedef float S; static constexpr int V = 4; };
+template <> struct LinT<DT_F16> { typedef _Float16 S; static constexpr int V = 8; };
+template <> struct LinT<DT_BF16> { typedef __bf16 S; static constexpr int V = 8; };
 
 inline int lin_status()
 {
@@ -135,24 +135,34 @@ template <int DT> __device__ __forceinline__ void lin_mma(f32x4 &d, const uint4 
     }
 }
 
-// One staged operand tile: R rows (output rows or columns) x BK summed indexes = R * 8 vectors of 16 bytes.
-//   KC (memory runs along the summed index): image [row][8 vectors], vector c of row r at c ^ (r & 7): the 16 rows x 4 vectors that one
+// One staged operand tile: R rows (output rows or columns) x C vectors of 16 bytes along the summed index (C = 8 or 4)
+//   KC (memory runs along the summed index): image [row][C vectors], vector c of row r at c ^ lin_turn(r): the 16 rows x 4 vectors that one
 //      fragment read touches cover all banks
 //   MC (memory runs across it): image [k][R / V vectors], vectors exchanged by lin_swz(k); 16-bit fragments are transposed by the LDS read
 //      itself (ds_read_b64_tr_b16: a group of 16 lanes addresses 4 k x 16 rows and lane i receives row i's four k), fp32 ones read word by word
+template <int C> __device__ __forceinline__ int lin_turn(int row) { return C == 8 ? row & 7 : (row >> 1) & 3; }
+
 template <int DT, int R> __device__ __forceinline__ int lin_swz(int k)
 {
     if constexpr (DT == DT_F32) return ((k >> 2) & 3) * 4;
     else return ((k & 3) * 2 + ((k >> 3) & 1) * 8) & (R / 8 - 1);
 }
 
-template <int DT, bool MC, int R> __device__ __forceinline__ uint4 lin_frag(const uint4 *img, int row0, int ks, int lane)
+// place of the tile's v-th vector (in the order of memory: runs of C or of R / V) inside its image
+template <int DT, bool MC, int R, int C> __device__ __forceinline__ int lin_place(int v)
+{
+    constexpr int V = LinT<DT>::V;
+    if constexpr (MC) return v / (R / V) * (R / V) + ((v % (R / V)) ^ lin_swz<DT, R>(v / (R / V)));
+    else return v / C * C + ((v % C) ^ lin_turn<C>(v / C));
+}
+
+template <int DT, bool MC, int R, int C> __device__ __forceinline__ uint4 lin_frag(const uint4 *img, int row0, int ks, int lane)
 {
     constexpr int V = LinT<DT>::V, CPR = R / V;
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!MC) {
         const int row = row0 + r;
-        return img[row * 8 + ((ks * 4 + g) ^ (row & 7))];
+        return img[row * C + ((ks * 4 + g) ^ lin_turn<C>(row))];
     } else if constexpr (DT == DT_F32) {
         const float *f = (const float *)img;
         float v[4];
@@ -217,15 +227,21 @@ template <typename S, int W> __device__ __forceinline__ void lin_save(S *p, cons
             if (e < cnt) p[e] = (S)f[e];
 }
 
-// 16 bytes' worth of consecutive outputs (m, n ..), cnt of them inside the matrix: sums v -> z, y
-template <int DT> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v)
+// 16 bytes' worth of consecutive outputs (m, n ..), cnt of them inside the matrix: sums v -> z, y.  The residual r is loaded by the caller, ahead
+template <int DT> __device__ __forceinline__ void lin_residual(float *r, const LinEpi &ep, int N, int m, int n)
+{
+    typedef typename LinT<DT>::S S;
+    lin_load<S, LinT<DT>::V>(r, (const S *)ep.res + (size_t)m * ep.ldr + n, N - n);
+}
+
+template <int DT> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v, const float *r)
 {
     typedef typename LinT<DT>::S S;
     constexpr int W = LinT<DT>::V;
     const int cnt = N - n;
     const size_t at = (size_t)m * N + n;
-    float t[W];
     if (ep.bias) {
+        float t[W];
         if (ep.bias_f32) lin_load<float, W>(t, (const float *)ep.bias + n, cnt);
         else lin_load<S, W>(t, (const S *)ep.bias + n, cnt);
 #pragma unroll
@@ -235,11 +251,9 @@ template <int DT> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep,
     if (ep.act != ACT_NONE)
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] = lin_act<DT>(v[e], ep.act);
-    if (ep.res) {
-        lin_load<S, W>(t, (const S *)ep.res + (size_t)m * ep.ldr + n, cnt);
+    if (ep.res)
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += t[e];
-    }
+        for (int e = 0; e < W; ++e) v[e] += r[e];
     lin_save<S, W>((S *)ep.y + at, v, cnt);
 }
 
@@ -263,24 +277,28 @@ __device__ __forceinline__ void lin_meet()
 }
 
 // out[m][n] = sum_k A(n, k) B(m, k).  A workgroup of WM x WN waves owns a BM x BN tile; the column operand is the matrix instruction's first
-// one, so a lane ends up with four consecutive columns of one row.  Two LDS images: while step t is multiplied, step t + 1 travels into the
-// other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel global -> LDS without registers (a partial last step
-// goes through registers, zero-filled); otherwise through registers, requested before the products and stored behind them.
-template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT>
+// one, so a lane ends up with four consecutive columns of one row.  Two LDS images of a step's operands, C vectors (16 C bytes) of every row:
+// while step t is multiplied, step t + 1 travels into the other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel
+// global -> LDS without registers (a partial last step goes through registers, zero-filled); otherwise through registers, requested before
+// the products and stored behind them.
+template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C>
 __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
 {
-    constexpr int V = LinT<DT>::V, BK = LinT<DT>::BK, NT = 64 * WM * WN, ES = 16 / V;
+    constexpr int V = LinT<DT>::V, BK = C * V, NT = 64 * WM * WN, ES = 16 / V;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    constexpr int NA = BN * 8 / NT, NB = BM * 8 / NT;       // vectors per thread and step
-    constexpr int IMG = (BM + BN) * 8;
+    constexpr int NA = BN * C / NT, NB = BM * C / NT;       // vectors per thread and step
+    constexpr int IMG = (BM + BN) * C;
     extern __shared__ uint4 lin_lds[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
-    // tiles in bands of 8 tile rows: neighbouring workgroups share operands
-    const unsigned band = 8 * g.tiles_n, b0 = blockIdx.x / band, in = blockIdx.x % band;
+    // consecutive workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD takes one run of the work (slice by slice, tile by tile),
+    // so what its workgroups share is fetched into that L2 once.  Inside a slice tiles go in bands of 8 tile rows
+    const unsigned all = gridDim.x, xcd = blockIdx.x & 7u, id = xcd * (all >> 3) + (xcd < (all & 7u) ? xcd : all & 7u) + (blockIdx.x >> 3);
+    const unsigned slice = id / (g.tiles_m * g.tiles_n), tile = id - slice * (g.tiles_m * g.tiles_n);
+    const unsigned band = 8 * g.tiles_n, b0 = tile / band, in = tile % band;
     const unsigned rows_in_band = g.tiles_m - b0 * 8 < 8 ? g.tiles_m - b0 * 8 : 8;
     const int m0 = (int)(b0 * 8 + in % rows_in_band) * BM, n0 = (int)(in / rows_in_band) * BN;
-    const int kbeg = (int)blockIdx.y * g.kspan, kend = g.K - kbeg < g.kspan ? g.K : kbeg + g.kspan;
+    const int kbeg = (int)slice * g.kspan, kend = g.K - kbeg < g.kspan ? g.K : kbeg + g.kspan;
 
     uint4 ra[NA], rb[NB];
     auto fetch = [&](int k0) {
@@ -288,67 +306,59 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
         for (int i = 0; i < NA; ++i) {
             const int v = tid + NT * i;
             if constexpr (AMC) ra[i] = lin_fetch<DT, true>(g.a, g.N, kend, n0 + v % (BN / V) * V, k0 + v / (BN / V));
-            else ra[i] = lin_fetch<DT, false>(g.a, g.N, kend, n0 + (v >> 3), k0 + (v & 7) * V);
+            else ra[i] = lin_fetch<DT, false>(g.a, g.N, kend, n0 + v / C, k0 + v % C * V);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int v = tid + NT * i;
             if constexpr (BMC) rb[i] = lin_fetch<DT, true>(g.b, g.M, kend, m0 + v % (BM / V) * V, k0 + v / (BM / V));
-            else rb[i] = lin_fetch<DT, false>(g.b, g.M, kend, m0 + (v >> 3), k0 + (v & 7) * V);
+            else rb[i] = lin_fetch<DT, false>(g.b, g.M, kend, m0 + v / C, k0 + v % C * V);
         }
     };
     auto stage = [&](uint4 *img) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int v = tid + NT * i;
-            if constexpr (AMC) img[(v / (BN / V)) * (BN / V) + ((v % (BN / V)) ^ lin_swz<DT, BN>(v / (BN / V)))] = ra[i];
-            else img[(v & ~7) + ((v & 7) ^ ((v >> 3) & 7))] = ra[i];
-        }
-        img += BN * 8;
+        for (int i = 0; i < NA; ++i) img[lin_place<DT, AMC, BN, C>(tid + NT * i)] = ra[i];
+        img += BN * C;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int v = tid + NT * i;
-            if constexpr (BMC) img[(v / (BM / V)) * (BM / V) + ((v % (BM / V)) ^ lin_swz<DT, BM>(v / (BM / V)))] = rb[i];
-            else img[(v & ~7) + ((v & 7) ^ ((v >> 3) & 7))] = rb[i];
-        }
+        for (int i = 0; i < NB; ++i) img[lin_place<DT, BMC, BM, C>(tid + NT * i)] = rb[i];
     };
     // direct copies: byte offsets of this lane's sources from the tile's corner of the step.  Rows behind the matrix take its last row
-    // (vector) -- their sums are never stored
+    // (vector) -- their sums are never stored.  The exchange of an image is its own inverse: the vector that belongs at place v is lin_place(v)
     unsigned oa[NA], ob[NB];
     const char *pa = nullptr, *pb = nullptr;
-    const size_t stepa = AMC ? (size_t)BK * g.a.ld * ES : 128, stepb = BMC ? (size_t)BK * g.b.ld * ES : 128;
+    const size_t stepa = AMC ? (size_t)BK * g.a.ld * ES : 16 * C, stepb = BMC ? (size_t)BK * g.b.ld * ES : 16 * C;
     if constexpr (DIRECT) {
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-            const int v = tid + NT * i;
+            const int v = lin_place<DT, AMC, BN, C>(tid + NT * i);
             if constexpr (AMC) {
-                const int k = v / (BN / V), c = (v % (BN / V)) ^ lin_swz<DT, BN>(k), n = n0 + c * V + V <= g.N ? c * V : g.N - V - n0;
+                const int k = v / (BN / V), c = v % (BN / V), n = n0 + c * V + V <= g.N ? c * V : g.N - V - n0;
                 oa[i] = (unsigned)((long long)k * g.a.ld + n) * ES;
             } else {
-                const int row = n0 + (v >> 3) < g.N ? v >> 3 : g.N - 1 - n0;
-                oa[i] = (unsigned)((long long)row * g.a.ld) * ES + (unsigned)((v & 7) ^ ((v >> 3) & 7)) * 16;
+                const int row = n0 + v / C < g.N ? v / C : g.N - 1 - n0;
+                oa[i] = (unsigned)((long long)row * g.a.ld) * ES + (unsigned)(v % C) * 16;
             }
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int v = tid + NT * i;
+            const int v = lin_place<DT, BMC, BM, C>(tid + NT * i);
             if constexpr (BMC) {
-                const int k = v / (BM / V), c = (v % (BM / V)) ^ lin_swz<DT, BM>(k), m = m0 + c * V + V <= g.M ? c * V : g.M - V - m0;
+                const int k = v / (BM / V), c = v % (BM / V), m = m0 + c * V + V <= g.M ? c * V : g.M - V - m0;
                 ob[i] = (unsigned)((long long)k * g.b.ld + m) * ES;
             } else {
-                const int row = m0 + (v >> 3) < g.M ? v >> 3 : g.M - 1 - m0;
-                ob[i] = (unsigned)((long long)row * g.b.ld) * ES + (unsigned)((v & 7) ^ ((v >> 3) & 7)) * 16;
+                const int row = m0 + v / C < g.M ? v / C : g.M - 1 - m0;
+                ob[i] = (unsigned)((long long)row * g.b.ld) * ES + (unsigned)(v % C) * 16;
             }
         }
         pa = (const char *)g.a.p + ((AMC ? (size_t)kbeg * g.a.ld + n0 : (size_t)n0 * g.a.ld + kbeg)) * ES;
         pb = (const char *)g.b.p + ((BMC ? (size_t)kbeg * g.b.ld + m0 : (size_t)m0 * g.b.ld + kbeg)) * ES;
     }
-    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lin_lds;
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lin_lds + wave * 1024;
     auto copy = [&](int img) {      // the next step's operands into image `img`
 #pragma unroll
-        for (int i = 0; i < NA; ++i) lin_copy16(pa, oa[i], lds0 + (img * IMG + wave * 64 + NT * i) * 16);
+        for (int i = 0; i < NA; ++i) lin_copy16(pa, oa[i], lds0 + (img * IMG + NT * i) * 16);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) lin_copy16(pb, ob[i], lds0 + (img * IMG + BN * 8 + wave * 64 + NT * i) * 16);
+        for (int i = 0; i < NB; ++i) lin_copy16(pb, ob[i], lds0 + (img * IMG + BN * C + NT * i) * 16);
         pa += stepa;
         pb += stepb;
     };
@@ -359,14 +369,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](const uint4 *ia) {
-        const uint4 *ib = ia + BN * 8;
+        const uint4 *ib = ia + BN * C;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+        for (int ks = 0; ks < C / 4; ++ks) {
             uint4 fa[FN], fb[FM];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) fa[i] = lin_frag<DT, AMC, BN>(ia, wn * (BN / WN) + 16 * i, ks, lane);
+            for (int i = 0; i < FN; ++i) fa[i] = lin_frag<DT, AMC, BN, C>(ia, wn * (BN / WN) + 16 * i, ks, lane);
 #pragma unroll
-            for (int j = 0; j < FM; ++j) fb[j] = lin_frag<DT, BMC, BM>(ib, wm * (BM / WM) + 16 * j, ks, lane);
+            for (int j = 0; j < FM; ++j) fb[j] = lin_frag<DT, BMC, BM, C>(ib, wm * (BM / WM) + 16 * j, ks, lane);
 #pragma unroll
             for (int i = 0; i < FN; ++i)
 #pragma unroll
@@ -403,34 +413,46 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
         }
     }
 
-    // the sums meet their epilogue through the LDS: a wave lays up to 64 rows of them (16-byte vector c of row r at c ^ (r & its mask)) into its
-    // own part of the images and takes them back row by row, so that every access to memory is a whole 16-byte vector
-    constexpr int CW = BN / WN, RH = BM / WM < 64 ? BM / WM : 64, CPR = CW / 4;      // columns of a wave, rows at a time, vectors per row
-    static_assert(WM * WN * RH * CPR <= 2 * IMG && (CPR & (CPR - 1)) == 0 && CPR <= 16 && BM / WM % RH == 0, "the images hold the waves' sums");
-    uint4 *own = lin_lds + wave * (RH * CPR);
+    // the sums meet their epilogue through the LDS: a wave lays RH rows of them (16-byte vector c of row r at c ^ (r & its mask)) into its own
+    // part of the images and takes them back row by row, so that every access to memory is a whole 16-byte vector
+    constexpr int CW = BN / WN, CPR = CW / 4, FIT = 2 * IMG / (WM * WN * CPR);       // columns of a wave, vectors per row, rows that fit
+    constexpr int RH = BM / WM <= FIT && BM / WM <= 64 ? BM / WM : FIT >= 64 ? 64 : FIT >= 32 ? 32 : 16;
+    static_assert(FIT >= 16 && (CPR & (CPR - 1)) == 0 && CPR <= 16 && BM / WM % RH == 0, "the images hold the waves' sums");
     constexpr int PER_ROW = CW / V, RPI = 64 / PER_ROW;         // lanes per row, rows per round
+    constexpr int AHEAD = RH / RPI < 4 ? RH / RPI : 4;          // rounds whose residuals are requested together
+    uint4 *own = lin_lds + wave * (RH * CPR);
     const int n = n0 + wn * CW + (lane % PER_ROW) * V;
+    lin_meet();         // all waves have read the last step
 #pragma unroll
-    for (int h = 0; h < BM / WM / RH; ++h) {
-        lin_meet();         // (h = 0: all waves have read the last step; otherwise the wave's own vectors are out)
+    for (int h = 0; h < BM / WM / RH; ++h) {        // (the part is the wave's own and its LDS accesses stay in order: no barrier)
 #pragma unroll
         for (int j = 0; j < RH / 16; ++j)
 #pragma unroll
             for (int i = 0; i < FN; ++i) own[(16 * j + (lane & 15)) * CPR + ((4 * i + (lane >> 4)) ^ (lane & (CPR - 1)))] = __builtin_bit_cast(uint4, acc[i][RH / 16 * h + j]);
-        lin_meet();
-        for (int r0 = 0; r0 < RH; r0 += RPI) {
-            const int r = r0 + lane / PER_ROW, m = m0 + wm * (BM / WM) + RH * h + r;
-            if (m >= g.M || n >= g.N) continue;
-            float v[V];
+        __builtin_amdgcn_wave_barrier();
+        for (int r0 = lane / PER_ROW; r0 < RH; r0 += AHEAD * RPI) {
+            float res[AHEAD][V];
+            const int mb = m0 + wm * (BM / WM) + RH * h;
+            if (g.ep.res && !g.part)
 #pragma unroll
-            for (int q = 0; q < V / 4; ++q) {
-                const f32x4 f = __builtin_bit_cast(f32x4, own[r * CPR + (((lane % PER_ROW) * (V / 4) + q) ^ (r & (CPR - 1)))]);
+                for (int q = 0; q < AHEAD; ++q)
+                    if (mb + r0 + q * RPI < g.M && n < g.N) lin_residual<DT>(res[q], g.ep, g.N, mb + r0 + q * RPI, n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * q + e] = f[e];
+            for (int q = 0; q < AHEAD; ++q) {
+                const int r = r0 + q * RPI, m = mb + r;
+                if (m >= g.M || n >= g.N) continue;
+                float v[V];
+#pragma unroll
+                for (int p = 0; p < V / 4; ++p) {
+                    const f32x4 f = __builtin_bit_cast(f32x4, own[r * CPR + (((lane % PER_ROW) * (V / 4) + p) ^ (r & (CPR - 1)))]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[4 * p + e] = f[e];
+                }
+                if (g.part) lin_save<float, V>(g.part + ((size_t)slice * g.M + m) * g.N + n, v, g.N - n);
+                else lin_epilogue<DT>(g.ep, g.N, m, n, v, res[q]);
             }
-            if (g.part) lin_save<float, V>(g.part + ((size_t)blockIdx.y * g.M + m) * g.N + n, v, g.N - n);
-            else lin_epilogue<DT>(g.ep, g.N, m, n, v);
         }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -463,9 +485,11 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_join(const float 
     }
     __syncthreads();
     if (wave || !live) return;
+    float r[W];
+    if (ep.res) lin_residual<DT>(r, ep, N, (int)m, n);
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] = ((v[e] + red[0][e][lane]) + red[1][e][lane]) + red[2][e][lane];
-    lin_epilogue<DT>(ep, N, (int)m, n, v);
+    lin_epilogue<DT>(ep, N, (int)m, n, v, r);
 }
 
 // dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.
@@ -489,6 +513,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
 #pragma unroll
     for (int e = 0; e < W; ++e) sum[e] = 0.f;
     if (n < a.N)
+#pragma unroll 2
         for (int m = (int)blockIdx.y * a.span + r; m < m1; m += rows) {
             float d[W], z[W];
             lin_load<S, W>(d, (const S *)a.gy + (size_t)m * a.ldg + n, cnt);
@@ -547,7 +572,11 @@ LinPlan lin_plan(int dtype, long long M, long long N, long long K)
 {
     LinPlan p;
     const int bk = lin_bk(dtype);
-    p.edge = dtype != DT_F32 && lin_tiles(M, N, 256) >= LIN_CUS ? 256 : lin_tiles(M, N, 128) >= 2 * LIN_CUS ? 128 : 64;
+    // fp32: 64 (the matrix instructions take so long that a small tile's operands arrive in time: 17408 x 768 x 256 72 us against 105 with 128,
+    // 1024^3 24 against 34).  16 bits: 256 once that fills the chip and the sum is long enough to pay for an epilogue that nothing overlaps
+    // (16384 x 4096 x 8192: 903 us, 128: 1040, 64: 1565; 8192 x 2048 x 8192: 240, 279, 384 -- but 17408 x 512 x 2048: 77, 60, 65), else 128 while
+    // every CU gets two, else 64 (2048^3 with gelu 31 us against 35)
+    p.edge = dtype == DT_F32 ? 64 : K >= 1024 && lin_tiles(M, N, 256) >= LIN_CUS ? 256 : lin_tiles(M, N, 128) >= 2 * LIN_CUS ? 128 : 64;
     p.tm = (unsigned)((M + p.edge - 1) / p.edge);
     p.tn = (unsigned)((N + p.edge - 1) / p.edge);
     const long long tiles = (long long)p.tm * p.tn, steps = (K + bk - 1) / bk;
@@ -571,12 +600,12 @@ inline bool lin_direct(const LinOperand &o, long long rows, bool mc, int dtype)
     return (uintptr_t)o.p % 16 == 0 && o.ld % v == 0 && (!mc || rows % v == 0) && o.ld * e * 256 < 0x7fffffffll;
 }
 
-template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT> int lin_run(LinArgs &g, const LinPlan &p, hipStream_t st)
+template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C> int lin_run(LinArgs &g, const LinPlan &p, hipStream_t st)
 {
-    const size_t lds = 2 * (BM + BN) * 8 * sizeof(uint4);
-    static const hipError_t attr = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const size_t lds = (size_t)2 * (BM + BN) * C * sizeof(uint4);
+    static const hipError_t attr = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (attr != hipSuccess) return (int)attr;
-    k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT><<<dim3(p.tm * p.tn, p.slices), 64 * WM * WN, lds, st>>>(g);
+    k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C><<<p.tm * p.tn * (unsigned)p.slices, 64 * WM * WN, lds, st>>>(g);
     return lin_status();
 }
 
@@ -593,10 +622,15 @@ template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *
     g.tiles_m = p.tm;
     g.tiles_n = p.tn;
     int r = BC_OK;
-    if (!direct) r = p.edge == 128 ? lin_run<DT, 128, 128, 2, 2, AMC, BMC, false>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false>(g, p, st);
-    else if (p.edge == 128) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true>(g, p, st);
-    else if (p.edge == 64) r = lin_run<DT, 64, 64, 2, 2, AMC, BMC, true>(g, p, st);
-    else if constexpr (DT != DT_F32) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true>(g, p, st);
+    if (p.edge == 64) r = direct ? lin_run<DT, 64, 64, 2, 2, AMC, BMC, true, 8>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false, 8>(g, p, st);
+    else if constexpr (DT != DT_F32) {
+        // (a short sum: steps of 64 bytes halve the images, three workgroups share a CU and one's epilogue runs beside another's products:
+        //  17408 x 512 x 2048 with gelu 77 us against 92; a long one: 128 bytes, half the barriers, 2048 x 2048 x 2048 29 us against 70)
+        if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false, 8>(g, p, st);
+        else if (p.edge == 256) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true, 8>(g, p, st);
+        else if (g.K < 1024) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 4>(g, p, st);
+        else r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 8>(g, p, st);
+    }
     if (r != BC_OK || p.slices == 1) return r;
     const long long units = (long long)g.M * ((g.N + LinT<DT>::V - 1) / LinT<DT>::V);
     k_lin_join<DT><<<(unsigned)((units + 63) / 64), 256, 0, st>>>(g.part, p.slices, g.M, g.N, g.ep);
