@@ -211,6 +211,16 @@ def load_library(path: str = None) -> ctypes.CDLL:
     return lib
 
 
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _raw_stream(index: int) -> int:
+    """Handle of the current stream of device ``index``."""
+    fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return fast(index) if fast is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 class HipBackend:
     """The product backend: raw device pointers into libblockcopy_hip.so on torch's current stream."""
 
@@ -1025,31 +1035,47 @@ class HipBackend:
     # -- channel operators on rows of features (blockcopy/utils/channel_ops.py; csrc/linear.hip, csrc/norm_residual.hip).  Every matrix is
     #    (rows, features) with unit feature stride; workspaces come from the caching allocator on the current stream, so a captured call owns
     #    its workspace inside the graph's pool
+    # (these calls are as short as a few microseconds of device work, so their host side is kept lean: one check per tensor, the current stream's
+    #  handle without a Stream object, the device switched only if it is another one)
     @staticmethod
-    def _rows_ok(t, shape, dtype, device):
-        return t is None or (t.dim() == 2 and tuple(t.shape) == tuple(shape) and t.dtype == dtype and t.device == device
-                             and (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]))
+    def _rows_ok(t, rows, cols, dtype, device):
+        if t is None:
+            return True
+        shape = t.shape
+        return (len(shape) == 2 and shape[0] == rows and shape[1] == cols and t.dtype == dtype and t.device == device
+                and (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols))
 
     @staticmethod
     def _ld(t):
         return 0 if t is None else max(t.stride(0), t.shape[1])      # (the stride of a single row may be anything)
 
+    def _launch(self, op, fn, device, args):
+        """fn(*args, stream) on the current stream of ``device``."""
+        index = device.index
+        if index == torch.cuda.current_device():
+            rc = fn(*args, _raw_stream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, _raw_stream(index))
+        if rc:
+            self._check(rc, op)
+
     def linear_fwd(self, x, weight, bias=None, act: int = 0, residual=None, keep_z: bool = False):
         """(y, z): y = act(z) + residual with z = x weight^T + bias; z is handed back (x's dtype) if ``keep_z``."""
         M, K = x.shape
         N = weight.shape[0]
-        assert x.is_cuda and x.dtype in _DTYPE_CODE, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
-        assert self._rows_ok(x, (M, K), x.dtype, x.device) and self._rows_ok(weight, (N, K), x.dtype, x.device) and self._rows_ok(residual, (M, N), x.dtype, x.device)
-        assert bias is None or (bias.shape == (N,) and bias.is_contiguous() and bias.dtype in (x.dtype, torch.float32) and bias.device == x.device)
-        code = _DTYPE_CODE[x.dtype]
-        ptr = lambda t: t.data_ptr() if t is not None else None
-        with torch.cuda.device_of(x):
-            y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-            z = torch.empty_like(y) if keep_z else None
-            need = self.lib.bc_linear_fwd_workspace(M, N, K, code)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-            self._check(self.lib.bc_linear_fwd(ptr(y), ptr(z), ptr(x), ptr(weight), ptr(bias), ptr(residual), M, N, K, self._ld(x), self._ld(weight), self._ld(residual),
-                                               int(act), code, int(bias is not None and bias.dtype == torch.float32), ptr(ws), need, self._stream()), "linear_fwd")
+        dt, dev = x.dtype, x.device
+        code = _DTYPE_CODE.get(dt)
+        assert x.is_cuda and code is not None, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
+        assert self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev) and self._rows_ok(residual, M, N, dt, dev)
+        assert bias is None or (bias.shape == (N,) and bias.is_contiguous() and bias.dtype in (dt, torch.float32) and bias.device == dev)
+        y = x.new_empty((M, N))
+        z = x.new_empty((M, N)) if keep_z else None
+        need = self.lib.bc_linear_fwd_workspace(M, N, K, code)
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
+        self._launch("linear_fwd", self.lib.bc_linear_fwd, dev,
+                     (y.data_ptr(), _ptr(z), x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), M, N, K, self._ld(x), self._ld(weight), self._ld(residual),
+                      act, code, bias is not None and bias.dtype == torch.float32, _ptr(ws), need))
         return y, z
 
     def linear_bwd(self, gy, z, x, weight, act: int, want, bias_dtype=None):
@@ -1057,45 +1083,48 @@ class HipBackend:
         M, N = gy.shape
         K = weight.shape[1] if weight is not None else x.shape[1]
         dt, dev = gy.dtype, gy.device
-        assert gy.is_cuda and dt in _DTYPE_CODE
-        assert all(self._rows_ok(t, s, dt, dev) for t, s in ((gy, (M, N)), (z, (M, N)), (x, (M, K)), (weight, (N, K)))) and (z is None or z.is_contiguous())
-        dx = torch.empty((M, K), dtype=dt, device=dev) if want[0] else None
-        dw = torch.empty((N, K), dtype=dt, device=dev) if want[1] else None
-        db = torch.empty((N,), dtype=bias_dtype or dt, device=dev) if want[2] else None
+        code = _DTYPE_CODE.get(dt)
+        assert gy.is_cuda and code is not None
+        assert (self._rows_ok(gy, M, N, dt, dev) and self._rows_ok(z, M, N, dt, dev) and self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev)
+                and (z is None or z.is_contiguous()))
+        dx = gy.new_empty((M, K)) if want[0] else None
+        dw = gy.new_empty((N, K)) if want[1] else None
+        db = gy.new_empty((N,), dtype=bias_dtype or dt) if want[2] else None
         if M == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-        code = _DTYPE_CODE[dt]
-        ptr = lambda t: t.data_ptr() if t is not None else None
-        with torch.cuda.device_of(gy):
-            need = self.lib.bc_linear_bwd_workspace(M, N, K, int(act), code)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            self._check(self.lib.bc_linear_bwd(ptr(dx), ptr(dw), ptr(db), ptr(gy), ptr(z), ptr(x), ptr(weight), M, N, K, self._ld(gy), self._ld(x), self._ld(weight),
-                                               int(act), code, int(db is not None and db.dtype == torch.float32), ptr(ws), need, self._stream()), "linear_bwd")
+        need = self.lib.bc_linear_bwd_workspace(M, N, K, act, code)
+        ws = gy.new_empty(need, dtype=torch.uint8)
+        self._launch("linear_bwd", self.lib.bc_linear_bwd, dev,
+                     (_ptr(dx), _ptr(dw), _ptr(db), gy.data_ptr(), _ptr(z), _ptr(x), _ptr(weight), M, N, K, self._ld(gy), self._ld(x), self._ld(weight),
+                      act, code, db is not None and db.dtype == torch.float32, ws.data_ptr(), need))
         return dx, dw, db
 
     @staticmethod
-    def _norm_params_ok(params, C, dtype, device, groups=None):
-        kinds = {p.dtype for p in params if p is not None}
-        assert len(kinds) <= 1 and kinds <= {dtype, torch.float32}, "norm parameters and gate must share one dtype: the rows' or float32"
+    def _norm_params(params, C, dtype, device, groups):
+        """1 if the norm's parameters are float32 besides rows of another type (checked: one dtype, contiguous, C values each, the gate groups * C)."""
+        kind = None
         for k, p in enumerate(params):
-            assert p is None or (p.is_contiguous() and p.device == device and p.numel() == (C * groups if groups and k == 2 else C))
-        return int(kinds == {torch.float32})
+            if p is not None:
+                assert p.dtype in (dtype, torch.float32) and p.dtype == (kind or p.dtype), "norm parameters and gate must share one dtype: the rows' or float32"
+                assert p.is_contiguous() and p.device == device and p.numel() == (C * groups if groups and k == 2 else C)
+                kind = p.dtype
+        return kind == torch.float32
 
     def norm_residual_fwd(self, h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind: int, in_kind: int, residual_scale: float, eps: float,
                           rows_per_gate: int = 0, keep_stats: bool = False):
         """(h_new, u, stats): h_new = residual_scale * h + gate * N_out(y), u = N_in(h_new) (blockcopy/utils/channel_ops.py); None for what is not asked for."""
         M, C = h.shape
-        assert h.is_cuda and h.dtype in _DTYPE_CODE, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
-        assert self._rows_ok(h, (M, C), h.dtype, h.device) and self._rows_ok(y, (M, C), h.dtype, h.device)
-        pf32 = self._norm_params_ok((out_weight, out_bias, gate, in_weight, in_bias), C, h.dtype, h.device, M // rows_per_gate if rows_per_gate else None)
-        ptr = lambda t: t.data_ptr() if t is not None else None
-        with torch.cuda.device_of(h):
-            ho = torch.empty((M, C), dtype=h.dtype, device=h.device) if y is not None else None
-            u = torch.empty((M, C), dtype=h.dtype, device=h.device) if in_kind else None
-            stats = torch.empty((M, 4), dtype=torch.float32, device=h.device) if keep_stats else None
-            self._check(self.lib.bc_norm_residual_fwd(ptr(ho), ptr(u), ptr(stats), ptr(h), ptr(y), ptr(out_weight), ptr(out_bias), ptr(gate), ptr(in_weight), ptr(in_bias),
-                                                      M, C, self._ld(h), self._ld(y), int(rows_per_gate), float(residual_scale), float(eps), int(out_kind), int(in_kind),
-                                                      _DTYPE_CODE[h.dtype], pf32, self._stream()), "norm_residual_fwd")
+        dt, dev = h.dtype, h.device
+        code = _DTYPE_CODE.get(dt)
+        assert h.is_cuda and code is not None, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
+        assert self._rows_ok(h, M, C, dt, dev) and self._rows_ok(y, M, C, dt, dev)
+        pf32 = self._norm_params((out_weight, out_bias, gate, in_weight, in_bias), C, dt, dev, M // rows_per_gate if rows_per_gate else 0)
+        ho = h.new_empty((M, C)) if y is not None else None
+        u = h.new_empty((M, C)) if in_kind else None
+        stats = h.new_empty((M, 4), dtype=torch.float32) if keep_stats else None
+        self._launch("norm_residual_fwd", self.lib.bc_norm_residual_fwd, dev,
+                     (_ptr(ho), _ptr(u), _ptr(stats), h.data_ptr(), _ptr(y), _ptr(out_weight), _ptr(out_bias), _ptr(gate), _ptr(in_weight), _ptr(in_bias), M, C, self._ld(h),
+                      self._ld(y), rows_per_gate, residual_scale, eps, out_kind, in_kind, code, pf32))
         return ho, u, stats
 
     def norm_residual_bwd(self, gh, gu, stats, h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind: int, in_kind: int, residual_scale: float,
@@ -1103,19 +1132,19 @@ class HipBackend:
         """Gradients (dh, dy, d out_weight, d out_bias, d gate, d in_weight, d in_bias) of ``norm_residual_fwd``; ``want`` = seven truth values."""
         M, C = h.shape
         dt, dev = h.dtype, h.device
-        assert all(self._rows_ok(t, (M, C), dt, dev) for t in (gh, gu, h, y)) and stats.is_contiguous() and M > 0
+        code = _DTYPE_CODE[dt]
+        assert (self._rows_ok(gh, M, C, dt, dev) and self._rows_ok(gu, M, C, dt, dev) and self._rows_ok(h, M, C, dt, dev) and self._rows_ok(y, M, C, dt, dev)
+                and stats.is_contiguous() and M > 0)
         params = (out_weight, out_bias, gate, in_weight, in_bias)
-        pf32 = self._norm_params_ok(params, C, dt, dev, M // rows_per_gate if rows_per_gate else None)
-        ptr = lambda t: t.data_ptr() if t is not None else None
-        with torch.cuda.device_of(h):
-            dh = torch.empty((M, C), dtype=dt, device=dev) if want[0] else None
-            dy = torch.empty((M, C), dtype=dt, device=dev) if want[1] else None
-            dp = [torch.empty_like(t) if w and t is not None else None for t, w in zip(params, want[2:])]
-            need = self.lib.bc_norm_residual_bwd_workspace(M, C, int(rows_per_gate), _DTYPE_CODE[dt]) if any(t is not None for t in dp) else 0
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            self._check(self.lib.bc_norm_residual_bwd(ptr(dh), ptr(dy), *map(ptr, dp), ptr(gh), ptr(gu), ptr(stats), ptr(h), ptr(y), ptr(out_weight), ptr(out_bias), ptr(gate),
-                                                      ptr(in_weight), M, C, self._ld(h), self._ld(y), self._ld(gh), self._ld(gu), int(rows_per_gate), float(residual_scale),
-                                                      int(out_kind), int(in_kind), _DTYPE_CODE[dt], pf32, ptr(ws), need, self._stream()), "norm_residual_bwd")
+        pf32 = self._norm_params(params, C, dt, dev, M // rows_per_gate if rows_per_gate else 0)
+        dh = h.new_empty((M, C)) if want[0] else None
+        dy = h.new_empty((M, C)) if want[1] else None
+        dp = [p.new_empty(p.shape) if w and p is not None else None for p, w in zip(params, want[2:])]
+        need = self.lib.bc_norm_residual_bwd_workspace(M, C, rows_per_gate, code) if any(p is not None for p in dp) else 0
+        ws = h.new_empty(need, dtype=torch.uint8) if need else None
+        self._launch("norm_residual_bwd", self.lib.bc_norm_residual_bwd, dev,
+                     (_ptr(dh), _ptr(dy), *map(_ptr, dp), _ptr(gh), _ptr(gu), stats.data_ptr(), h.data_ptr(), _ptr(y), _ptr(out_weight), _ptr(out_bias), _ptr(gate),
+                      _ptr(in_weight), M, C, self._ld(h), self._ld(y), self._ld(gh), self._ld(gu), rows_per_gate, residual_scale, out_kind, in_kind, code, pf32, _ptr(ws), need))
         return (dh, dy, *dp)
 
     # -- network-input stage: window gather from the frame-state map + 7x7 / stride 2 stem conv (csrc/stem7x7.inc)

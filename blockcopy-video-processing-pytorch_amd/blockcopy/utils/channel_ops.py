@@ -19,6 +19,9 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from blockcopy.backend import BlockCopyBackendError, get_backend
+from blockcopy.core.tensorwrapper import TensorWrapper
+
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 NORMS = {"none": 0, "rms": 1, "layer": 2}
 MAX_NORM_CHANNELS = 16384
@@ -26,10 +29,8 @@ _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _backend(x):
-    from blockcopy.backend import BlockCopyBackendError, get_backend
-
     be = get_backend()
-    if be.name == "hip" and not x.is_cuda:
+    if not x.is_cuda and be.name == "hip":
         raise BlockCopyBackendError("channel operators need GPU tensors (no CPU path)")
     return be
 
@@ -57,6 +58,8 @@ def _features(x, dim, name):
 def _rows(x):
     """(rows, features) view of x, or of a contiguous copy where its strides allow none (features apart, overlapping rows)."""
     f = x.shape[-1]
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     if x.dim() != 2:
         try:
             x = x.view(-1, f) if x.numel() else x.reshape(x.numel() // f if f else 0, f)
@@ -94,19 +97,15 @@ def _wrapped(like, out, dim):
     if dim == 1:
         out = out.permute(0, 3, 1, 2)
     if like is not None:
-        from blockcopy.core.tensorwrapper import TensorWrapper
-
         return TensorWrapper._wrap_like(out, like, like.is_blocks)
     return out
 
 
 def _argument(x, dim, name):
     """(plain tensor with features last, TensorWrapper or None, effective dim)"""
-    from blockcopy.core.tensorwrapper import is_tensorwrapper
-
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name}: a tensor is needed, got {type(x).__name__}")
-    wrapper = x if is_tensorwrapper(x) and x.is_init else None
+    wrapper = x if isinstance(x, TensorWrapper) and x.is_init else None
     if wrapper is not None:
         dim = 1
     x = _plain(x)

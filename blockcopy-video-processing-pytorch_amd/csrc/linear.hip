@@ -227,17 +227,16 @@ template <typename S, int W> __device__ __forceinline__ void lin_save(S *p, cons
             if (e < cnt) p[e] = (S)f[e];
 }
 
-// 16 bytes' worth of consecutive outputs (m, n ..), cnt of them inside the matrix: sums v -> z, y.  The residual r is loaded by the caller, ahead
-template <int DT> __device__ __forceinline__ void lin_residual(float *r, const LinEpi &ep, int N, int m, int n)
+// W consecutive outputs (m, n ..; 16 bytes' worth), cnt of them inside the matrix: sums v -> z, y.  The residual r is loaded by the caller, ahead
+template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_residual(float *r, const LinEpi &ep, int N, int m, int n)
 {
     typedef typename LinT<DT>::S S;
-    lin_load<S, LinT<DT>::V>(r, (const S *)ep.res + (size_t)m * ep.ldr + n, N - n);
+    lin_load<S, W>(r, (const S *)ep.res + (size_t)m * ep.ldr + n, N - n);
 }
 
-template <int DT> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v, const float *r)
+template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v, const float *r)
 {
     typedef typename LinT<DT>::S S;
-    constexpr int W = LinT<DT>::V;
     const int cnt = N - n;
     const size_t at = (size_t)m * N + n;
     if (ep.bias) {
@@ -492,13 +491,66 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_join(const float 
     lin_epilogue<DT>(ep, N, (int)m, n, v, r);
 }
 
+// Few rows (a token, a handful of regions): bound by reading the weight once.  A workgroup takes 16 columns and all rows, its waves a share of the
+// sum each (slices of 64 bytes per weight row, four at a time: 256 bytes in a row), straight from memory into the matrix instruction, four
+// slices ahead; the waves' sums meet in the LDS in their order -- one launch, no partial sums in memory (1 x 4096 x 4096 bf16: the tile kernel
+// with 8 slices and their join 11.1 us).  MB x 16 rows
+template <int DT, int MB, int NW> __global__ __launch_bounds__(64 * NW) void k_lin_few(const LinArgs g)
+{
+    constexpr int V = LinT<DT>::V, SL = 4 * V, UN = 4;          // summed indexes of a slice, slices at a time
+    __shared__ f32x4 red[NW][MB][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int n0 = (int)blockIdx.x * 16, r = lane & 15, kl = (lane >> 4) * V;
+    const int rounds = (g.K + SL * UN - 1) / (SL * UN);
+    f32x4 acc[MB];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint4 w[UN], x[UN][MB];
+    auto ask = [&](int round) {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int k = (round * UN + u) * SL + kl;
+            w[u] = lin_fetch<DT, false>(g.a, g.N, g.K, n0 + r, k);
+#pragma unroll
+            for (int j = 0; j < MB; ++j) x[u][j] = lin_fetch<DT, false>(g.b, g.M, g.K, 16 * j + r, k);
+        }
+    };
+    if (wave < rounds) ask(wave);
+    for (int round = wave; round < rounds; round += NW) {
+        uint4 wc[UN], xc[UN][MB];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            wc[u] = w[u];
+#pragma unroll
+            for (int j = 0; j < MB; ++j) xc[u][j] = x[u][j];
+        }
+        if (round + NW < rounds) ask(round + NW);
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int j = 0; j < MB; ++j) lin_mma<DT>(acc[j], wc[u], xc[u][j]);
+    }
+#pragma unroll
+    for (int j = 0; j < MB; ++j) red[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= MB) return;
+    f32x4 s = red[0][wave][lane];
+    for (int q = 1; q < NW; ++q) s += red[q][wave][lane];
+    const int m = 16 * wave + r, n = n0 + 4 * (lane >> 4);
+    if (m >= g.M || n >= g.N) return;
+    float v[4] = {s[0], s[1], s[2], s[3]}, res[4];
+    if (g.ep.res) lin_residual<DT, 4>(res, g.ep, g.N, m, n);
+    lin_epilogue<DT, 4>(g.ep, g.N, m, n, v, res);
+}
+
 // dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.
 struct DactArgs {
     const void *gy, *z;         // z NULL: no activation, dz = gy is not stored
     void *dz;
-    float *part;                // [gridDim.y][N], or NULL: no sums asked for
-    long long ldg;
-    int M, N, span, act, tpr_log;
+    float *part;                // [gridDim.y][N] (one run of rows: not used, the sums go to db)
+    void *db;                   // NULL: no sums asked for
+    long long ldg, ldz;         // ldz: elements between the rows of dz
+    int M, N, span, act, tpr_log, db_f32;
 };
 
 template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactArgs a)
@@ -521,12 +573,12 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
                 lin_load<S, W>(z, (const S *)a.z + (size_t)m * a.N + n, cnt);
 #pragma unroll
                 for (int e = 0; e < W; ++e) d[e] *= lin_dact<DT>(z[e], a.act);
-                lin_save<S, W>((S *)a.dz + (size_t)m * a.N + n, d, cnt);
+                lin_save<S, W>((S *)a.dz + (size_t)m * a.ldz + n, d, cnt);
             }
 #pragma unroll
             for (int e = 0; e < W; ++e) sum[e] += d[e];
         }
-    if (!a.part) return;
+    if (!a.db) return;
 #pragma unroll
     for (int e = 0; e < W; ++e) red[e * 256 + tid] = sum[e];
     __syncthreads();
@@ -535,7 +587,10 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
         for (int e = 0; e < W; ++e) {
             float s = 0.f;
             for (int q = 0; q < rows; ++q) s += red[e * 256 + (q << a.tpr_log) + c];
-            if (e < cnt) a.part[(size_t)blockIdx.y * a.N + n + e] = s;
+            if (e >= cnt) continue;
+            if (gridDim.y > 1) a.part[(size_t)blockIdx.y * a.N + n + e] = s;
+            else if (a.db_f32) ((float *)a.db)[n + e] = s;
+            else ((S *)a.db)[n + e] = (S)s;
         }
 }
 
@@ -646,6 +701,19 @@ template <bool AMC, bool BMC> int lin_product(int dtype, LinArgs &g, const LinPl
     }
 }
 
+constexpr int LIN_FEW = 32;      // rows up to which the forward product takes k_lin_few
+
+template <int DT> int lin_few(const LinArgs &g, hipStream_t st)
+{
+    const unsigned wgs = ((unsigned)g.N + 15) / 16;
+    if (g.M <= 16) {        // 16 waves where there are too few columns to fill the chip with 8
+        if (wgs < LIN_CUS) k_lin_few<DT, 1, 16><<<wgs, 1024, 0, st>>>(g);
+        else k_lin_few<DT, 1, 8><<<wgs, 512, 0, st>>>(g);
+    } else
+        k_lin_few<DT, 2, 8><<<wgs, 512, 0, st>>>(g);
+    return lin_status();
+}
+
 inline bool lin_aligned(const void *p, int dtype) { return (uintptr_t)p % lin_esize(dtype) == 0; }
 
 int lin_sizes(long long M, int N, int K, int dtype)
@@ -679,13 +747,13 @@ DactPlan lin_dact_plan(long long M, int N, int dtype)
     return p;
 }
 
-template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, void *db, int db_f32, hipStream_t st)
+template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, hipStream_t st)
 {
     DactArgs a = a0;
     a.span = p.span;
     a.tpr_log = p.tpr_log;
     k_lin_dact<DT><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
-    if (db) k_lin_colsum<DT><<<(a.N + 15) / 16, 256, 0, st>>>(db, db_f32, a.part, (int)p.gy, a.N);
+    if (a.db && p.gy > 1) k_lin_colsum<DT><<<(a.N + 15) / 16, 256, 0, st>>>(a.db, a.db_f32, a.part, (int)p.gy, a.N);
     return lin_status();
 }
 
@@ -694,7 +762,7 @@ template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, void *
 BC_EXPORT long long bc_linear_fwd_workspace(long long M, int N, int K, int dtype)
 {
     if (lin_sizes(M, N, K, dtype) != BC_OK || M == 0) return 0;
-    return lin_part_bytes(lin_plan(dtype, M, N, K), M, N);
+    return M <= LIN_FEW ? 0 : lin_part_bytes(lin_plan(dtype, M, N, K), M, N);
 }
 
 BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, long long M, int N, int K, long long ldx,
@@ -707,7 +775,7 @@ BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, cons
     if (!y || !x || !w) return BC_ERR_NULL;
     if (!lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(y, dtype) || !lin_aligned(z, dtype) || !lin_aligned(residual, dtype)) return BC_ERR_ALIGN;
     const LinPlan p = lin_plan(dtype, M, N, K);
-    const long long need = lin_part_bytes(p, M, N);
+    const long long need = M <= LIN_FEW ? 0 : lin_part_bytes(p, M, N);
     if (need > 0 && !workspace) return BC_ERR_NULL;
     if (workspace_bytes < need) return BC_ERR_SHAPE;
     if (need > 0 && (uintptr_t)workspace % 16 != 0) return BC_ERR_ALIGN;
@@ -718,6 +786,8 @@ BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, cons
     g.N = N;
     g.K = K;
     g.ep = {y, z, bias, residual, ldr, bias_f32, act};
+    if (M <= LIN_FEW)
+        return dtype == DT_F32 ? lin_few<DT_F32>(g, (hipStream_t)stream) : dtype == DT_F16 ? lin_few<DT_F16>(g, (hipStream_t)stream) : lin_few<DT_BF16>(g, (hipStream_t)stream);
     return lin_product<false, false>(dtype, g, p, workspace, (hipStream_t)stream);
 }
 
@@ -765,13 +835,16 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
         a.gy = gy;
         a.z = act != ACT_NONE ? z : nullptr;
         a.dz = act != ACT_NONE ? wsp : nullptr;
-        a.part = db ? (float *)(wsp + s.dz) : nullptr;
+        a.part = (float *)(wsp + s.dz);
+        a.db = db;
+        a.db_f32 = bias_f32;
+        a.ldz = N;
         a.ldg = ldg;
         a.M = (int)M;
         a.N = N;
         a.act = act;
-        const int r = dtype == DT_F32 ? lin_dact_run<DT_F32>(a, p, db, bias_f32, st) : dtype == DT_F16 ? lin_dact_run<DT_F16>(a, p, db, bias_f32, st)
-                                                                                                     : lin_dact_run<DT_BF16>(a, p, db, bias_f32, st);
+        const int r = dtype == DT_F32 ? lin_dact_run<DT_F32>(a, p, st) : dtype == DT_F16 ? lin_dact_run<DT_F16>(a, p, st)
+                                                                                                     : lin_dact_run<DT_BF16>(a, p, st);
         if (r != BC_OK) return r;
         if (act != ACT_NONE) { dz = wsp; ldz = N; }
     }

@@ -97,17 +97,24 @@ template <int WPR, int NW> struct NrSum {
 // `cnt` of V elements at column `at` of row `base` (in elements).  With the base in scalar registers (whole waves share a row) a lane's address
 // is one 32-bit offset.  Rows of any width and start: the 16-byte accesses ask for the alignment of an element only (the hardware takes
 // unaligned vectors), the last vector of a row goes element by element.
+template <typename S, int V> struct NrVec { typedef S T __attribute__((ext_vector_type(V), aligned(sizeof(S)))); };
+
+template <typename S, int V> __device__ __forceinline__ typename NrVec<S, V>::T nr_raw(const void *q, size_t base, unsigned at, int cnt)
+{
+    typedef typename NrVec<S, V>::T SV;
+    const S *p = (const S *)q + base + at;
+    if (cnt >= V) return *(const SV *)p;
+    SV v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < cnt ? p[e] : (S)0.f;
+    return v;
+}
+
 template <typename S, int V> __device__ __forceinline__ void nr_load(float *f, const void *q, size_t base, unsigned at, int cnt)
 {
-    typedef S SV __attribute__((ext_vector_type(V), aligned(sizeof(S))));
-    const S *p = (const S *)q + base + at;
-    if (cnt >= V) {
-        const SV v = *(const SV *)p;
+    const typename NrVec<S, V>::T v = nr_raw<S, V>(q, base, at, cnt);
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = (float)v[e];
-    } else
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = e < cnt ? (float)p[e] : 0.f;
+    for (int e = 0; e < V; ++e) f[e] = (float)v[e];
 }
 
 template <typename S, int V> __device__ __forceinline__ void nr_store(void *q, size_t base, unsigned at, int cnt, const float *f)
@@ -139,6 +146,30 @@ template <typename S, int V> __device__ __forceinline__ void nr_param(float *f, 
             nr_load<float, V>(f, p, base, at, cnt);
     } else
         nr_load<S, V>(f, p, base, at, cnt);
+}
+
+// one row of a tensor as a lane holds it before its turn: NV vectors as they come from memory (requested a row ahead, so that the latency of
+// memory lies behind the row in hand)
+template <typename S, int V, int NV> struct NrRow {
+    typename NrVec<S, V>::T v[NV];
+    __device__ __forceinline__ void ask(const void *q, size_t base, const unsigned *col, const int *cnt, bool live)
+    {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (q && live) v[i] = nr_raw<S, V>(q, base, col[i], cnt[i]);
+            else
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[i][e] = (S)0.f;
+        }
+    }
+    __device__ __forceinline__ float at(int k) const { return (float)v[k / V][k % V]; }
+};
+
+// a parameter's channels of this lane, in registers for all its rows
+template <typename S, int V, int NV> __device__ __forceinline__ void nr_params(float *f, const void *p, int pf32, size_t base, const unsigned *col, const int *cnt, float none)
+{
+#pragma unroll
+    for (int i = 0; i < NV; ++i) nr_param<S, V>(f + i * V, p, pf32, base, col[i], cnt[i], none);
 }
 
 // x[E] -> normalised in place (0 behind the row's end); mean and 1 / deviation returned.  E = NV vectors of V
@@ -182,57 +213,73 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
         col[i] = (i * G + lr) * V;
         cnt[i] = a.C - (int)col[i];
     }
-    for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.M; r0 += (long long)gridDim.x * RPB) {      // (uniform: every wave meets every barrier)
-        const long long row = r0 + slot;
+    constexpr bool KEEP = WPR < 16;     // parameters and the next row stay in registers (16 waves leave a lane 128 of them: asked for at their turn)
+    const bool outer = a.y != nullptr && a.out_kind != NORM_NONE, inner = a.in_kind != NORM_NONE;
+    float wo[E], bo[E], gate[E], wi[E], bi[E];
+    if constexpr (KEEP) {
+        nr_params<S, V, NV>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+        nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV>(bi, a.bi, a.pf32, 0, col, cnt, 0.f);
+        if (!a.rows_per_gate) nr_params<S, V, NV>(gate, a.gate, a.pf32, 0, col, cnt, 1.f);
+    }
+    const long long hop = (long long)gridDim.x * RPB;
+    NrRow<S, V, NV> ry, rh;
+    long long row = (long long)blockIdx.x * RPB + slot;
+    if constexpr (KEEP) {
+        ry.ask(a.y, (size_t)row * a.ldy, col, cnt, row < a.M);
+        rh.ask(a.h, (size_t)row * a.ldh, col, cnt, row < a.M);
+    }
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.M; r0 += hop) {      // (uniform: every wave meets every barrier)
         const bool live = row < a.M;
-        const size_t gate_at = a.rows_per_gate ? (size_t)(row / a.rows_per_gate) * a.C : 0;
-        float x[E], w[V], b[V], mean_y = 0.f, rstd_y = 0.f, mean_h = 0.f, rstd_h = 0.f;
+        float x[E], mean_y = 0.f, rstd_y = 0.f, mean_h = 0.f, rstd_h = 0.f, h[E];
+        if constexpr (!KEEP) {
+            ry.ask(a.y, (size_t)row * a.ldy, col, cnt, live);
+            rh.ask(a.h, (size_t)row * a.ldh, col, cnt, live);
+        }
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = 0.f;
+        for (int i = 0; i < E; ++i) {
+            x[i] = ry.at(i);
+            h[i] = rh.at(i);
+        }
+        const long long next = row + hop;
+        if (KEEP && r0 + hop < a.M) {
+            ry.ask(a.y, (size_t)next * a.ldy, col, cnt, next < a.M);
+            rh.ask(a.h, (size_t)next * a.ldh, col, cnt, next < a.M);
+        }
         if (a.y) {
-            if (live)
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (cnt[i] > 0) nr_load<S, V>(x + i * V, a.y, (size_t)row * a.ldy, col[i], cnt[i]);
-            if (a.out_kind != NORM_NONE) {
+            if (!KEEP || a.rows_per_gate) nr_params<S, V, NV>(gate, live ? a.gate : nullptr, a.pf32, live && a.rows_per_gate ? (size_t)(row / a.rows_per_gate) * a.C : 0, col, cnt, 1.f);
+            if (outer) {
                 nr_normalise<V, NV>(x, a.out_kind, cnt, inv_c, a.eps, sum, mean_y, rstd_y);
+                if constexpr (!KEEP) {
+                    nr_params<S, V, NV>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+                    nr_params<S, V, NV>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+                }
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (cnt[i] > 0) {
-                        nr_param<S, V>(w, a.wo, a.pf32, 0, col[i], cnt[i], 1.f);
-                        nr_param<S, V>(b, a.bo, a.pf32, 0, col[i], cnt[i], 0.f);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) x[i * V + e] = x[i * V + e] * w[e] + b[e];
-                    }
+                for (int i = 0; i < E; ++i) x[i] = x[i] * wo[i] + bo[i];
             }
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = i % V < cnt[i / V] ? a.alpha * h[i] + gate[i] * x[i] : 0.f;
             if (live)
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (cnt[i] > 0) {
-                        nr_load<S, V>(b, a.h, (size_t)row * a.ldh, col[i], cnt[i]);
-                        nr_param<S, V>(w, a.gate, a.pf32, gate_at, col[i], cnt[i], 1.f);
+                for (int i = 0; i < NV; ++i) nr_store<S, V>(a.ho, (size_t)row * a.C, col[i], cnt[i], x + i * V);
+        } else
 #pragma unroll
-                        for (int e = 0; e < V; ++e) x[i * V + e] = a.alpha * b[e] + w[e] * x[i * V + e];
-                        nr_store<S, V>(a.ho, (size_t)row * a.C, col[i], cnt[i], x + i * V);
-                    }
-        } else if (live)
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (cnt[i] > 0) nr_load<S, V>(x + i * V, a.h, (size_t)row * a.ldh, col[i], cnt[i]);
-        if (a.in_kind != NORM_NONE) {
+            for (int i = 0; i < E; ++i) x[i] = h[i];
+        if (inner) {
             nr_normalise<V, NV>(x, a.in_kind, cnt, inv_c, a.eps, sum, mean_h, rstd_h);
+            if constexpr (!KEEP) {
+                nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+                nr_params<S, V, NV>(bi, a.bi, a.pf32, 0, col, cnt, 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = x[i] * wi[i] + bi[i];
             if (live)
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (cnt[i] > 0) {
-                        nr_param<S, V>(w, a.wi, a.pf32, 0, col[i], cnt[i], 1.f);
-                        nr_param<S, V>(b, a.bi, a.pf32, 0, col[i], cnt[i], 0.f);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) x[i * V + e] = x[i * V + e] * w[e] + b[e];
-                        nr_store<S, V>(a.u, (size_t)row * a.C, col[i], cnt[i], x + i * V);
-                    }
+                for (int i = 0; i < NV; ++i) nr_store<S, V>(a.u, (size_t)row * a.C, col[i], cnt[i], x + i * V);
         }
         if (a.stats && live && lr == 0) *(float4 *)(a.stats + 4 * row) = float4{mean_y, rstd_y, mean_h, rstd_h};
+        row = next;
     }
 }
 
@@ -265,7 +312,7 @@ template <int V, int NV, int NT> __device__ __forceinline__ void nr_put_sums(flo
 }
 
 template <int DT, int V, int NV, int WPR>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(const NormArgs a)
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ? 1 : 3) void k_norm_bwd(const NormArgs a)
 {
     typedef typename NrT<DT>::S S;
     constexpr int NT = WPR > 4 ? 64 * WPR : 256, NW = NT / 64, E = V * NV;
@@ -293,60 +340,61 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(const Nor
     float s_gate[E], s_wo[E], s_bo[E], s_wi[E], s_bi[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) s_gate[i] = s_wo[i] = s_bo[i] = s_wi[i] = s_bi[i] = 0.f;
+    constexpr bool KEEP = WPR < 16;     // (as in k_norm_fwd)
+    float wo[E], bo[E], gate[E], wi[E];
+    auto outer = [&]() {
+        nr_params<S, V, NV>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+        nr_params<S, V, NV>(gate, a.gate, a.pf32, gate_at, col, cnt, 1.f);
+    };
+    if constexpr (KEEP) {
+        outer();
+        nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+    }
 
+    NrRow<S, V, NV> rgh, ry, rh, rgu;
+    float4 rst;
+    auto ask = [&](int r) {
+        const bool live = r < last;
+        const long long row = base + r;
+        rst = live ? *(const float4 *)(a.stats + 4 * row) : float4{0.f, 0.f, 0.f, 0.f};
+        ry.ask(a.y, (size_t)row * a.ldy, col, cnt, live);
+        rh.ask(a.in_kind != NORM_NONE ? a.h : nullptr, (size_t)row * a.ldh, col, cnt, live);
+        rgu.ask(a.gu, (size_t)row * a.ldgu, col, cnt, live);
+        rgh.ask(a.gh, (size_t)row * a.ldgh, col, cnt, live);
+    };
+    if constexpr (KEEP) ask(first + slot);
     for (int r0 = first; r0 < last; r0 += RPB) {
         const bool live = r0 + slot < last;
-        const long long row = base + r0 + slot;
-        float n[E], g[E], p[E], w[V], b[V];      // normalised y; normalised h', then the gradient of h'; working row
-        float4 st = {0.f, 0.f, 0.f, 0.f};
-        if (live) st = *(const float4 *)(a.stats + 4 * row);
+        const size_t out = (size_t)(base + r0 + slot) * a.C;
+        if constexpr (!KEEP) ask(r0 + slot);
+        float n[E], g[E], p[E], hn[E];      // normalised y; gradient of h'; working row; normalised h'
+        const float4 st = rst;
 #pragma unroll
-        for (int i = 0; i < E; ++i) n[i] = g[i] = p[i] = 0.f;
-        if (live)
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (cnt[i] > 0) {
-                    if (a.gh) nr_load<S, V>(g + i * V, a.gh, (size_t)row * a.ldgh, col[i], cnt[i]);
-                    if (a.y) nr_load<S, V>(n + i * V, a.y, (size_t)row * a.ldy, col[i], cnt[i]);
-                }
+        for (int i = 0; i < E; ++i) {
+            n[i] = ry.at(i);
+            g[i] = rgh.at(i);
+            hn[i] = rh.at(i);
+            p[i] = rgu.at(i);
+        }
+        if (KEEP && r0 + RPB < last) ask(r0 + RPB + slot);
+        // (rows and channels that do not exist are zeros from here on: gradients zero, normalised values forced to zero)
         if (a.out_kind != NORM_NONE)
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < V; ++e) n[i * V + e] = live && e < cnt[i] ? (n[i * V + e] - st.x) * st.y : 0.f;
+            for (int i = 0; i < E; ++i) n[i] = i % V < cnt[i / V] ? (n[i] - st.x) * st.y : 0.f;
         if (a.in_kind != NORM_NONE) {
-            float hn[E];
-#pragma unroll
-            for (int i = 0; i < E; ++i) hn[i] = 0.f;
-            if (live)
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (cnt[i] > 0) {
-                        nr_load<S, V>(hn + i * V, a.h, (size_t)row * a.ldh, col[i], cnt[i]);
-                        if (a.y) {
-                            float t[V];
-                            nr_param<S, V>(w, a.wo, a.pf32, 0, col[i], cnt[i], 1.f);
-                            nr_param<S, V>(b, a.bo, a.pf32, 0, col[i], cnt[i], 0.f);
-#pragma unroll
-                            for (int e = 0; e < V; ++e) t[e] = n[i * V + e] * w[e] + b[e];
-                            nr_param<S, V>(w, a.gate, a.pf32, gate_at, col[i], cnt[i], 1.f);
-#pragma unroll
-                            for (int e = 0; e < V; ++e) hn[i * V + e] = a.alpha * hn[i * V + e] + w[e] * t[e];
-                        }
-                        if (a.gu) nr_load<S, V>(p + i * V, a.gu, (size_t)row * a.ldgu, col[i], cnt[i]);
-                        nr_param<S, V>(w, a.wi, a.pf32, 0, col[i], cnt[i], 1.f);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const int k = i * V + e;
-                            hn[k] = e < cnt[i] ? (hn[k] - st.z) * st.w : 0.f;
-                            s_wi[k] += p[k] * hn[k];
-                            s_bi[k] += p[k];
-                            p[k] *= w[e];
-                        }
-                    }
             float m1 = 0.f, m2 = 0.f;
+            if constexpr (!KEEP) {
+                outer();
+                nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+            }
 #pragma unroll
             for (int i = 0; i < E; ++i) {
+                if (a.y) hn[i] = a.alpha * hn[i] + gate[i] * (n[i] * wo[i] + bo[i]);
+                hn[i] = i % V < cnt[i / V] ? (hn[i] - st.z) * st.w : 0.f;
+                s_wi[i] += p[i] * hn[i];
+                s_bi[i] += p[i];
+                p[i] *= wi[i];
                 m1 += p[i] * hn[i];
                 m2 += p[i];
             }
@@ -358,35 +406,26 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(const Nor
         }
         if (a.need_dh && live)
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (cnt[i] > 0) {
+            for (int i = 0; i < NV; ++i) {
+                float d[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) b[e] = a.alpha * g[i * V + e];
-                    nr_store<S, V>(a.dh, (size_t)row * a.C, col[i], cnt[i], b);
-                }
+                for (int e = 0; e < V; ++e) d[e] = a.alpha * g[i * V + e];
+                nr_store<S, V>(a.dh, out, col[i], cnt[i], d);
+            }
         if (!a.y) continue;
+        if constexpr (!KEEP) outer();
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (cnt[i] > 0 && live) {
-                float t[V];
-                nr_param<S, V>(w, a.wo, a.pf32, 0, col[i], cnt[i], 1.f);
-                nr_param<S, V>(b, a.bo, a.pf32, 0, col[i], cnt[i], 0.f);
-#pragma unroll
-                for (int e = 0; e < V; ++e) t[e] = n[i * V + e] * w[e] + b[e];
-                nr_param<S, V>(b, a.gate, a.pf32, gate_at, col[i], cnt[i], 1.f);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const int k = i * V + e;
-                    s_gate[k] += g[k] * t[e];
-                    const float q = g[k] * b[e];
-                    s_wo[k] += q * n[k];
-                    s_bo[k] += q;
-                    p[k] = q * w[e];
-                    m1 += p[k] * n[k];
-                    m2 += p[k];
-                }
-            }
+        for (int i = 0; i < E; ++i) {
+            if (!(live && i % V < cnt[i / V])) g[i] = 0.f;
+            s_gate[i] += g[i] * (n[i] * wo[i] + bo[i]);
+            const float q = g[i] * gate[i];
+            s_wo[i] += q * n[i];
+            s_bo[i] += q;
+            p[i] = q * wo[i];
+            m1 += p[i] * n[i];
+            m2 += p[i];
+        }
         if (a.out_kind != NORM_NONE) {
             sum(m1, m2, a.out_kind == NORM_LAYER);
             m1 *= inv_c;
@@ -396,8 +435,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(const Nor
         }
         if (a.need_dy && live)
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (cnt[i] > 0) nr_store<S, V>(a.dy, (size_t)row * a.C, col[i], cnt[i], p + i * V);
+            for (int i = 0; i < NV; ++i) nr_store<S, V>(a.dy, out, col[i], cnt[i], p + i * V);
     }
     if (!a.part) return;
     float *dst = a.part + (size_t)blockIdx.x * 5 * a.C;
@@ -428,6 +466,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_join(const NormJ
     const int b0 = per_group ? (int)blockIdx.z * a.chunks : 0, nb = per_group ? a.chunks : a.blocks;
     float s = 0.f;
     if (c < a.C)
+#pragma unroll 8
         for (int b = run; b < nb; b += 16) s += a.part[((size_t)(b0 + b) * 5 + which) * a.C + c];
     red[threadIdx.x] = s;
     __syncthreads();
@@ -504,14 +543,17 @@ int nr_check(long long M, int C, int dtype, int out_kind, int in_kind, long long
     return BC_OK;
 }
 
-// about two workgroups per CU, the rows of a gate group divided evenly among whole workgroups
+// as many workgroups as run at once (three of four waves per CU for 16-bit rows, two for fp32), the rows of a gate group divided evenly among
+// whole workgroups
 struct NormChunks { int chunks, span, groups; };
-NormChunks nr_chunks(long long M, long long rows_per_gate, int rows_per_block)
+NormChunks nr_chunks(long long M, long long rows_per_gate, int dtype, const NormShape &s)
 {
+    const int rows_per_block = nr_rows_per_block(s);
     NormChunks c;
     const long long per = rows_per_gate ? rows_per_gate : M;
     c.groups = (int)(M / per);
-    long long n = (512 + c.groups - 1) / c.groups;
+    const int want = dtype == DT_F32 || s.WPR > 4 ? 512 : 768;
+    long long n = (want + c.groups - 1) / c.groups;
     const long long most = (per + rows_per_block - 1) / rows_per_block;
     if (n > most) n = most;
     long long span = (per + n - 1) / n;
@@ -547,13 +589,13 @@ BC_EXPORT int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const voi
     const NormShape s = nr_shape(C);
     a.g_log = s.g_log;
     const long long blocks = (M + nr_rows_per_block(s) - 1) / nr_rows_per_block(s);
-    return nr_dispatch(dtype, false, a, s, (unsigned)(blocks < 8192 ? blocks : 8192), (hipStream_t)stream);
+    return nr_dispatch(dtype, false, a, s, (unsigned)(blocks < 4096 ? blocks : 4096), (hipStream_t)stream);
 }
 
 BC_EXPORT long long bc_norm_residual_bwd_workspace(long long M, int C, long long rows_per_gate, int dtype)
 {
     if (M < 1 || C < 1 || C > NR_MAX_C || dtype < 0 || dtype > 2 || rows_per_gate < 0 || (rows_per_gate && M % rows_per_gate)) return 0;
-    const NormChunks c = nr_chunks(M, rows_per_gate, nr_rows_per_block(nr_shape(C)));
+    const NormChunks c = nr_chunks(M, rows_per_gate, dtype, nr_shape(C));
     return 20ll * C * c.chunks * c.groups;
 }
 
@@ -574,7 +616,7 @@ BC_EXPORT int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void 
         if (ps[i] && (uintptr_t)ps[i] % pe) return BC_ERR_ALIGN;
     if ((uintptr_t)stats % 16) return BC_ERR_ALIGN;
     const NormShape s = nr_shape(C);
-    const NormChunks c = nr_chunks(M, rows_per_gate, nr_rows_per_block(s));
+    const NormChunks c = nr_chunks(M, rows_per_gate, dtype, s);
     const bool sums = d_out_weight || d_out_bias || d_gate || d_in_weight || d_in_bias;
     if (sums && !workspace) return BC_ERR_NULL;
     if (sums && workspace_bytes < 20ll * C * c.chunks * c.groups) return BC_ERR_SHAPE;

@@ -122,8 +122,8 @@ def test_c_entries_validate_before_any_device_call():
     assert lin(M=0) == 0 and lin(M=-1) == -2 and lin(n=0) == -2 and lin(k=0) == -2 and lin(dt=3) == -3 and lin(act=5) == -2 and lin(act=-1) == -2
     assert lin(ldx=15) == -2 and lin(ldw=15) == -2 and lin(res=256, ldr=7) == -2 and lin(y=N) == -1 and lin(x=N) == -1 and lin(w=N) == -1
     assert lin(x=258) == -5 and lin(M=1 << 31) == -4
-    need = lib.bc_linear_fwd_workspace(4, 8, 1 << 16, 0)
-    assert need > 0 and lin(k=1 << 16, ldx=1 << 16, ldw=1 << 16) == -1 and lin(k=1 << 16, ldx=1 << 16, ldw=1 << 16, ws=256, wsb=need - 1) == -2
+    need = lib.bc_linear_fwd_workspace(100, 8, 1 << 16, 0)
+    assert need > 0 and lin(M=100, k=1 << 16, ldx=1 << 16, ldw=1 << 16) == -1 and lin(M=100, k=1 << 16, ldx=1 << 16, ldw=1 << 16, ws=256, wsb=need - 1) == -2
     bwd = lambda *, dx=256, dw=256, db=256, gy=256, z=256, x=256, w=256, M=4, n=8, k=16, ldg=8, ldx=16, ldw=16, act=1, dt=0, ws=256, wsb=1 << 30: lib.bc_linear_bwd(
         dx, dw, db, gy, z, x, w, M, n, k, ldg, ldx, ldw, act, dt, 0, ws, wsb, N)
     assert bwd(M=0) == -2 and bwd(gy=N) == -1 and bwd(z=N) == -1 and bwd(x=N) == -1 and bwd(w=N) == -1 and bwd(ldg=7) == -2 and bwd(ws=N) == -1
