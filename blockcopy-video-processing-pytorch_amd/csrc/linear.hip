@@ -104,6 +104,7 @@ template <int DT> __device__ __forceinline__ float lin_dact(float z, int act)
 struct LinOperand {
     const void *p;
     long long ld;       // elements between consecutive rows of memory
+    int run;            // readable elements of a row of memory
 };
 
 struct LinEpi {
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
         for (int i = 0; i < NA; ++i) {
             const int v = lin_place<DT, AMC, BN, C>(tid + NT * i);
             if constexpr (AMC) {
-                const int k = v / (BN / V), c = v % (BN / V), n = n0 + c * V + V <= g.N ? c * V : g.N - V - n0;
+                const int k = v / (BN / V), c = v % (BN / V), n = n0 + c * V + V <= g.a.run ? c * V : g.a.run - V - n0;
                 oa[i] = (unsigned)((long long)k * g.a.ld + n) * ES;
             } else {
                 const int row = n0 + v / C < g.N ? v / C : g.N - 1 - n0;
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
         for (int i = 0; i < NB; ++i) {
             const int v = lin_place<DT, BMC, BM, C>(tid + NT * i);
             if constexpr (BMC) {
-                const int k = v / (BM / V), c = v % (BM / V), m = m0 + c * V + V <= g.M ? c * V : g.M - V - m0;
+                const int k = v / (BM / V), c = v % (BM / V), m = m0 + c * V + V <= g.b.run ? c * V : g.b.run - V - m0;
                 ob[i] = (unsigned)((long long)k * g.b.ld + m) * ES;
             } else {
                 const int row = m0 + v / C < g.M ? v / C : g.M - 1 - m0;
@@ -545,8 +546,8 @@ template <int DT, int MB, int NW> __global__ __launch_bounds__(64 * NW) void k_l
 
 // dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.
 struct DactArgs {
-    const void *gy, *z;         // z NULL: no activation, dz = gy is not stored
-    void *dz;
+    const void *gy, *z;         // z NULL: no activation, dz = gy
+    void *dz;                   // NULL: not stored
     float *part;                // [gridDim.y][N] (one run of rows: not used, the sums go to db)
     void *db;                   // NULL: no sums asked for
     long long ldg, ldz;         // ldz: elements between the rows of dz
@@ -573,8 +574,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
                 lin_load<S, W>(z, (const S *)a.z + (size_t)m * a.N + n, cnt);
 #pragma unroll
                 for (int e = 0; e < W; ++e) d[e] *= lin_dact<DT>(z[e], a.act);
-                lin_save<S, W>((S *)a.dz + (size_t)m * a.ldz + n, d, cnt);
             }
+            if (a.dz) lin_save<S, W>((S *)a.dz + (size_t)m * a.ldz + n, d, cnt);
 #pragma unroll
             for (int e = 0; e < W; ++e) sum[e] += d[e];
         }
@@ -592,6 +593,23 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
             else if (a.db_f32) ((float *)a.db)[n + e] = s;
             else ((S *)a.db)[n + e] = (S)s;
         }
+}
+
+// rows of any start and width -> rows that start on 16 bytes (ldo elements apart, a multiple of a vector; the columns behind the row's end are
+// zeros): two elements per thread, whole 4-byte words written
+template <int DT> __global__ __launch_bounds__(256) void k_lin_pack(void *out, const void *in, long long ld, int rows, int len, int ldo)
+{
+    typedef typename LinT<DT>::S S;
+    typedef S S2 __attribute__((ext_vector_type(2)));
+    const unsigned pairs = (unsigned)ldo / 2;
+    for (size_t id = (size_t)blockIdx.x * 256 + threadIdx.x; id < (size_t)rows * pairs; id += (size_t)gridDim.x * 256) {
+        const unsigned row = (unsigned)(id / pairs), c = (unsigned)(id - (size_t)row * pairs) * 2;
+        const S *p = (const S *)in + (size_t)row * ld + c;
+        S2 v;
+        v[0] = c < (unsigned)len ? p[0] : (S)0.f;
+        v[1] = c + 1 < (unsigned)len ? p[1] : (S)0.f;
+        *(S2 *)((S *)out + (size_t)row * ldo + c) = v;
+    }
 }
 
 // 16 columns x 16 runs of partial sums per workgroup, joined in order
@@ -649,10 +667,10 @@ inline long long lin_part_bytes(const LinPlan &p, long long M, long long N) { re
 inline int lin_esize(int dtype) { return dtype == DT_F32 ? 4 : 2; }
 
 // may an operand travel global -> LDS directly: aligned 16-byte vectors that never straddle a row's end, offsets inside a tile below 2^31
-inline bool lin_direct(const LinOperand &o, long long rows, bool mc, int dtype)
+inline bool lin_direct(const LinOperand &o, bool mc, int dtype)
 {
     const int e = lin_esize(dtype), v = 16 / e;
-    return (uintptr_t)o.p % 16 == 0 && o.ld % v == 0 && (!mc || rows % v == 0) && o.ld * e * 256 < 0x7fffffffll;
+    return (uintptr_t)o.p % 16 == 0 && o.ld % v == 0 && (!mc || o.run % v == 0) && o.ld * e * 256 < 0x7fffffffll;
 }
 
 template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C> int lin_run(LinArgs &g, const LinPlan &p, hipStream_t st)
@@ -667,7 +685,7 @@ template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIREC
 template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *ws, hipStream_t st)
 {
     g.part = p.slices > 1 ? (float *)ws : nullptr;
-    const bool direct = lin_direct(g.a, g.N, AMC, DT) && lin_direct(g.b, g.M, BMC, DT);
+    const bool direct = lin_direct(g.a, AMC, DT) && lin_direct(g.b, BMC, DT);
     if (!direct && p.edge == 256) {     // (the register route has no large tile)
         p.edge = 128;
         p.tm = (unsigned)(((long long)g.M + 127) / 128);
@@ -701,8 +719,6 @@ template <bool AMC, bool BMC> int lin_product(int dtype, LinArgs &g, const LinPl
     }
 }
 
-constexpr int LIN_FEW = 32;      // rows up to which the forward product takes k_lin_few
-
 template <int DT> int lin_few(const LinArgs &g, hipStream_t st)
 {
     const unsigned wgs = ((unsigned)g.N + 15) / 16;
@@ -725,6 +741,28 @@ int lin_sizes(long long M, int N, int K, int dtype)
         (((long long)N + 63) / 64) * (((long long)K + 63) / 64) > 0x7fffff00ll)
         return BC_ERR_RANGE;
     return BC_OK;
+}
+
+// Is it worth bringing operands whose rows do not start on 16 bytes into order first?  The register route takes about twice the direct one's time
+// (16 bits: 4.3 GFLOP 22 us against 11, 69 GFLOP 104 against 58, its weight gradient 272 against 110; fp32: 4.2 GFLOP 65 against 42), the copy two
+// passes over the operands and a launch: worth it from about 2 GFLOP on, unless one side is so short that the copy outweighs the products
+inline bool lin_worth(long long M, long long N, long long K) { return (double)M * (double)N * (double)K >= 1e9 && M * N >= 200 * (M + N); }
+inline int lin_padded(long long len, int dtype) { return (int)lin_round(len, 16 / lin_esize(dtype)); }
+inline long long lin_pack_bytes(long long rows, long long len, int dtype) { return lin_round(rows * lin_padded(len, dtype) * lin_esize(dtype), 256); }
+
+// the operand in order, in the workspace at *ws (moved on)
+LinOperand lin_pack(const LinOperand &o, long long rows, char **ws, int dtype, hipStream_t st)
+{
+    const LinOperand r = {*ws, lin_padded(o.run, dtype), lin_padded(o.run, dtype)};
+    const long long words = rows * r.ld / 2;
+    const unsigned grid = (unsigned)((words + 1023) / 1024 < 4096 ? (words + 1023) / 1024 : 4096);
+    switch (dtype) {
+    case DT_F32: k_lin_pack<DT_F32><<<grid, 256, 0, st>>>(*ws, o.p, o.ld, (int)rows, o.run, (int)r.ld); break;
+    case DT_F16: k_lin_pack<DT_F16><<<grid, 256, 0, st>>>(*ws, o.p, o.ld, (int)rows, o.run, (int)r.ld); break;
+    default: k_lin_pack<DT_BF16><<<grid, 256, 0, st>>>(*ws, o.p, o.ld, (int)rows, o.run, (int)r.ld);
+    }
+    *ws += lin_pack_bytes(rows, o.run, dtype);
+    return r;
 }
 
 struct DactPlan { int tpr_log, span; unsigned gx, gy; };
@@ -759,10 +797,20 @@ template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, hipStr
 
 }  // namespace
 
+// does the forward product take k_lin_few: few rows, and enough columns to fill part of the chip or a short sum (8 x 8192 x 128 13 us there, 7 as
+// tiles); 16-bit rows must start on 4 bytes (13 x 2047 x 1001: 13 us against 8, 13 x 2046 x 1001: 5.8).  Beyond 16 rows only short sums
+// (32 x 1024 x 1024 4.8 us against 6.0, 32 x 4096 x 4096 14 against 11)
+static bool lin_takes_few(const void *x, const void *w, long long M, int N, int K, long long ldx, long long ldw, int dtype)
+{
+    if (M > 32 || (M > 16 && K > 1024) || (N < 1024 && K > 2048)) return false;
+    return dtype == DT_F32 || ((uintptr_t)x % 4 == 0 && (uintptr_t)w % 4 == 0 && ldx % 2 == 0 && ldw % 2 == 0);
+}
+
 BC_EXPORT long long bc_linear_fwd_workspace(long long M, int N, int K, int dtype)
 {
     if (lin_sizes(M, N, K, dtype) != BC_OK || M == 0) return 0;
-    return M <= LIN_FEW ? 0 : lin_part_bytes(lin_plan(dtype, M, N, K), M, N);
+    const long long pack = K % (16 / lin_esize(dtype)) && lin_worth(M, N, K) ? lin_pack_bytes(M, K, dtype) + lin_pack_bytes(N, K, dtype) : 0;
+    return lin_part_bytes(lin_plan(dtype, M, N, K), M, N) + pack;
 }
 
 BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, long long M, int N, int K, long long ldx,
@@ -774,32 +822,45 @@ BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, cons
     if (M == 0) return BC_OK;
     if (!y || !x || !w) return BC_ERR_NULL;
     if (!lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(y, dtype) || !lin_aligned(z, dtype) || !lin_aligned(residual, dtype)) return BC_ERR_ALIGN;
-    const LinPlan p = lin_plan(dtype, M, N, K);
-    const long long need = M <= LIN_FEW ? 0 : lin_part_bytes(p, M, N);
+    if (bias && (uintptr_t)bias % (bias_f32 ? 4 : lin_esize(dtype))) return BC_ERR_ALIGN;
+    const long long need = bc_linear_fwd_workspace(M, N, K, dtype);
     if (need > 0 && !workspace) return BC_ERR_NULL;
     if (workspace_bytes < need) return BC_ERR_SHAPE;
-    if (need > 0 && (uintptr_t)workspace % 16 != 0) return BC_ERR_ALIGN;
+    if (need > 0 && (uintptr_t)workspace % 256 != 0) return BC_ERR_ALIGN;
+    hipStream_t st = (hipStream_t)stream;
+    const LinPlan p = lin_plan(dtype, M, N, K);
     LinArgs g = {};
-    g.a = {w, ldw};
-    g.b = {x, ldx};
+    g.a = {w, ldw, K};
+    g.b = {x, ldx, K};
     g.M = (int)M;
     g.N = N;
     g.K = K;
     g.ep = {y, z, bias, residual, ldr, bias_f32, act};
-    if (M <= LIN_FEW)
-        return dtype == DT_F32 ? lin_few<DT_F32>(g, (hipStream_t)stream) : dtype == DT_F16 ? lin_few<DT_F16>(g, (hipStream_t)stream) : lin_few<DT_BF16>(g, (hipStream_t)stream);
-    return lin_product<false, false>(dtype, g, p, workspace, (hipStream_t)stream);
+    if (lin_takes_few(x, w, M, N, K, ldx, ldw, dtype))
+        return dtype == DT_F32 ? lin_few<DT_F32>(g, st) : dtype == DT_F16 ? lin_few<DT_F16>(g, st) : lin_few<DT_BF16>(g, st);
+    char *free_ws = (char *)workspace + lin_part_bytes(p, M, N);
+    if (K % (16 / lin_esize(dtype)) && lin_worth(M, N, K)) {
+        if (!lin_direct(g.a, false, dtype)) g.a = lin_pack(g.a, N, &free_ws, dtype, st);
+        if (!lin_direct(g.b, false, dtype)) g.b = lin_pack(g.b, M, &free_ws, dtype, st);
+    }
+    return lin_product<false, false>(dtype, g, p, workspace, st);
 }
 
-// the workspace of a backward pass: dz (activations only), the column sums' partials, and the slices of one product at a time
-struct LinBwdSpace { long long dz, part, slices; };
+// the workspace of a backward pass: dz (with an activation, or where gy is brought into order), the column sums' partials, the slices of one
+// product at a time, and x and w in order.  What is brought into order goes by the sizes alone, here and in the call
+struct LinBwdSpace { long long dz, part, slices, pack; bool order_n, order_k; };
 static LinBwdSpace lin_bwd_space(long long M, int N, int K, int act, int dtype)
 {
     LinBwdSpace s;
-    s.dz = act != ACT_NONE ? lin_round(M * N * lin_esize(dtype), 256) : 0;
+    const int v = 16 / lin_esize(dtype);
+    const bool worth = lin_worth(M, N, K);
+    s.order_n = N % v && worth;
+    s.order_k = K % v && worth;
+    s.dz = act != ACT_NONE || s.order_n ? lin_pack_bytes(M, N, dtype) : 0;
     s.part = lin_round(4ll * N * lin_dact_plan(M, N, dtype).gy, 256);
     const long long x = lin_part_bytes(lin_plan(dtype, M, K, N), M, K), w = lin_part_bytes(lin_plan(dtype, N, K, M), N, K);
     s.slices = x > w ? x : w;
+    s.pack = s.order_k ? lin_pack_bytes(M, K, dtype) + lin_pack_bytes(N, K, dtype) : 0;
     return s;
 }
 
@@ -807,7 +868,7 @@ BC_EXPORT long long bc_linear_bwd_workspace(long long M, int N, int K, int act, 
 {
     if (lin_sizes(M, N, K, dtype) != BC_OK || M == 0 || act < 0 || act >= ACT_COUNT) return 0;
     const LinBwdSpace s = lin_bwd_space(M, N, K, act, dtype);
-    return s.dz + s.part + s.slices;
+    return s.dz + s.part + s.slices + s.pack;
 }
 
 BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const void *z, const void *x, const void *w, long long M, int N, int K, long long ldg,
@@ -820,53 +881,55 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
     if (!gy || (act != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return BC_ERR_NULL;
     if (!lin_aligned(gy, dtype) || !lin_aligned(z, dtype) || !lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(dx, dtype) || !lin_aligned(dw, dtype))
         return BC_ERR_ALIGN;
+    if (db && (uintptr_t)db % (bias_f32 ? 4 : lin_esize(dtype))) return BC_ERR_ALIGN;
     const LinBwdSpace s = lin_bwd_space(M, N, K, act, dtype);
-    if (s.dz + s.part + s.slices > 0 && !workspace) return BC_ERR_NULL;
-    if (workspace_bytes < s.dz + s.part + s.slices) return BC_ERR_SHAPE;
+    if (!workspace) return BC_ERR_NULL;
+    if (workspace_bytes < s.dz + s.part + s.slices + s.pack) return BC_ERR_SHAPE;
     if ((uintptr_t)workspace % 256 != 0) return BC_ERR_ALIGN;
     hipStream_t st = (hipStream_t)stream;
-    char *wsp = (char *)workspace;
+    char *wsp = (char *)workspace, *pack = wsp + s.dz + s.part + s.slices;
     void *slices = wsp + s.dz + s.part;
-    const void *dz = gy;
-    long long ldz = ldg;
-    if (act != ACT_NONE || db) {
+    LinOperand dz = {gy, ldg, N};
+    const bool store = act != ACT_NONE || (s.order_n && !lin_direct(dz, true, dtype));
+    if (store || db) {
         const DactPlan p = lin_dact_plan(M, N, dtype);
         DactArgs a = {};
         a.gy = gy;
         a.z = act != ACT_NONE ? z : nullptr;
-        a.dz = act != ACT_NONE ? wsp : nullptr;
+        a.dz = store ? wsp : nullptr;
         a.part = (float *)(wsp + s.dz);
         a.db = db;
         a.db_f32 = bias_f32;
-        a.ldz = N;
         a.ldg = ldg;
+        a.ldz = lin_padded(N, dtype);       // (what lies behind a row's end is never part of a stored sum)
         a.M = (int)M;
         a.N = N;
         a.act = act;
-        const int r = dtype == DT_F32 ? lin_dact_run<DT_F32>(a, p, st) : dtype == DT_F16 ? lin_dact_run<DT_F16>(a, p, st)
-                                                                                                     : lin_dact_run<DT_BF16>(a, p, st);
+        const int r = dtype == DT_F32 ? lin_dact_run<DT_F32>(a, p, st) : dtype == DT_F16 ? lin_dact_run<DT_F16>(a, p, st) : lin_dact_run<DT_BF16>(a, p, st);
         if (r != BC_OK) return r;
-        if (act != ACT_NONE) { dz = wsp; ldz = N; }
+        if (store) dz = {wsp, a.ldz, (int)a.ldz};
     }
     if (dx) {       // dx[m][k] = sum_n dz[m][n] w[n][k]: the weight runs across the summed index
         LinArgs g = {};
-        g.a = {w, ldw};
-        g.b = {dz, ldz};
+        g.a = {w, ldw, K};
+        if (s.order_k && !lin_direct(g.a, true, dtype)) g.a = lin_pack(g.a, N, &pack, dtype, st);
+        g.b = {dz.p, dz.ld, N};
         g.M = (int)M;
         g.N = K;
         g.K = N;
-                g.ep = {dx, nullptr, nullptr, nullptr, 0, 0, ACT_NONE};
+        g.ep = {dx, nullptr, nullptr, nullptr, 0, 0, ACT_NONE};
         const int r = lin_product<true, false>(dtype, g, lin_plan(dtype, M, K, N), slices, st);
         if (r != BC_OK) return r;
     }
     if (dw) {       // dw[n][k] = sum_m dz[m][n] x[m][k]: both run across it
         LinArgs g = {};
-        g.a = {x, ldx};
-        g.b = {dz, ldz};
+        g.a = {x, ldx, K};
+        if (s.order_k && !lin_direct(g.a, true, dtype)) g.a = lin_pack(g.a, M, &pack, dtype, st);
+        g.b = dz;
         g.M = N;
         g.N = K;
         g.K = (int)M;
-                g.ep = {dw, nullptr, nullptr, nullptr, 0, 0, ACT_NONE};
+        g.ep = {dw, nullptr, nullptr, nullptr, 0, 0, ACT_NONE};
         const int r = lin_product<true, true>(dtype, g, lin_plan(dtype, N, K, M), slices, st);
         if (r != BC_OK) return r;
     }

@@ -283,32 +283,33 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
     }
 }
 
-// the five column sums of a workgroup: its rows' lanes with the same channels meet in the LDS, in the order of the rows' slots
-template <int V, int NV, int NT> __device__ __forceinline__ void nr_put_sums(float *lds, float *dst, const float *acc, const unsigned *col, const int *cnt, int tid, int G, int RPB)
+// the five column sums of a workgroup: lanes of a wave that hold the same channels of different rows add up by exchange, the waves' sums meet
+// in the LDS in the order of the waves
+template <int V, int NV, int WPR, int NW> __device__ __forceinline__ void nr_put_sums(float *lds, float *dst, float *acc, const unsigned *col, const int *cnt, int wave, int lr, int g_log)
 {
-    if (RPB == 1) {
+    constexpr int E = V * NV, ROWS = WPR > 4 ? 1 : 4 / WPR;       // groups of waves with rows of their own
+    if constexpr (WPR == 1)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (cnt[i] > 0)
+        for (int i = 0; i < E; ++i)
+            for (int m = 1 << g_log; m < 64; m <<= 1) acc[i] += __shfl_xor(acc[i], m);
+    if constexpr (ROWS > 1) {
+        const int lane = threadIdx.x & 63;
+        __syncthreads();
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (e < cnt[i]) dst[col[i] + e] = acc[i * V + e];
-        return;
+        for (int i = 0; i < E; ++i) lds[i * 256 + threadIdx.x] = acc[i];
+        __syncthreads();
+        if (wave >= WPR || (WPR == 1 && lane >> g_log)) return;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            float t = 0.f;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) t += lds[i * 256 + r * 64 * WPR + lr];
+            acc[i] = t;
+        }
     }
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NV * V; ++i) lds[i * NT + tid] = acc[i];
-    __syncthreads();
-    if (tid < G)
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (cnt[i] > 0)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float s = 0.f;
-                    for (int r = 0; r < RPB; ++r) s += lds[(i * V + e) * NT + r * G + tid];
-                    if (e < cnt[i]) dst[col[i] + e] = s;
-                }
+    for (int i = 0; i < E; ++i)
+        if (i % V < cnt[i / V]) dst[col[i / V] + i % V] = acc[i];
 }
 
 template <int DT, int V, int NV, int WPR>
@@ -317,7 +318,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
     typedef typename NrT<DT>::S S;
     constexpr int NT = WPR > 4 ? 64 * WPR : 256, NW = NT / 64, E = V * NV;
     __shared__ float red[4 * NW];
-    __shared__ float meet[WPR > 2 ? 1 : NT * E];
+    __shared__ float meet[WPR > 2 ? 1 : 256 * E];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = WPR > 1 ? 64 * WPR : 1 << a.g_log, lr = WPR > 1 ? tid % (64 * WPR) : tid & (G - 1), RPB = NT / G;
     const int slot = WPR > 1 ? wave / WPR : tid >> a.g_log;       // (a scalar where whole waves share a row)
@@ -440,12 +441,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
     if (!a.part) return;
     float *dst = a.part + (size_t)blockIdx.x * 5 * a.C;
     if (a.y) {
-        nr_put_sums<V, NV, NT>(meet, dst, s_gate, col, cnt, tid, G, RPB);
-        nr_put_sums<V, NV, NT>(meet, dst + a.C, s_wo, col, cnt, tid, G, RPB);
-        nr_put_sums<V, NV, NT>(meet, dst + 2 * (size_t)a.C, s_bo, col, cnt, tid, G, RPB);
+        nr_put_sums<V, NV, WPR, NW>(meet, dst, s_gate, col, cnt, wave, lr, a.g_log);
+        nr_put_sums<V, NV, WPR, NW>(meet, dst + a.C, s_wo, col, cnt, wave, lr, a.g_log);
+        nr_put_sums<V, NV, WPR, NW>(meet, dst + 2 * (size_t)a.C, s_bo, col, cnt, wave, lr, a.g_log);
     }
-    nr_put_sums<V, NV, NT>(meet, dst + 3 * (size_t)a.C, s_wi, col, cnt, tid, G, RPB);
-    nr_put_sums<V, NV, NT>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, tid, G, RPB);
+    nr_put_sums<V, NV, WPR, NW>(meet, dst + 3 * (size_t)a.C, s_wi, col, cnt, wave, lr, a.g_log);
+    nr_put_sums<V, NV, WPR, NW>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, wave, lr, a.g_log);
 }
 
 // column sums of the workgroups: 16 columns x 16 runs of workgroups per launch block, joined in a fixed order.  blockIdx.y: which of the five

@@ -292,6 +292,14 @@ def test_linear_row_strides(dt, pad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+def test_linear_large_odd_rows_of_wider_matrices(dt):
+    """Operands that are brought into order first: odd widths, rows of a wider matrix, with and without an activation."""
+    _linear_case(dt, 1100, 1003, 1001, "silu", train=True, pad=3, seed=8)
+    _linear_case(dt, 1100, 1001, 1001, "none", train=True, pad=8, seed=9)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 def test_linear_bias_in_float32(dt):
     _linear_case(dt, 40, 48, 56, "gelu", train=True, bias_dtype=torch.float32, seed=7)
@@ -323,7 +331,7 @@ def test_linear_whole_numbers_are_exact(dt, M, K, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DT)
-@pytest.mark.parametrize("M,K,N", [(4100, 72, 4104), (4104, 4104, 72), (72, 4104, 4104), (4099, 136, 4101), (8200, 1032, 2056)])
+@pytest.mark.parametrize("M,K,N", [(4100, 72, 4104), (4104, 4104, 72), (72, 4104, 4104), (4099, 136, 4101), (8200, 1032, 2056), (2100, 1001, 1003), (1500, 1002, 1004)])
 def test_linear_large_tiles_are_exact(dt, M, K, N):
     """Enough work for the large tile in each of the three products (and, with odd sizes, what takes its place): whole numbers, exact results."""
     import blockcopy
