@@ -44,15 +44,16 @@ def _plain(t):
     return t.as_subclass(torch.Tensor) if isinstance(t, torch.Tensor) else t
 
 
-def _features(x, dim, name):
+def _features(x, dim):
     """x with its features last."""
-    if dim == -1 or dim == x.dim() - 1:
-        if x.dim() < 1:
-            raise ValueError(f"{name}: a tensor with a feature axis is needed, got a scalar")
-        return x
-    if dim == 1 and x.dim() == 4:
-        return x.permute(0, 2, 3, 1)
-    raise ValueError(f"{name}: features are the last axis (dim=-1) or axis 1 of a (N, C, H, W) map (dim=1), got dim={dim} for shape {tuple(x.shape)}")
+    return x.permute(0, 2, 3, 1) if dim == 1 else x
+
+
+def _back(t, shape, dim):
+    """Rows (rows, features) as a tensor of ``shape`` (its axis order, features anywhere), or None."""
+    if t is None:
+        return None
+    return t.view(shape) if dim == -1 else t.view(shape[0], shape[2], shape[3], shape[1]).permute(0, 3, 1, 2)
 
 
 def _rows(x):
@@ -71,8 +72,8 @@ def _rows(x):
 
 
 def _matching(name, t, shape, like, what):
-    if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: {what} must have the shape {tuple(shape)} (features last; nothing is broadcast), got "
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
+        raise ValueError(f"{name}: {what} must have the shape {tuple(shape)} (nothing is broadcast), got "
                          f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
     if t.dtype != like.dtype or t.device != like.device:
         raise TypeError(f"{name}: {what} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
@@ -83,62 +84,68 @@ def _vector(name, p, n, like, what):
     if p is None:
         return None
     p = _plain(p)
-    if not isinstance(p, torch.Tensor) or tuple(p.shape) != (n,):
+    if not isinstance(p, torch.Tensor) or p.shape != (n,):
         raise ValueError(f"{name}: {what} must be a vector of {n} channels, got {tuple(p.shape) if isinstance(p, torch.Tensor) else p!r}")
-    if p.dtype not in (like.dtype, torch.float32) or p.device != like.device:
+    if (p.dtype != like.dtype and p.dtype != torch.float32) or p.device != like.device:
         raise TypeError(f"{name}: {what} must be {like.dtype} or float32 on {like.device}, got {p.dtype} on {p.device}")
-    return p.contiguous()
-
-
-def _wrapped(like, out, dim):
-    """Rows (features last) back into the argument's axis order and kind."""
-    if out is None:
-        return None
-    if dim == 1:
-        out = out.permute(0, 3, 1, 2)
-    if like is not None:
-        return TensorWrapper._wrap_like(out, like, like.is_blocks)
-    return out
+    return p if p.is_contiguous() else p.contiguous()
 
 
 def _argument(x, dim, name):
-    """(plain tensor with features last, TensorWrapper or None, effective dim)"""
+    """(plain tensor, its number of features, TensorWrapper or None, -1 or 1: where the features are)"""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name}: a tensor is needed, got {type(x).__name__}")
     wrapper = x if isinstance(x, TensorWrapper) and x.is_init else None
-    if wrapper is not None:
-        dim = 1
     x = _plain(x)
     if x.dtype not in _DTYPES:
         raise TypeError(f"{name}: float32, float16 or bfloat16 tensors, got {x.dtype}")
-    f = _features(x, dim, name)
-    if dim == x.dim() - 1:
+    n = x.dim()
+    if wrapper is not None:
+        dim = 1
+    elif n and (dim == -1 or dim == n - 1):
         dim = -1
-    if f.shape[-1] == 0:
+    if not (dim == -1 and n or dim == 1 and n == 4):
+        raise ValueError(f"{name}: features are the last axis (dim=-1) or axis 1 of a (N, C, H, W) map (dim=1), got dim={dim} for shape {tuple(x.shape)}")
+    if x.shape[dim] == 0:
         raise ValueError(f"{name}: no features in shape {tuple(x.shape)}")
-    return f, wrapper, dim
+    return x, x.shape[dim], wrapper, dim
+
+
+def _wrapped(out, wrapper):
+    return out if out is None or wrapper is None else TensorWrapper._wrap_like(out, wrapper, wrapper.is_blocks)
 
 
 # ------------------------------------------------------------------------------------------------ product
+def _linear_rows(be, x, weight, bias, residual, act, dim, keep_z):
+    """(y in the axis order of x, z, x's rows, the weight's rows)"""
+    xr, wr = _rows(_features(x, dim)), _rows(weight if weight.dim() == 2 else weight.flatten(1))
+    y, z = be.linear_fwd(xr, wr, bias, act, None if residual is None else _rows(_features(residual, dim)), keep_z)
+    shape = list(x.shape)
+    shape[dim] = wr.shape[0]
+    return _back(y, shape, dim), z, xr, wr
+
+
 class _LinearAct(torch.autograd.Function):
+    # (one node from argument to result: axis order, rows and their way back are inside)
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, be):
-        keep = act != 0 and any(ctx.needs_input_grad[:3])
-        y, z = be.linear_fwd(x, weight, bias, act, residual, keep)
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight if ctx.needs_input_grad[0] else None, z)
-        ctx.act, ctx.be, ctx.shape = act, be, (x.shape[0], weight.shape[0], weight.shape[1])
-        ctx.bias_dtype = None if bias is None else bias.dtype
+    def forward(ctx, x, weight, bias, residual, act, dim, be):
+        want = ctx.needs_input_grad
+        y, z, xr, wr = _linear_rows(be, x, weight, bias, residual, act, dim, act != 0 and (want[0] or want[1] or want[2]))
+        ctx.save_for_backward(xr if want[1] else None, wr if want[0] else None, z)
+        ctx.meta = act, dim, be, x.shape, weight.shape, None if bias is None else bias.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        x, weight, z = ctx.saved_tensors
+        xr, wr, z = ctx.saved_tensors
+        act, dim, be, x_shape, w_shape, bias_dtype = ctx.meta
         want = ctx.needs_input_grad
         dx = dw = db = None
-        if any(want[:3]):
-            dx, dw, db = ctx.be.linear_bwd(_rows(gy), z, x, weight, ctx.act, want[:3], ctx.bias_dtype)
-        return dx, dw, db, gy if want[3] else None, None, None
+        if want[0] or want[1] or want[2]:
+            dx, dw, db = be.linear_bwd(_rows(_features(gy, dim)), z, xr, wr, act, want[:3], bias_dtype)
+            dx, dw = _back(dx, x_shape, dim), None if dw is None else dw.view(w_shape)
+        return dx, dw, db, gy if want[3] else None, None, None, None
 
 
 def linear_act(x, weight, bias=None, activation: str = "none", residual=None, dim: int = -1):
@@ -148,83 +155,89 @@ def linear_act(x, weight, bias=None, activation: str = "none", residual=None, di
     ``none relu gelu gelu_tanh silu``; residual of the result's shape.  Any number of rows (none among them), any sizes, row strides as they
     come.  Under autograd the pre-activations are kept in x's dtype for the backward pass."""
     name = "linear_act"
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"{name}: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    xf, wrapper, dim = _argument(x, dim, name)
+    x, k, wrapper, dim = _argument(x, dim, name)
     weight = _plain(weight)
-    if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
-        weight = weight.flatten(1)
-    if weight.dim() != 2 or weight.shape[1] != xf.shape[-1] or weight.shape[0] == 0:
-        raise ValueError(f"{name}: weight must be (out, {xf.shape[-1]}), got {tuple(weight.shape)}")
-    if weight.dtype != xf.dtype or weight.device != xf.device:
-        raise TypeError(f"{name}: weight must be {xf.dtype} on {xf.device}, got {weight.dtype} on {weight.device}")
-    bias = _vector(name, bias, weight.shape[0], xf, "bias")
-    shape = (*xf.shape[:-1], weight.shape[0])
-    res = None
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError(f"{name}: weight must be a tensor, got {type(weight).__name__}")
+    n = weight.dim()
+    if not (n == 2 or n == 4 and weight.shape[2] == weight.shape[3] == 1) or weight.shape[1] != k or weight.shape[0] == 0:
+        raise ValueError(f"{name}: weight must be (out, {k}), got {tuple(weight.shape)}")
+    if weight.dtype != x.dtype or weight.device != x.device:
+        raise TypeError(f"{name}: weight must be {x.dtype} on {x.device}, got {weight.dtype} on {weight.device}")
+    bias = _vector(name, bias, weight.shape[0], x, "bias")
     if residual is not None:
-        res = _features(_plain(residual), dim, name)
-        _matching(name, res, shape, xf, "residual")
-        res = _rows(res)
-    be = _backend(xf)
-    xr, wr = _rows(xf), _rows(weight)
-    act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (xr, wr, bias, res)):
-        y = _LinearAct.apply(xr, wr, bias, res, act, be)
+        residual = _plain(residual)
+        shape = list(x.shape)
+        shape[dim] = weight.shape[0]
+        _matching(name, residual, torch.Size(shape), x, "residual")
+    be = _backend(x)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
+        y = _LinearAct.apply(x, weight, bias, residual, act, dim, be)
     else:
-        y = be.linear_fwd(xr, wr, bias, act, res)[0]
-    return _wrapped(wrapper, y.view(shape), dim)
+        y = _linear_rows(be, x, weight, bias, residual, act, dim, False)[0]
+    return _wrapped(y, wrapper)
 
 
 # ------------------------------------------------------------------------------------------------ norms around a block
+def _norm_rows(be, h, y, params, kinds, dim, keep_stats):
+    """(h', u, stats, h's rows, y's rows); h', u in the axis order of h"""
+    hr, yr = _rows(_features(h, dim)), None if y is None else _rows(_features(y, dim))
+    wo, bo, gate, wi, bi = params
+    if hr.shape[0] == 0:
+        return None if y is None else h.new_empty(h.shape), h.new_empty(h.shape) if kinds[1] else None, None, hr, yr
+    ho, u, stats = be.norm_residual_fwd(hr, yr, wo, bo, None if gate is None else gate.view(-1), wi, bi, *kinds, keep_stats)
+    return _back(ho, h.shape, dim), _back(u, h.shape, dim), stats, hr, yr
+
+
 class _NormResidual(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind, in_kind, scale, eps, rows_per_gate, be):
+    def forward(ctx, h, y, out_weight, out_bias, gate, in_weight, in_bias, kinds, dim, be):
         ctx.set_materialize_grads(False)
-        ho, u, stats = be.norm_residual_fwd(h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind, in_kind, scale, eps, rows_per_gate, True)
-        ctx.save_for_backward(h, y, out_weight, out_bias, gate, in_weight, in_bias, stats)
-        ctx.meta, ctx.be = (out_kind, in_kind, scale, rows_per_gate), be
+        ho, u, stats, hr, yr = _norm_rows(be, h, y, (out_weight, out_bias, gate, in_weight, in_bias), kinds, dim, True)
+        ctx.save_for_backward(hr, yr, out_weight, out_bias, gate, in_weight, in_bias, stats)
+        ctx.meta = kinds, dim, be, h.shape
         return (ho, u) if ho is not None and u is not None else (ho if ho is not None else u)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         h, y, out_weight, out_bias, gate, in_weight, in_bias, stats = ctx.saved_tensors
-        out_kind, in_kind, scale, rows_per_gate = ctx.meta
+        (out_kind, in_kind, scale, _, rows_per_gate), dim, be, shape = ctx.meta
         gh = grads[0] if y is not None else None
         gu = grads[-1] if in_kind else None
-        want = list(ctx.needs_input_grad[:7])
+        want = ctx.needs_input_grad[:7]
         if gh is None and gu is None:
-            return (None,) * 13
+            return (None,) * 10
+        flat = None if gate is None else gate.view(-1)
         if h.shape[0] == 0:
-            out = [torch.zeros_like(t) if w else None for t, w in zip((h, y, out_weight, out_bias, gate, in_weight, in_bias), want)]
+            out = [torch.zeros_like(t) if w else None for t, w in zip((h, y, out_weight, out_bias, flat, in_weight, in_bias), want)]
         else:
-            out = ctx.be.norm_residual_bwd(None if gh is None else _rows(gh), None if gu is None else _rows(gu), stats, h, y, out_weight, out_bias, gate, in_weight, in_bias,
-                                           out_kind, in_kind, scale, rows_per_gate, want)
-        return (*out, None, None, None, None, None, None)
+            out = be.norm_residual_bwd(None if gh is None else _rows(_features(gh, dim)), None if gu is None else _rows(_features(gu, dim)), stats, h, y, out_weight, out_bias,
+                                       flat, in_weight, in_bias, out_kind, in_kind, scale, rows_per_gate, want)
+        dh, dy, dwo, dbo, dg, dwi, dbi = out
+        return (_back(dh, shape, dim), _back(dy, shape, dim), dwo, dbo, None if dg is None else dg.view(gate.shape), dwi, dbi, None, None, None)
 
 
-def _gate(name, gate, hf, dim, packed):
-    """(gate as (C,) or (samples, C), rows per gate): shapes (C,), or h's own with ones (broadcast over rows) and, for a gate per sample, h's
-    first size; (C, 1, 1) as well for maps."""
-    C = hf.shape[-1]
+def _gate(name, gate, h, C, dim, packed):
+    """(gate, rows per gate): shapes (C,), (C, 1, 1) for maps, or h's own with ones (one gate for all rows) and, for a gate per sample, h's first size."""
     gate = _plain(gate)
     if not isinstance(gate, torch.Tensor):
         raise TypeError(f"{name}: gate must be a tensor, got {type(gate).__name__}")
-    if gate.dtype not in (hf.dtype, torch.float32) or gate.device != hf.device:
-        raise TypeError(f"{name}: gate must be {hf.dtype} or float32 on {hf.device}, got {gate.dtype} on {gate.device}")
-    shape = tuple(gate.shape)
-    if dim == 1 and shape == (C, 1, 1):
-        return gate.reshape(C).contiguous(), 0
-    if shape == (C,):
-        return gate.contiguous(), 0
-    g = gate.permute(0, 2, 3, 1) if dim == 1 and gate.dim() == 4 else gate
-    if g.dim() == hf.dim() and g.dim() >= 2 and g.shape[-1] == C and all(s == 1 for s in g.shape[1:-1]):
-        if g.shape[0] == 1:
-            return g.reshape(C).contiguous(), 0
-        if g.shape[0] == hf.shape[0] and not packed:
-            rows = hf.numel() // C
-            return g.reshape(-1, C).contiguous(), rows // hf.shape[0] if rows else 0
-    raise ValueError(f"{name}: gate must hold one value per channel ({C},) or per sample and channel, got {shape} for {tuple(hf.shape)} (features last)"
+    if (gate.dtype != h.dtype and gate.dtype != torch.float32) or gate.device != h.device:
+        raise TypeError(f"{name}: gate must be {h.dtype} or float32 on {h.device}, got {gate.dtype} on {gate.device}")
+    s = gate.shape
+    gate = gate if gate.is_contiguous() else gate.contiguous()
+    if s == (C,) or dim == 1 and s == (C, 1, 1):
+        return gate, 0
+    if len(s) == h.dim() >= 2 and s[dim] == C and gate.numel() == s[0] * C:
+        if s[0] == 1:
+            return gate, 0
+        if s[0] == h.shape[0] and not packed:
+            return gate, h.numel() // (C * s[0])
+    raise ValueError(f"{name}: gate must hold one value per channel ({C},) or per sample and channel, got {tuple(s)} for {tuple(h.shape)}"
                      + ("; packed tiles are no samples" if packed else ""))
 
 
@@ -236,41 +249,44 @@ def norm_residual(h, y=None, *, out_norm: str = "none", out_weight=None, out_bia
     value per channel, or per sample and channel.  Without ``y`` there is no block yet: h' is h itself.  Without ``in_norm`` u is None.
     Parameters in h's dtype or float32; up to 16384 channels.  u is formed from h' before its rounding."""
     name = "norm_residual"
-    for k, what in ((out_norm, "out_norm"), (in_norm, "in_norm")):
-        if k not in NORMS:
-            raise ValueError(f"{name}: {what} must be one of {', '.join(NORMS)}, got {k!r}")
-    if y is None and (out_norm != "none" or gate is not None or float(residual_scale) != 1.0):
+    out_kind, in_kind, scale, eps = NORMS.get(out_norm), NORMS.get(in_norm), float(residual_scale), float(eps)
+    if out_kind is None or in_kind is None:
+        raise ValueError(f"{name}: out_norm and in_norm must be one of {', '.join(NORMS)}, got {out_norm!r}, {in_norm!r}")
+    if y is None and (out_kind or gate is not None or scale != 1.0):
         raise ValueError(f"{name}: out_norm, gate and residual_scale need a block's output y")
-    if y is None and in_norm == "none":
+    if y is None and not in_kind:
         raise ValueError(f"{name}: nothing to do (neither y nor in_norm)")
-    for norm, vecs, what in ((out_norm, (out_weight, out_bias), "out"), (in_norm, (in_weight, in_bias), "in")):
-        if norm == "none" and any(v is not None for v in vecs):
-            raise ValueError(f"{name}: {what}_weight / {what}_bias without {what}_norm")
-    if not float(eps) >= 0.0:
+    if not out_kind and (out_weight is not None or out_bias is not None) or not in_kind and (in_weight is not None or in_bias is not None):
+        raise ValueError(f"{name}: a norm's weight or bias without the norm")
+    if not eps >= 0.0:
         raise ValueError(f"{name}: eps must not be negative, got {eps}")
-    hf, wrapper, dim = _argument(h, dim, name)
-    C = hf.shape[-1]
+    given = h
+    h, C, wrapper, dim = _argument(h, dim, name)
     if C > MAX_NORM_CHANNELS:
         raise ValueError(f"{name}: at most {MAX_NORM_CHANNELS} channels, got {C}")
-    packed = wrapper is not None and wrapper.is_blocks
-    yf = None
     if y is not None:
-        yf = _features(_plain(y), dim, name)
-        _matching(name, yf, hf.shape, hf, "y")
-    params = [_vector(name, p, C, hf, w) for p, w in ((out_weight, "out_weight"), (out_bias, "out_bias"), (in_weight, "in_weight"), (in_bias, "in_bias"))]
+        y = _plain(y)
+        _matching(name, y, h.shape, h, "y")
     rows_per_gate = 0
     if gate is not None:
-        gate, rows_per_gate = _gate(name, gate, hf, dim, packed)
-    params.insert(2, gate)
-    if len({p.dtype for p in params if p is not None}) > 1:
-        params = [None if p is None else p.float() for p in params]
-    be = _backend(hf)
-    hr, yr = _rows(hf), None if yf is None else _rows(yf)
-    kinds = (NORMS[out_norm], NORMS[in_norm], float(residual_scale), float(eps), rows_per_gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hr, yr, *params)):
-        out = _NormResidual.apply(hr, yr, *params, *kinds, be)
-        ho, u = out if isinstance(out, tuple) else ((out, None) if yr is not None else (None, out))
+        gate, rows_per_gate = _gate(name, gate, h, C, dim, wrapper is not None and wrapper.is_blocks)
+    params = (_vector(name, out_weight, C, h, "out_weight"), _vector(name, out_bias, C, h, "out_bias"), gate, _vector(name, in_weight, C, h, "in_weight"),
+              _vector(name, in_bias, C, h, "in_bias"))
+    kind, grad = None, h.requires_grad or (y is not None and y.requires_grad)
+    for p in params:
+        if p is not None:
+            grad = grad or p.requires_grad
+            if kind is None:
+                kind = p.dtype
+            elif p.dtype != kind:
+                kind = False
+    if kind is False:       # (the kernel takes one type of parameters)
+        params = tuple(None if p is None else p.float() for p in params)
+    be = _backend(h)
+    kinds = (out_kind, in_kind, scale, eps, rows_per_gate)
+    if grad and torch.is_grad_enabled():
+        out = _NormResidual.apply(h, y, *params, kinds, dim, be)
+        ho, u = out if isinstance(out, tuple) else ((out, None) if y is not None else (None, out))
     else:
-        ho, u, _ = be.norm_residual_fwd(hr, yr, *params, *kinds)
-    back = lambda t: None if t is None else _wrapped(wrapper, t.view(hf.shape), dim)
-    return (h if y is None else back(ho)), back(u)
+        ho, u = _norm_rows(be, h, y, params, kinds, dim, False)[:2]
+    return (given if y is None else _wrapped(ho, wrapper)), _wrapped(u, wrapper)

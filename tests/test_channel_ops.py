@@ -28,6 +28,7 @@ class PlainBackend:
     @staticmethod
     def _norm(h, y, wo, bo, gate, wi, bi, out_kind, in_kind, scale, eps, rpg):
         kinds = ("none", "rms", "layer")
+        gate = gate if gate is None or not rpg else gate.view(-1, h.shape[1])
         return CO.norm_residual(h, y, {"wo": wo, "bo": bo, "wi": wi, "bi": bi}, gate, scale, kinds[out_kind], kinds[in_kind], eps, rpg)
 
     def norm_residual_fwd(self, h, y, wo, bo, gate, wi, bi, out_kind, in_kind, scale, eps, rpg=0, keep_stats=False):
@@ -226,6 +227,10 @@ def test_no_rows(plain_backend):
     ho, u = blockcopy.norm_residual(h, h, in_norm="rms", in_weight=v)
     gh, gv = torch.autograd.grad(ho.sum() + u.sum(), [h, v])
     assert ho.shape == u.shape == gh.shape == (0, 4) and torch.equal(gv, torch.zeros(4))
+    h, g = torch.empty(2, 0, 4, requires_grad=True), torch.ones(2, 1, 4, requires_grad=True)
+    ho, u = blockcopy.norm_residual(h, h, gate=g)
+    gh, gg = torch.autograd.grad(ho.sum(), [h, g])
+    assert u is None and ho.shape == gh.shape == (2, 0, 4) and torch.equal(gg, torch.zeros(2, 1, 4))
 
 
 # ------------------------------------------------------------------------------------------------ GPU
