@@ -228,25 +228,31 @@ template <typename S, int W> __device__ __forceinline__ void lin_save(S *p, cons
             if (e < cnt) p[e] = (S)f[e];
 }
 
-// W consecutive outputs (m, n ..; 16 bytes' worth), cnt of them inside the matrix: sums v -> z, y.  The residual r is loaded by the caller, ahead
+// W consecutive outputs (m, n ..; 16 bytes' worth), cnt of them inside the matrix: sums v -> z, y.  The bias b and the residual r are loaded by the caller, ahead
 template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_residual(float *r, const LinEpi &ep, int N, int m, int n)
 {
     typedef typename LinT<DT>::S S;
     lin_load<S, W>(r, (const S *)ep.res + (size_t)m * ep.ldr + n, N - n);
 }
 
-template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v, const float *r)
+// the bias of W columns (a lane keeps its columns: loaded once)
+template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_bias(float *b, const LinEpi &ep, int N, int n)
+{
+    typedef typename LinT<DT>::S S;
+#pragma unroll
+    for (int e = 0; e < W; ++e) b[e] = 0.f;
+    if (!ep.bias || n >= N) return;
+    if (ep.bias_f32) lin_load<float, W>(b, (const float *)ep.bias + n, N - n);
+    else lin_load<S, W>(b, (const S *)ep.bias + n, N - n);
+}
+
+template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v, const float *b, const float *r)
 {
     typedef typename LinT<DT>::S S;
     const int cnt = N - n;
     const size_t at = (size_t)m * N + n;
-    if (ep.bias) {
-        float t[W];
-        if (ep.bias_f32) lin_load<float, W>(t, (const float *)ep.bias + n, cnt);
-        else lin_load<S, W>(t, (const S *)ep.bias + n, cnt);
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += t[e];
-    }
+    for (int e = 0; e < W; ++e) v[e] += b[e];
     if (ep.z) lin_save<S, W>((S *)ep.z + at, v, cnt);
     if (ep.act != ACT_NONE)
 #pragma unroll
@@ -422,6 +428,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
     constexpr int AHEAD = RH / RPI < 4 ? RH / RPI : 4;          // rounds whose residuals are requested together
     uint4 *own = lin_lds + wave * (RH * CPR);
     const int n = n0 + wn * CW + (lane % PER_ROW) * V;
+    float bias[V];
+    lin_bias<DT>(bias, g.ep, g.N, n);
     lin_meet();         // all waves have read the last step
 #pragma unroll
     for (int h = 0; h < BM / WM / RH; ++h) {        // (the part is the wave's own and its LDS accesses stay in order: no barrier)
@@ -449,7 +457,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
                     for (int e = 0; e < 4; ++e) v[4 * p + e] = f[e];
                 }
                 if (g.part) lin_save<float, V>(g.part + ((size_t)slice * g.M + m) * g.N + n, v, g.N - n);
-                else lin_epilogue<DT>(g.ep, g.N, m, n, v, res[q]);
+                else lin_epilogue<DT>(g.ep, g.N, m, n, v, bias, res[q]);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -485,11 +493,12 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_join(const float 
     }
     __syncthreads();
     if (wave || !live) return;
-    float r[W];
+    float b[W], r[W];
+    lin_bias<DT>(b, ep, N, n);
     if (ep.res) lin_residual<DT>(r, ep, N, (int)m, n);
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] = ((v[e] + red[0][e][lane]) + red[1][e][lane]) + red[2][e][lane];
-    lin_epilogue<DT>(ep, N, (int)m, n, v, r);
+    lin_epilogue<DT>(ep, N, (int)m, n, v, b, r);
 }
 
 // Few rows (a token, a handful of regions): bound by reading the weight once.  A workgroup takes 16 columns and all rows, its waves a share of the
@@ -539,9 +548,10 @@ template <int DT, int MB, int NW> __global__ __launch_bounds__(64 * NW) void k_l
     for (int q = 1; q < NW; ++q) s += red[q][wave][lane];
     const int m = 16 * wave + r, n = n0 + 4 * (lane >> 4);
     if (m >= g.M || n >= g.N) return;
-    float v[4] = {s[0], s[1], s[2], s[3]}, res[4];
+    float v[4] = {s[0], s[1], s[2], s[3]}, bias[4], res[4];
+    lin_bias<DT, 4>(bias, g.ep, g.N, n);
     if (g.ep.res) lin_residual<DT, 4>(res, g.ep, g.N, m, n);
-    lin_epilogue<DT, 4>(g.ep, g.N, m, n, v, res);
+    lin_epilogue<DT, 4>(g.ep, g.N, m, n, v, bias, res);
 }
 
 // dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.
@@ -566,7 +576,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
 #pragma unroll
     for (int e = 0; e < W; ++e) sum[e] = 0.f;
     if (n < a.N)
-#pragma unroll 2
+#pragma unroll 4
         for (int m = (int)blockIdx.y * a.span + r; m < m1; m += rows) {
             float d[W], z[W];
             lin_load<S, W>(d, (const S *)a.gy + (size_t)m * a.ldg + n, cnt);
@@ -645,16 +655,21 @@ LinPlan lin_plan(int dtype, long long M, long long N, long long K)
 {
     LinPlan p;
     const int bk = lin_bk(dtype);
+    const long long steps = (K + bk - 1) / bk, t128 = lin_tiles(M, N, 128);
+    long long s = t128 >= LIN_CUS ? 1 : 2 * LIN_CUS / t128;
+    s = s < steps / 8 ? s : steps / 8;
     // fp32: 64 (the matrix instructions take so long that a small tile's operands arrive in time: 17408 x 768 x 256 72 us against 105 with 128,
     // 1024^3 24 against 34).  16 bits: 256 once that fills the chip and the sum is long enough to pay for an epilogue that nothing overlaps
     // (16384 x 4096 x 8192: 903 us, 128: 1040, 64: 1565; 8192 x 2048 x 8192: 240, 279, 384 -- but 17408 x 512 x 2048: 77, 60, 65), else 128 while
-    // every CU gets two, else 64 (2048^3 with gelu 31 us against 35)
-    p.edge = dtype == DT_F32 ? 64 : K >= 1024 && lin_tiles(M, N, 256) >= LIN_CUS ? 256 : lin_tiles(M, N, 128) >= 2 * LIN_CUS ? 128 : 64;
+    // that, with a long sum in slices of at least 8 steps, gives every CU one (2048 x 512 x 17408: 50 us, 64: 122), else 64 (1024^3 16 us against 22)
+    p.edge = dtype == DT_F32 ? 64 : K >= 1024 && lin_tiles(M, N, 256) >= LIN_CUS ? 256 : t128 * (s > 1 ? s : 1) >= LIN_CUS ? 128 : 64;
     p.tm = (unsigned)((M + p.edge - 1) / p.edge);
     p.tn = (unsigned)((N + p.edge - 1) / p.edge);
-    const long long tiles = (long long)p.tm * p.tn, steps = (K + bk - 1) / bk;
-    long long s = tiles >= LIN_CUS ? 1 : 2 * LIN_CUS / tiles;
-    s = s < steps / 4 ? s : steps / 4;
+    const long long tiles = (long long)p.tm * p.tn;
+    if (p.edge != 128) {        // (64: a slice of at least 4 steps)
+        s = tiles >= LIN_CUS ? 1 : 2 * LIN_CUS / tiles;
+        s = s < steps / 4 ? s : steps / 4;
+    }
     if (s < 1) s = 1;
     const long long per = (steps + s - 1) / s;
     p.kspan = (int)(per * bk);
@@ -737,9 +752,8 @@ int lin_sizes(long long M, int N, int K, int dtype)
     if (dtype < 0 || dtype > 2) return BC_ERR_ELEM;
     if (M < 0 || N < 1 || K < 1) return BC_ERR_SHAPE;
     if (M > 0x7fffff00ll || N > 0x7fffff00 || K > 0x7fffff00) return BC_ERR_RANGE;
-    if (((M + 63) / 64) * (((long long)N + 63) / 64) > 0x7fffff00ll || ((M + 63) / 64) * (((long long)K + 63) / 64) > 0x7fffff00ll ||
-        (((long long)N + 63) / 64) * (((long long)K + 63) / 64) > 0x7fffff00ll)
-        return BC_ERR_RANGE;
+    const long long m = (M + 63) / 64, n = ((long long)N + 63) / 64, k = ((long long)K + 63) / 64, most = 0xffffff;      // (tiles x 256 threads of a launch)
+    if (m > most / n || m > most / k || n > most / k) return BC_ERR_RANGE;
     return BC_OK;
 }
 

@@ -42,6 +42,7 @@ struct NormArgs {
     const void *gh, *gu;                        // gradients of h' and u (NULL: zeros)
     void *dh, *dy;
     float *part;                                // [workgroups][5][C]: column sums of gate, wo, bo, wi, bi
+    float *means;                               // [M][2]: mean(p n), mean(p) of the inner norm's backward (rows of more than 8192 channels)
     long long ldh, ldy, ldgh, ldgu;
     int M, C, g_log, rows_per_gate, span, chunks;
     int out_kind, in_kind, pf32, need_dh, need_dy;
@@ -312,6 +313,7 @@ template <int V, int NV, int WPR, int NW> __device__ __forceinline__ void nr_put
         if (i % V < cnt[i / V]) dst[col[i / V] + i % V] = acc[i];
 }
 
+// (rows of more than 8192 channels, 16 per lane: the five sums of each would not fit the 128 registers of a lane; they go to k_norm_cols)
 template <int DT, int V, int NV, int WPR>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ? 1 : 3) void k_norm_bwd(const NormArgs a)
 {
@@ -338,6 +340,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
     const int first = chunk * a.span, last = per_group - first < a.span ? per_group : first + a.span;
     const size_t gate_at = a.rows_per_gate ? (size_t)group * a.C : 0;
 
+    constexpr bool SUMS = E == 8;
     float s_gate[E], s_wo[E], s_bo[E], s_wi[E], s_bi[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) s_gate[i] = s_wo[i] = s_bo[i] = s_wi[i] = s_bi[i] = 0.f;
@@ -393,8 +396,10 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
             for (int i = 0; i < E; ++i) {
                 if (a.y) hn[i] = a.alpha * hn[i] + gate[i] * (n[i] * wo[i] + bo[i]);
                 hn[i] = i % V < cnt[i / V] ? (hn[i] - st.z) * st.w : 0.f;
-                s_wi[i] += p[i] * hn[i];
-                s_bi[i] += p[i];
+                if constexpr (SUMS) {
+                    s_wi[i] += p[i] * hn[i];
+                    s_bi[i] += p[i];
+                }
                 p[i] *= wi[i];
                 m1 += p[i] * hn[i];
                 m2 += p[i];
@@ -402,6 +407,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
             sum(m1, m2, a.in_kind == NORM_LAYER);
             m1 *= inv_c;
             m2 = a.in_kind == NORM_LAYER ? m2 * inv_c : 0.f;
+            if (!SUMS && a.means && live && lr == 0) *(float2 *)(a.means + 2 * (base + r0 + slot)) = float2{m1, m2};
 #pragma unroll
             for (int i = 0; i < E; ++i) g[i] += st.w * (p[i] - m2 - hn[i] * m1);
         }
@@ -419,10 +425,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             if (!(live && i % V < cnt[i / V])) g[i] = 0.f;
-            s_gate[i] += g[i] * (n[i] * wo[i] + bo[i]);
             const float q = g[i] * gate[i];
-            s_wo[i] += q * n[i];
-            s_bo[i] += q;
+            if constexpr (SUMS) {
+                s_gate[i] += g[i] * (n[i] * wo[i] + bo[i]);
+                s_wo[i] += q * n[i];
+                s_bo[i] += q;
+            }
             p[i] = q * wo[i];
             m1 += p[i] * n[i];
             m2 += p[i];
@@ -438,7 +446,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
 #pragma unroll
             for (int i = 0; i < NV; ++i) nr_store<S, V>(a.dy, out, col[i], cnt[i], p + i * V);
     }
-    if (!a.part) return;
+    if (!SUMS || !a.part) return;
     float *dst = a.part + (size_t)blockIdx.x * 5 * a.C;
     if (a.y) {
         nr_put_sums<V, NV, WPR, NW>(meet, dst, s_gate, col, cnt, wave, lr, a.g_log);
@@ -447,6 +455,66 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
     }
     nr_put_sums<V, NV, WPR, NW>(meet, dst + 3 * (size_t)a.C, s_wi, col, cnt, wave, lr, a.g_log);
     nr_put_sums<V, NV, WPR, NW>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, wave, lr, a.g_log);
+}
+
+// the column sums of wide rows in a second pass: with the rows' statistics and means known everything is element by element.  A lane takes V
+// channels, a workgroup a strip of 64 V of them and a run of rows, its four waves every fourth
+template <int DT> __global__ __launch_bounds__(256) void k_norm_cols(const NormArgs a)
+{
+    typedef typename NrT<DT>::S S;
+    constexpr int V = NrT<DT>::V;
+    __shared__ float meet[3][5 * V][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const unsigned col[1] = {(blockIdx.x * 64 + lane) * V};
+    const int cnt[1] = {a.C - (int)col[0]};
+    const int group = (int)blockIdx.y / a.chunks, chunk = (int)blockIdx.y % a.chunks, per_group = a.rows_per_gate ? a.rows_per_gate : a.M;
+    const long long base = (long long)group * per_group;
+    const int first = chunk * a.span, last = per_group - first < a.span ? per_group : first + a.span;
+    float wo[V], bo[V], gate[V], wi[V], s[5 * V];
+    nr_params<S, V, 1>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+    nr_params<S, V, 1>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+    nr_params<S, V, 1>(gate, a.gate, a.pf32, a.rows_per_gate ? (size_t)group * a.C : 0, col, cnt, 1.f);
+    nr_params<S, V, 1>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+#pragma unroll
+    for (int i = 0; i < 5 * V; ++i) s[i] = 0.f;
+    if (cnt[0] > 0)
+#pragma unroll 2
+        for (int r = first + wave; r < last; r += 4) {
+            const long long row = base + r;
+            const float4 st = *(const float4 *)(a.stats + 4 * row);
+            const float2 mean = a.in_kind != NORM_NONE ? *(const float2 *)(a.means + 2 * row) : float2{0.f, 0.f};
+            NrRow<S, V, 1> ry, rh, rgu, rgh;
+            ry.ask(a.y, (size_t)row * a.ldy, col, cnt, true);
+            rh.ask(a.in_kind != NORM_NONE ? a.h : nullptr, (size_t)row * a.ldh, col, cnt, true);
+            rgu.ask(a.gu, (size_t)row * a.ldgu, col, cnt, true);
+            rgh.ask(a.gh, (size_t)row * a.ldgh, col, cnt, true);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float n = a.out_kind != NORM_NONE ? (ry.at(e) - st.x) * st.y : ry.at(e);
+                float g = rgh.at(e);
+                if (a.in_kind != NORM_NONE) {
+                    const float h = a.y ? a.alpha * rh.at(e) + gate[e] * (n * wo[e] + bo[e]) : rh.at(e);
+                    const float hn = (h - st.z) * st.w, u = rgu.at(e);
+                    s[3 * V + e] += u * hn;
+                    s[4 * V + e] += u;
+                    g += st.w * (u * wi[e] - mean.y - hn * mean.x);
+                }
+                s[e] += g * (n * wo[e] + bo[e]);
+                s[V + e] += g * gate[e] * n;
+                s[2 * V + e] += g * gate[e];
+            }
+        }
+    if (wave)
+#pragma unroll
+        for (int i = 0; i < 5 * V; ++i) meet[wave - 1][i][lane] = s[i];
+    __syncthreads();
+    if (wave) return;
+    float *dst = a.part + (size_t)blockIdx.y * 5 * a.C + col[0];
+#pragma unroll
+    for (int i = 0; i < 5 * V; ++i) {
+        const float t = ((s[i] + meet[0][i][lane]) + meet[1][i][lane]) + meet[2][i][lane];
+        if (i % V < cnt[0]) dst[(size_t)(i / V) * a.C + i % V] = t;
+    }
 }
 
 // column sums of the workgroups: 16 columns x 16 runs of workgroups per launch block, joined in a fixed order.  blockIdx.y: which of the five
@@ -540,20 +608,18 @@ int nr_check(long long M, int C, int dtype, int out_kind, int in_kind, long long
     if (M < 0 || C < 1 || C > NR_MAX_C || out_kind < 0 || out_kind > 2 || in_kind < 0 || in_kind > 2) return BC_ERR_SHAPE;
     if (M > 0x7fffffffll) return BC_ERR_RANGE;
     if (rows_per_gate < 0 || (rows_per_gate && (!gate || M % rows_per_gate))) return BC_ERR_SHAPE;
+    if (rows_per_gate && M / rows_per_gate > 65535) return BC_ERR_RANGE;       // (a launch dimension)
     if (!y && (out_kind != NORM_NONE || gate || in_kind == NORM_NONE)) return BC_ERR_SHAPE;
     return BC_OK;
 }
 
-// as many workgroups as run at once (three of four waves per CU for 16-bit rows, two for fp32), the rows of a gate group divided evenly among
-// whole workgroups
+// the rows of a gate group divided evenly among whole workgroups (chunks)
 struct NormChunks { int chunks, span, groups; };
-NormChunks nr_chunks(long long M, long long rows_per_gate, int dtype, const NormShape &s)
+NormChunks nr_split(long long M, long long rows_per_gate, int want, int rows_per_block)
 {
-    const int rows_per_block = nr_rows_per_block(s);
     NormChunks c;
     const long long per = rows_per_gate ? rows_per_gate : M;
     c.groups = (int)(M / per);
-    const int want = dtype == DT_F32 || s.WPR > 4 ? 512 : 768;
     long long n = (want + c.groups - 1) / c.groups;
     const long long most = (per + rows_per_block - 1) / rows_per_block;
     if (n > most) n = most;
@@ -562,6 +628,27 @@ NormChunks nr_chunks(long long M, long long rows_per_gate, int dtype, const Norm
     c.span = (int)span;
     c.chunks = (int)((per + span - 1) / span);
     return c;
+}
+
+// as many workgroups as run at once: three of four waves per CU for 16-bit rows, two for fp32
+NormChunks nr_rows_split(long long M, long long rows_per_gate, int dtype, const NormShape &s)
+{
+    return nr_split(M, rows_per_gate, dtype == DT_F32 || s.WPR > 4 ? 512 : 768, nr_rows_per_block(s));
+}
+
+inline unsigned nr_strips(int C, int dtype) { const int v = 64 * 16 / (dtype == DT_F32 ? 4 : 2); return (unsigned)((C + v - 1) / v); }
+
+// the workgroups that leave column sums: those of the rows, or (wide rows) about 1024 of k_norm_cols
+NormChunks nr_sums_split(long long M, long long rows_per_gate, int C, int dtype, const NormShape &s)
+{
+    return s.E == 8 ? nr_rows_split(M, rows_per_gate, dtype, s) : nr_split(M, rows_per_gate, (int)(1024 / nr_strips(C, dtype)), 4);
+}
+
+long long nr_bwd_space(long long M, int C, long long rows_per_gate, int dtype)
+{
+    const NormShape s = nr_shape(C);
+    const NormChunks c = nr_sums_split(M, rows_per_gate, C, dtype, s);
+    return 20ll * C * c.chunks * c.groups + (s.E == 8 ? 0 : 8 * M);
 }
 
 }  // namespace
@@ -596,8 +683,7 @@ BC_EXPORT int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const voi
 BC_EXPORT long long bc_norm_residual_bwd_workspace(long long M, int C, long long rows_per_gate, int dtype)
 {
     if (M < 1 || C < 1 || C > NR_MAX_C || dtype < 0 || dtype > 2 || rows_per_gate < 0 || (rows_per_gate && M % rows_per_gate)) return 0;
-    const NormChunks c = nr_chunks(M, rows_per_gate, dtype, nr_shape(C));
-    return 20ll * C * c.chunks * c.groups;
+    return nr_bwd_space(M, C, rows_per_gate, dtype);
 }
 
 BC_EXPORT int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void *d_out_bias, void *d_gate, void *d_in_weight, void *d_in_bias, const void *gh, const void *gu,
@@ -617,25 +703,36 @@ BC_EXPORT int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void 
         if (ps[i] && (uintptr_t)ps[i] % pe) return BC_ERR_ALIGN;
     if ((uintptr_t)stats % 16) return BC_ERR_ALIGN;
     const NormShape s = nr_shape(C);
-    const NormChunks c = nr_chunks(M, rows_per_gate, dtype, s);
+    const NormChunks c = nr_rows_split(M, rows_per_gate, dtype, s), q = nr_sums_split(M, rows_per_gate, C, dtype, s);
     const bool sums = d_out_weight || d_out_bias || d_gate || d_in_weight || d_in_bias;
     if (sums && !workspace) return BC_ERR_NULL;
-    if (sums && workspace_bytes < 20ll * C * c.chunks * c.groups) return BC_ERR_SHAPE;
-    if (sums && (uintptr_t)workspace % 4) return BC_ERR_ALIGN;
+    if (sums && workspace_bytes < nr_bwd_space(M, C, rows_per_gate, dtype)) return BC_ERR_SHAPE;
+    if (sums && (uintptr_t)workspace % 256) return BC_ERR_ALIGN;
     NormArgs a = {};
     a.h = h; a.y = y; a.wo = out_weight; a.bo = out_bias; a.gate = gate; a.wi = in_weight;
     a.stats = (float *)stats; a.gh = gh; a.gu = gu; a.dh = dh; a.dy = dy; a.part = sums ? (float *)workspace : nullptr;
+    a.means = sums && s.E != 8 ? (float *)((char *)workspace + 20ll * C * q.chunks * q.groups) : nullptr;
     a.ldh = ldh; a.ldy = ldy; a.ldgh = ldgh; a.ldgu = ldgu; a.M = (int)M; a.C = C; a.rows_per_gate = (int)rows_per_gate;
     a.out_kind = out_kind; a.in_kind = in_kind; a.pf32 = params_f32; a.alpha = residual_scale;
     a.need_dh = dh != nullptr; a.need_dy = dy != nullptr;
     a.g_log = s.g_log; a.span = c.span; a.chunks = c.chunks;
     const int r = nr_dispatch(dtype, true, a, s, (unsigned)(c.chunks * c.groups), (hipStream_t)stream);
     if (r != BC_OK || !sums) return r;
+    if (s.E != 8) {
+        a.span = q.span;
+        a.chunks = q.chunks;
+        const dim3 grid(nr_strips(C, dtype), (unsigned)(q.chunks * q.groups));
+        switch (dtype) {
+        case DT_F32: k_norm_cols<DT_F32><<<grid, 256, 0, (hipStream_t)stream>>>(a); break;
+        case DT_F16: k_norm_cols<DT_F16><<<grid, 256, 0, (hipStream_t)stream>>>(a); break;
+        default: k_norm_cols<DT_BF16><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        }
+    }
     NormJoin j = {};
     j.part = (const float *)workspace;
     j.out[0] = d_gate; j.out[1] = d_out_weight; j.out[2] = d_out_bias; j.out[3] = d_in_weight; j.out[4] = d_in_bias;
-    j.C = C; j.blocks = c.chunks * c.groups; j.chunks = c.chunks; j.groups = c.groups; j.f32 = params_f32;
-    const dim3 grid((unsigned)((C + 15) / 16), 5, (unsigned)c.groups);
+    j.C = C; j.blocks = q.chunks * q.groups; j.chunks = q.chunks; j.groups = q.groups; j.f32 = params_f32;
+    const dim3 grid((unsigned)((C + 15) / 16), 5, (unsigned)q.groups);
     switch (dtype) {
     case DT_F32: k_norm_join<DT_F32><<<grid, 256, 0, (hipStream_t)stream>>>(j); break;
     case DT_F16: k_norm_join<DT_F16><<<grid, 256, 0, (hipStream_t)stream>>>(j); break;

@@ -630,7 +630,7 @@ long long bc_linear_bwd_workspace(long long M, int N, int K, int act, int dtype)
 /* h_out = residual_scale * h + gate * t,  t = N_out(y) * out_weight + out_bias;  u = N_in(h_out) * in_weight + in_bias, over the C <= 16384 features of a
  * row.  N (kinds): 0 none, 1 x / sqrt(mean(x^2) + eps), 2 (x - mean) / sqrt(mean((x - mean)^2) + eps).  y NULL: no block yet (out_kind 0, no gate; h_out is h,
  * not stored).  in_kind 0: no u.  Parameters NULL = ones / zeros, all fp32 (params_f32) or all dtype; gate (C), or (M / rows_per_gate, C) with
- * rows_per_gate > 0: row m takes gate row m / rows_per_gate.  u is formed from h_out before its rounding.  stats (M, 4) fp32, 16-byte aligned:
+ * rows_per_gate > 0: row m takes gate row m / rows_per_gate (at most 65535 of them).  u is formed from h_out before its rounding.  stats (M, 4) fp32, 16-byte aligned:
  * {mean, 1 / deviation} of y and of h_out for the backward pass (NULL: not kept). */
 int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const void *h, const void *y, const void *out_weight, const void *out_bias, const void *gate,
                          const void *in_weight, const void *in_bias, long long M, int C, long long ldh, long long ldy, long long rows_per_gate, float residual_scale,

@@ -97,7 +97,7 @@ def test_refusals_of_norm_residual(plain_backend):
            (ValueError, lambda: f(h, y, out_norm="rms", out_weight=torch.ones(1))), (ValueError, lambda: f(h, y, in_norm="rms", eps=-1.0)),
            (ValueError, lambda: f(h, y, in_norm="rms", eps=float("nan"))), (ValueError, lambda: f(torch.randn(1, 16385), in_norm="rms")),
            (TypeError, lambda: f(h.double(), in_norm="rms")), (ValueError, lambda: f(torch.randn(2, 3, 8), torch.randn(2, 3, 8), gate=torch.ones(2, 3, 8))),
-           (ValueError, lambda: f(h, y, dim=0))]
+           (ValueError, lambda: f(h, y, dim=0)), (ValueError, lambda: f(torch.randn(65536, 1), torch.randn(65536, 1), gate=torch.ones(65536, 1)))]
     for kind, call in bad:
         with pytest.raises(kind):
             call()
@@ -132,6 +132,7 @@ def test_c_entries_validate_before_any_device_call():
     fwd = lambda *, ho=256, u=256, h=256, y=256, gate=N, M=6, C=8, ldh=8, ldy=8, rpg=0, ok=1, ik=1, dt=0, stats=N: lib.bc_norm_residual_fwd(
         ho, u, stats, h, y, N, N, gate, N, N, M, C, ldh, ldy, rpg, 1.0, 1e-6, ok, ik, dt, 0, N)
     assert fwd(M=0) == 0 and fwd(C=16385) == -2 and fwd(C=0) == -2 and fwd(ok=3) == -2 and fwd(ik=-1) == -2 and fwd(dt=4) == -3 and fwd(ldh=7) == -2
+    assert fwd(M=65536, gate=256, rpg=1) == -4 and lin(M=1 << 30, n=1 << 30) == -4
     assert fwd(rpg=2) == -2 and fwd(gate=256, rpg=4) == -2 and fwd(y=N) == -2 and fwd(y=N, ok=0, ik=0) == -2 and fwd(h=N) == -1 and fwd(u=N) == -1
     assert fwd(stats=264) == -5 and fwd(h=257) == -5 and fwd(M=1 << 31) == -4
     nb = lambda *, dh=256, dy=256, dwo=256, stats=256, h=256, y=256, M=6, C=8, ldh=8, ws=256, wsb=1 << 30: lib.bc_norm_residual_bwd(
@@ -507,6 +508,8 @@ def test_norm_without_a_block_and_many_rows(dt):
     _norm_case(dt, 1, 300, "none", "rms", block=False, gate="none", seed=6)
     _norm_case(dt, 9001, 16, "rms", "layer", seed=7)
     _norm_case(dt, 4200, 48, "layer", "rms", gate="sample", groups=2100, seed=8)
+    _norm_case(dt, 130, 8200, "layer", "none", seed=13)
+    _norm_case(dt, 130, 9001, "none", "layer", block=False, gate="none", seed=14)
 
 
 @pytest.mark.gpu
@@ -514,6 +517,7 @@ def test_norm_without_a_block_and_many_rows(dt):
 def test_norm_float32_parameters(dt):
     _norm_case(dt, 40, 200, "layer", "rms", pf32=True, seed=9)
     _norm_case(dt, 30, 77, "rms", "layer", pf32=True, gate="sample", groups=3, seed=10)
+    _norm_case(dt, 12, 9000, "rms", "layer", pf32=True, gate="sample", groups=3, seed=12)
 
 
 @pytest.mark.gpu
