@@ -150,18 +150,30 @@ template <typename S, int V> __device__ __forceinline__ void nr_param(float *f, 
 }
 
 // one row of a tensor as a lane holds it before its turn: NV vectors as they come from memory (requested a row ahead, so that the latency of
-// memory lies behind the row in hand)
-template <typename S, int V, int NV> struct NrRow {
+// memory lies behind the row in hand).  LAST: the last vector of a row is read as the row's last V elements and moved down at its turn by
+// those that belong to the vector before -- one load like all others; element by element its 16-bit pieces are put together as they arrive,
+// in front of everything behind them
+template <typename S, int V, int NV, bool LAST> struct NrRow {
     typename NrVec<S, V>::T v[NV];
+    static __device__ __forceinline__ bool last(unsigned col, int cnt) { return LAST && cnt > 0 && cnt < V && (int)col + cnt >= V; }
     __device__ __forceinline__ void ask(const void *q, size_t base, const unsigned *col, const int *cnt, bool live)
     {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (q && live) v[i] = nr_raw<S, V>(q, base, col[i], cnt[i]);
-            else
+            if (!q || !live)
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[i][e] = (S)0.f;
+            else {
+                const bool l = last(col[i], cnt[i]);
+                v[i] = nr_raw<S, V>(q, base, l ? col[i] + cnt[i] - V : col[i], l ? V : cnt[i]);
+            }
         }
+    }
+    __device__ __forceinline__ void settle(const unsigned *col, const int *cnt)
+    {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (last(col[i], cnt[i])) v[i] = __builtin_bit_cast(typename NrVec<S, V>::T, __builtin_bit_cast(unsigned __int128, v[i]) >> ((V - cnt[i]) * (128 / V)));
     }
     __device__ __forceinline__ float at(int k) const { return (float)v[k / V][k % V]; }
 };
@@ -196,7 +208,7 @@ template <int V, int NV, class Sum> __device__ __forceinline__ void nr_normalise
     for (int i = 0; i < NV * V; ++i) x[i] *= rstd;
 }
 
-template <int DT, int V, int NV, int WPR>
+template <int DT, int V, int NV, int WPR, bool ODD>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const NormArgs a)
 {
     typedef typename NrT<DT>::S S;
@@ -225,7 +237,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
         if (!a.rows_per_gate) nr_params<S, V, NV>(gate, a.gate, a.pf32, 0, col, cnt, 1.f);
     }
     const long long hop = (long long)gridDim.x * RPB;
-    NrRow<S, V, NV> ry, rh;
+    NrRow<S, V, NV, ODD> ry, rh;
     long long row = (long long)blockIdx.x * RPB + slot;
     if constexpr (KEEP) {
         ry.ask(a.y, (size_t)row * a.ldy, col, cnt, row < a.M);
@@ -238,6 +250,8 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
             ry.ask(a.y, (size_t)row * a.ldy, col, cnt, live);
             rh.ask(a.h, (size_t)row * a.ldh, col, cnt, live);
         }
+        ry.settle(col, cnt);
+        rh.settle(col, cnt);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             x[i] = ry.at(i);
@@ -314,8 +328,8 @@ template <int V, int NV, int WPR, int NW> __device__ __forceinline__ void nr_put
 }
 
 // (rows of more than 8192 channels, 16 per lane: the five sums of each would not fit the 128 registers of a lane; they go to k_norm_cols)
-template <int DT, int V, int NV, int WPR>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ? 1 : 3) void k_norm_bwd(const NormArgs a)
+template <int DT, int V, int NV, int WPR, bool ODD>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 || ODD ? 1 : 3) void k_norm_bwd(const NormArgs a)
 {
     typedef typename NrT<DT>::S S;
     constexpr int NT = WPR > 4 ? 64 * WPR : 256, NW = NT / 64, E = V * NV;
@@ -356,7 +370,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
         nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
     }
 
-    NrRow<S, V, NV> rgh, ry, rh, rgu;
+    NrRow<S, V, NV, ODD> rgh, ry, rh, rgu;
     float4 rst;
     auto ask = [&](int r) {
         const bool live = r < last;
@@ -374,6 +388,10 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 ?
         if constexpr (!KEEP) ask(r0 + slot);
         float n[E], g[E], p[E], hn[E];      // normalised y; gradient of h'; working row; normalised h'
         const float4 st = rst;
+        ry.settle(col, cnt);
+        rh.settle(col, cnt);
+        rgu.settle(col, cnt);
+        rgh.settle(col, cnt);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             n[i] = ry.at(i);
@@ -483,11 +501,15 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_cols(const NormA
             const long long row = base + r;
             const float4 st = *(const float4 *)(a.stats + 4 * row);
             const float2 mean = a.in_kind != NORM_NONE ? *(const float2 *)(a.means + 2 * row) : float2{0.f, 0.f};
-            NrRow<S, V, 1> ry, rh, rgu, rgh;
+            NrRow<S, V, 1, true> ry, rh, rgu, rgh;
             ry.ask(a.y, (size_t)row * a.ldy, col, cnt, true);
             rh.ask(a.in_kind != NORM_NONE ? a.h : nullptr, (size_t)row * a.ldh, col, cnt, true);
             rgu.ask(a.gu, (size_t)row * a.ldgu, col, cnt, true);
             rgh.ask(a.gh, (size_t)row * a.ldgh, col, cnt, true);
+            ry.settle(col, cnt);
+            rh.settle(col, cnt);
+            rgu.settle(col, cnt);
+            rgh.settle(col, cnt);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float n = a.out_kind != NORM_NONE ? (ry.at(e) - st.x) * st.y : ry.at(e);
@@ -552,12 +574,12 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_join(const NormJ
 // ------------------------------------------------------------------------------------------------------------------ host side
 constexpr int NR_MAX_C = 16384;
 
-struct NormShape { int E, WPR, g_log; };
+struct NormShape { int E, WPR, g_log; bool odd; };
 
 // lanes per row so that a lane owns eight channels (sixteen beyond 8192)
-NormShape nr_shape(int C)
+NormShape nr_shape(int C, int dtype)
 {
-    NormShape s = {8, 1, 0};
+    NormShape s = {8, 1, 0, C % (dtype == DT_F32 ? 4 : 8) != 0};
     while (s.WPR < 16 && 64 * s.WPR * s.E < C) s.WPR *= 2;
     if (64 * s.WPR * s.E < C) s.E = 16;
     while (s.g_log < 6 && (s.E << s.g_log) < C) ++s.g_log;
@@ -570,8 +592,13 @@ template <int DT, int V, int NV> int nr_go(bool bwd, const NormArgs &a, int wpr,
 {
 #define NR_GO(W)                                                                                       \
     if (wpr == W) {                                                                                    \
-        if (bwd) k_norm_bwd<DT, V, NV, W><<<grid, W > 4 ? 64 * W : 256, 0, st>>>(a);                   \
-        else k_norm_fwd<DT, V, NV, W><<<grid, W > 4 ? 64 * W : 256, 0, st>>>(a);                       \
+        constexpr bool can = W < 16;                                                                   \
+        const bool odd = can && a.C % V != 0;                                                          \
+        constexpr int T = W > 4 ? 64 * W : 256;                                                        \
+        if (bwd && odd) k_norm_bwd<DT, V, NV, W, can><<<grid, T, 0, st>>>(a);                          \
+        else if (bwd) k_norm_bwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                          \
+        else if (odd) k_norm_fwd<DT, V, NV, W, can><<<grid, T, 0, st>>>(a);                            \
+        else k_norm_fwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                                   \
         return nr_status();                                                                            \
     }
     if constexpr (V * NV == 8) {
@@ -630,10 +657,10 @@ NormChunks nr_split(long long M, long long rows_per_gate, int want, int rows_per
     return c;
 }
 
-// as many workgroups as run at once: three of four waves per CU for 16-bit rows, two for fp32
+// as many workgroups as run at once: three of four waves per CU for 16-bit rows of whole vectors, two for others
 NormChunks nr_rows_split(long long M, long long rows_per_gate, int dtype, const NormShape &s)
 {
-    return nr_split(M, rows_per_gate, dtype == DT_F32 || s.WPR > 4 ? 512 : 768, nr_rows_per_block(s));
+    return nr_split(M, rows_per_gate, dtype == DT_F32 || s.WPR > 4 || s.odd ? 512 : 768, nr_rows_per_block(s));
 }
 
 inline unsigned nr_strips(int C, int dtype) { const int v = 64 * 16 / (dtype == DT_F32 ? 4 : 2); return (unsigned)((C + v - 1) / v); }
@@ -646,7 +673,7 @@ NormChunks nr_sums_split(long long M, long long rows_per_gate, int C, int dtype,
 
 long long nr_bwd_space(long long M, int C, long long rows_per_gate, int dtype)
 {
-    const NormShape s = nr_shape(C);
+    const NormShape s = nr_shape(C, dtype);
     const NormChunks c = nr_sums_split(M, rows_per_gate, C, dtype, s);
     return 20ll * C * c.chunks * c.groups + (s.E == 8 ? 0 : 8 * M);
 }
@@ -674,7 +701,7 @@ BC_EXPORT int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const voi
     a.ho = h_out; a.u = u; a.stats = stats;
     a.ldh = ldh; a.ldy = ldy; a.M = (int)M; a.C = C; a.rows_per_gate = (int)rows_per_gate;
     a.out_kind = out_kind; a.in_kind = in_kind; a.pf32 = params_f32; a.alpha = residual_scale; a.eps = eps;
-    const NormShape s = nr_shape(C);
+    const NormShape s = nr_shape(C, dtype);
     a.g_log = s.g_log;
     const long long blocks = (M + nr_rows_per_block(s) - 1) / nr_rows_per_block(s);
     return nr_dispatch(dtype, false, a, s, (unsigned)(blocks < 4096 ? blocks : 4096), (hipStream_t)stream);
@@ -702,7 +729,7 @@ BC_EXPORT int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void 
     for (int i = 0; i < 9; ++i)
         if (ps[i] && (uintptr_t)ps[i] % pe) return BC_ERR_ALIGN;
     if ((uintptr_t)stats % 16) return BC_ERR_ALIGN;
-    const NormShape s = nr_shape(C);
+    const NormShape s = nr_shape(C, dtype);
     const NormChunks c = nr_rows_split(M, rows_per_gate, dtype, s), q = nr_sums_split(M, rows_per_gate, C, dtype, s);
     const bool sums = d_out_weight || d_out_bias || d_gate || d_in_weight || d_in_bias;
     if (sums && !workspace) return BC_ERR_NULL;
