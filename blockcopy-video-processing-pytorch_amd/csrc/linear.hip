@@ -10,6 +10,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/blockcopy_hip.h"
 
 #define BC_EXPORT extern "C" __attribute__((visibility("default")))
@@ -65,38 +67,64 @@ template <int DT> __device__ __forceinline__ float lin_phi(float z, float &e)
 // gelu_tanh is z * (1 + tanh(u)) / 2 = z * sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3): one exponential, nothing cancels
 constexpr float GELU_A = 0.7978845608028654f, GELU_B = 0.044715f;
 
-template <int DT> __device__ __forceinline__ float lin_act(float z, int act)
+template <int DT, int ACT> __device__ __forceinline__ float lin_act1(float z)
 {
     float e;
-    switch (act) {
-    case ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-    case ACT_GELU: return z * lin_phi<DT>(z, e);
-    case ACT_GELU_TANH: return z * lin_sigmoid<DT>(2.f * GELU_A * z * fmaf(GELU_B * z, z, 1.f));
-    case ACT_SILU: return z * lin_sigmoid<DT>(z);
-    default: return z;
-    }
+    if constexpr (ACT == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+    else if constexpr (ACT == ACT_GELU) return z * lin_phi<DT>(z, e);
+    else if constexpr (ACT == ACT_GELU_TANH) return z * lin_sigmoid<DT>(2.f * GELU_A * z * fmaf(GELU_B * z, z, 1.f));
+    else return z * lin_sigmoid<DT>(z);
 }
 
 // act'(z).  Beyond +-64 every derivative is 0 or 1 to the last bit; the clamp keeps 0 * infinity out of the products (NaN passes through)
-template <int DT> __device__ __forceinline__ float lin_dact(float z, int act)
+template <int DT, int ACT> __device__ __forceinline__ float lin_dact1(float z)
 {
     const float c = z > 64.f ? 64.f : (z < -64.f ? -64.f : z);
-    switch (act) {
-    case ACT_RELU: return z != z ? z : (z > 0.f ? 1.f : 0.f);
-    case ACT_GELU: {
+    if constexpr (ACT == ACT_RELU) return z != z ? z : (z > 0.f ? 1.f : 0.f);
+    else if constexpr (ACT == ACT_GELU) {
         float e;
         const float p = lin_phi<DT>(c, e);
         return fmaf(c * e, 0.3989422804014327f, p);
-    }
-    case ACT_GELU_TANH: {
+    } else if constexpr (ACT == ACT_GELU_TANH) {
         const float s = lin_sigmoid<DT>(2.f * GELU_A * c * fmaf(GELU_B * c, c, 1.f));
         return s + c * s * (1.f - s) * 2.f * GELU_A * fmaf(3.f * GELU_B * c, c, 1.f);
-    }
-    case ACT_SILU: {
+    } else {
         const float s = lin_sigmoid<DT>(c);
         return s * fmaf(c, 1.f - s, 1.f);
     }
-    default: return 1.f;
+}
+
+// W values at once, the choice outside: their chains of dependent instructions run side by side (a choice per value kept them apart: one
+// exponential's latency after the other)
+template <int DT, int ACT, int W> __device__ __forceinline__ void lin_acts1(float *v)
+{
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = lin_act1<DT, ACT>(v[e]);
+}
+
+template <int DT, int W> __device__ __forceinline__ void lin_acts(float *v, int act)
+{
+    switch (act) {
+    case ACT_RELU: return lin_acts1<DT, ACT_RELU, W>(v);
+    case ACT_GELU: return lin_acts1<DT, ACT_GELU, W>(v);
+    case ACT_GELU_TANH: return lin_acts1<DT, ACT_GELU_TANH, W>(v);
+    case ACT_SILU: return lin_acts1<DT, ACT_SILU, W>(v);
+    }
+}
+
+template <int DT, int ACT, int W> __device__ __forceinline__ void lin_dacts1(float *g, const float *z)      // g *= act'(z)
+{
+#pragma unroll
+    for (int e = 0; e < W; ++e) g[e] *= lin_dact1<DT, ACT>(z[e]);
+}
+
+template <int DT, int W> __device__ __forceinline__ void lin_dacts(float *g, const float *z, int act)
+{
+    switch (act) {
+    case ACT_RELU: return lin_dacts1<DT, ACT_RELU, W>(g, z);
+    case ACT_GELU: return lin_dacts1<DT, ACT_GELU, W>(g, z);
+    case ACT_GELU_TANH: return lin_dacts1<DT, ACT_GELU_TANH, W>(g, z);
+    case ACT_SILU: return lin_dacts1<DT, ACT_SILU, W>(g, z);
     }
 }
 
@@ -254,9 +282,7 @@ template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_epilo
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] += b[e];
     if (ep.z) lin_save<S, W>((S *)ep.z + at, v, cnt);
-    if (ep.act != ACT_NONE)
-#pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = lin_act<DT>(v[e], ep.act);
+    lin_acts<DT, W>(v, ep.act);
     if (ep.res)
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] += r[e];
@@ -582,8 +608,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
             lin_load<S, W>(d, (const S *)a.gy + (size_t)m * a.ldg + n, cnt);
             if (a.z) {
                 lin_load<S, W>(z, (const S *)a.z + (size_t)m * a.N + n, cnt);
-#pragma unroll
-                for (int e = 0; e < W; ++e) d[e] *= lin_dact<DT>(z[e], a.act);
+                lin_dacts<DT, W>(d, z, a.act);
             }
             if (a.dz) lin_save<S, W>((S *)a.dz + (size_t)m * a.ldz + n, d, cnt);
 #pragma unroll
@@ -659,10 +684,13 @@ LinPlan lin_plan(int dtype, long long M, long long N, long long K)
     long long s = t128 >= LIN_CUS ? 1 : 2 * LIN_CUS / t128;
     s = s < steps / 8 ? s : steps / 8;
     // fp32: 64 (the matrix instructions take so long that a small tile's operands arrive in time: 17408 x 768 x 256 72 us against 105 with 128,
-    // 1024^3 24 against 34).  16 bits: 256 once that fills the chip and the sum is long enough to pay for an epilogue that nothing overlaps
-    // (16384 x 4096 x 8192: 903 us, 128: 1040, 64: 1565; 8192 x 2048 x 8192: 240, 279, 384 -- but 17408 x 512 x 2048: 77, 60, 65), else 128 while
-    // that, with a long sum in slices of at least 8 steps, gives every CU one (2048 x 512 x 17408: 50 us, 64: 122), else 64 (1024^3 16 us against 22)
-    p.edge = dtype == DT_F32 ? 64 : K >= 1024 && lin_tiles(M, N, 256) >= LIN_CUS ? 256 : t128 * (s > 1 ? s : 1) >= LIN_CUS ? 128 : 64;
+    // 1024^3 24 against 34).  16 bits: 256 once that fills the chip's rounds and the sum is long enough to pay for an epilogue that nothing overlaps
+    // (16384 x 4096 x 8192: 845 us, 128: 970, 64: 1512; 8192 x 2048 x 8192: 225, 250, 345; 8192 x 768 x 4096: 54, 61, 76 -- but 17408 x 512 x 2048: 73,
+    // 58, 66), else 128 while that, with a long sum in slices of at least 8 steps, gives every CU one (2048 x 512 x 17408: 50 us, 64: 122), else 64
+    // (1024^3 11 us against 17)
+    const long long t256 = lin_tiles(M, N, 256), rounds = (t256 + LIN_CUS - 1) / LIN_CUS;
+    const bool full = t256 >= LIN_CUS && 10 * t256 >= 7 * rounds * LIN_CUS;
+    p.edge = dtype == DT_F32 ? 64 : K > 512 && full ? 256 : t128 * (s > 1 ? s : 1) >= LIN_CUS ? 128 : 64;
     p.tm = (unsigned)((M + p.edge - 1) / p.edge);
     p.tn = (unsigned)((N + p.edge - 1) / p.edge);
     const long long tiles = (long long)p.tm * p.tn;
@@ -691,8 +719,16 @@ inline bool lin_direct(const LinOperand &o, bool mc, int dtype)
 template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C> int lin_run(LinArgs &g, const LinPlan &p, hipStream_t st)
 {
     const size_t lds = (size_t)2 * (BM + BN) * C * sizeof(uint4);
-    static const hipError_t attr = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (attr != hipSuccess) return (int)attr;
+    if (lds > 64 * 1024) {      // (asked for once per device)
+        static std::atomic<unsigned long long> asked{0};
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        if (e == hipSuccess && !(asked.load() >> (dev & 63) & 1)) {
+            e = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e == hipSuccess) asked.fetch_or(1ull << (dev & 63));
+        }
+        if (e != hipSuccess) return (int)e;
+    }
     k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C><<<p.tm * p.tn * (unsigned)p.slices, 64 * WM * WN, lds, st>>>(g);
     return lin_status();
 }
@@ -713,10 +749,10 @@ template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *
     if (p.edge == 64) r = direct ? lin_run<DT, 64, 64, 2, 2, AMC, BMC, true, 8>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false, 8>(g, p, st);
     else if constexpr (DT != DT_F32) {
         // (a short sum: steps of 64 bytes halve the images, three workgroups share a CU and one's epilogue runs beside another's products:
-        //  17408 x 512 x 2048 with gelu 77 us against 92; a long one: 128 bytes, half the barriers, 2048 x 2048 x 2048 29 us against 70)
+        //  17408 x 512 x 2048 58 us against 65; a long one: 128 bytes, half the barriers: 8192 x 768 x 4096 61 us against 67, 2048^3 26 against 32)
         if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false, 8>(g, p, st);
         else if (p.edge == 256) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true, 8>(g, p, st);
-        else if (g.K < 1024) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 4>(g, p, st);
+        else if (g.K <= 512) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 4>(g, p, st);
         else r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 8>(g, p, st);
     }
     if (r != BC_OK || p.slices == 1) return r;

@@ -337,7 +337,7 @@ def test_linear_whole_numbers_are_exact(dt, M, K, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DT)
-@pytest.mark.parametrize("M,K,N", [(4100, 72, 4104), (4104, 4104, 72), (72, 4104, 4104), (4099, 136, 4101), (8200, 1032, 2056), (2100, 1001, 1003), (1500, 1002, 1004)])
+@pytest.mark.parametrize("M,K,N", [(4100, 72, 4104), (4104, 4104, 72), (72, 4104, 4104), (4099, 136, 4101), (8200, 1032, 2056), (8192, 576, 2048), (2100, 1001, 1003), (1500, 1002, 1004)])
 def test_linear_large_tiles_are_exact(dt, M, K, N):
     """Enough work for the large tile in each of the three products (and, with odd sizes, what takes its place): whole numbers, exact results."""
     import blockcopy
@@ -650,7 +650,7 @@ def test_captured_and_replayed():
     gen = torch.Generator().manual_seed(37)
     mk = lambda *s: _rand(gen, *s, dtype=torch.float16)
     ins = [[mk(513, 1000), mk(40, 1000), mk(40), mk(513, 40)] for _ in range(3)]
-    side = torch.cuda.Stream()
+    side, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
     graphs = []
     for _ in range(2):
         live = [t.clone().requires_grad_(i < 3) for i, t in enumerate(ins[0])]
@@ -675,8 +675,9 @@ def test_captured_and_replayed():
                 for a, b in zip(live, ins[(r + k) % 3]):
                     a.copy_(b)
         torch.cuda.synchronize()
-        for g, *_ in graphs:
-            g.replay()
+        for (g, *_), s in zip(graphs, streams):        # (at once, each on a stream of its own)
+            with torch.cuda.stream(s):
+                g.replay()
         torch.cuda.synchronize()
         want = []
         for k in range(2):
