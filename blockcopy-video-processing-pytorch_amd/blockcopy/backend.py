@@ -1078,15 +1078,16 @@ class HipBackend:
                       act, code, bias is not None and bias.dtype == torch.float32, _ptr(ws), need))
         return y, z
 
-    def linear_bwd(self, gy, z, x, weight, act: int, want, bias_dtype=None):
-        """(dx, dw, db) of ``linear_fwd`` for the gradient ``gy`` of y; ``want`` = three truth values, None in the place of the others."""
+    def linear_bwd(self, gy, z, x, weight, act: int, want, bias_dtype=None, saved: bool = False):
+        """(dx, dw, db) of ``linear_fwd`` for the gradient ``gy`` of y; ``want`` = three truth values, None in the place of the others;
+        ``saved``: the other tensors are a forward call's own (checked there)."""
         M, N = gy.shape
         K = weight.shape[1] if weight is not None else x.shape[1]
         dt, dev = gy.dtype, gy.device
         code = _DTYPE_CODE.get(dt)
         assert gy.is_cuda and code is not None
-        assert (self._rows_ok(gy, M, N, dt, dev) and self._rows_ok(z, M, N, dt, dev) and self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev)
-                and (z is None or z.is_contiguous()))
+        assert self._rows_ok(gy, M, N, dt, dev)
+        assert saved or (self._rows_ok(z, M, N, dt, dev) and self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev) and (z is None or z.is_contiguous()))
         dx = gy.new_empty((M, K)) if want[0] else None
         dw = gy.new_empty((N, K)) if want[1] else None
         db = gy.new_empty((N,), dtype=bias_dtype or dt) if want[2] else None
@@ -1128,18 +1129,22 @@ class HipBackend:
         return ho, u, stats
 
     def norm_residual_bwd(self, gh, gu, stats, h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind: int, in_kind: int, residual_scale: float,
-                          rows_per_gate: int, want):
-        """Gradients (dh, dy, d out_weight, d out_bias, d gate, d in_weight, d in_bias) of ``norm_residual_fwd``; ``want`` = seven truth values."""
+                          rows_per_gate: int, want, saved: bool = False):
+        """Gradients (dh, dy, d out_weight, d out_bias, d gate, d in_weight, d in_bias) of ``norm_residual_fwd``; ``want`` = seven truth values;
+        ``saved``: all but gh, gu are a forward call's own (checked there)."""
         M, C = h.shape
         dt, dev = h.dtype, h.device
         code = _DTYPE_CODE[dt]
-        assert (self._rows_ok(gh, M, C, dt, dev) and self._rows_ok(gu, M, C, dt, dev) and self._rows_ok(h, M, C, dt, dev) and self._rows_ok(y, M, C, dt, dev)
-                and stats.is_contiguous() and M > 0)
+        assert self._rows_ok(gh, M, C, dt, dev) and self._rows_ok(gu, M, C, dt, dev) and M > 0
+        assert saved or (self._rows_ok(h, M, C, dt, dev) and self._rows_ok(y, M, C, dt, dev) and stats.is_contiguous())
         params = (out_weight, out_bias, gate, in_weight, in_bias)
-        pf32 = self._norm_params(params, C, dt, dev, M // rows_per_gate if rows_per_gate else 0)
+        if saved:
+            pf32 = any(p is not None and p.dtype == torch.float32 for p in params)
+        else:
+            pf32 = self._norm_params(params, C, dt, dev, M // rows_per_gate if rows_per_gate else 0)
         dh = h.new_empty((M, C)) if want[0] else None
         dy = h.new_empty((M, C)) if want[1] else None
-        dp = [p.new_empty(p.shape) if w and p is not None else None for p, w in zip(params, want[2:])]
+        dp = [p.new_empty(p.shape) if p is not None and want[i + 2] else None for i, p in enumerate(params)]
         need = self.lib.bc_norm_residual_bwd_workspace(M, C, rows_per_gate, code) if any(p is not None for p in dp) else 0
         ws = h.new_empty(need, dtype=torch.uint8) if need else None
         self._launch("norm_residual_bwd", self.lib.bc_norm_residual_bwd, dev,

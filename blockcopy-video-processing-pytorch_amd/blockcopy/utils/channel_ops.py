@@ -115,6 +115,17 @@ def _wrapped(out, wrapper):
     return out if out is None or wrapper is None else TensorWrapper._wrap_like(out, wrapper, wrapper.is_blocks)
 
 
+def _first_order(fn):
+    """``once_differentiable`` where a second derivative could be asked for at all (create_graph), else the function itself: its guard costs as
+    much host time as a small product's launch."""
+    guarded = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return backward
+
+
 # ------------------------------------------------------------------------------------------------ product
 def _linear_rows(be, x, weight, bias, residual, act, dim, keep_z):
     """(y in the axis order of x, z, x's rows, the weight's rows)"""
@@ -136,14 +147,14 @@ class _LinearAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gy):
         xr, wr, z = ctx.saved_tensors
         act, dim, be, x_shape, w_shape, bias_dtype = ctx.meta
         want = ctx.needs_input_grad
         dx = dw = db = None
         if want[0] or want[1] or want[2]:
-            dx, dw, db = be.linear_bwd(_rows(_features(gy, dim)), z, xr, wr, act, want[:3], bias_dtype)
+            dx, dw, db = be.linear_bwd(_rows(_features(gy, dim)), z, xr, wr, act, want, bias_dtype, saved=True)
             dx, dw = _back(dx, x_shape, dim), None if dw is None else dw.view(w_shape)
         return dx, dw, db, gy if want[3] else None, None, None, None
 
@@ -202,7 +213,7 @@ class _NormResidual(torch.autograd.Function):
         return (ho, u) if ho is not None and u is not None else (ho if ho is not None else u)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, *grads):
         h, y, out_weight, out_bias, gate, in_weight, in_bias, stats = ctx.saved_tensors
         (out_kind, in_kind, scale, _, rows_per_gate), dim, be, shape = ctx.meta
@@ -216,7 +227,7 @@ class _NormResidual(torch.autograd.Function):
             out = [torch.zeros_like(t) if w else None for t, w in zip((h, y, out_weight, out_bias, flat, in_weight, in_bias), want)]
         else:
             out = be.norm_residual_bwd(None if gh is None else _rows(_features(gh, dim)), None if gu is None else _rows(_features(gu, dim)), stats, h, y, out_weight, out_bias,
-                                       flat, in_weight, in_bias, out_kind, in_kind, scale, rows_per_gate, want)
+                                       flat, in_weight, in_bias, out_kind, in_kind, scale, rows_per_gate, want, saved=True)
         dh, dy, dwo, dbo, dg, dwi, dbi = out
         return (_back(dh, shape, dim), _back(dy, shape, dim), dwo, dbo, None if dg is None else dg.view(gate.shape), dwi, dbi, None, None, None)
 

@@ -20,7 +20,7 @@ class PlainBackend:
         y = CO.act(z, CO.ACTS[act])[0] + (0 if res is None else res.double())
         return y.to(x.dtype), z.to(x.dtype) if keep_z else None
 
-    def linear_bwd(self, gy, z, x, w, act, want, bias_dtype=None):
+    def linear_bwd(self, gy, z, x, w, act, want, bias_dtype=None, saved=False):
         dz = gy.double() * (1 if act == 0 else CO.act(z.double(), CO.ACTS[act])[1])
         return ((dz @ w.double()).to(gy.dtype) if want[0] else None, (dz.t() @ x.double()).to(gy.dtype) if want[1] else None,
                 dz.sum(0).to(bias_dtype or gy.dtype) if want[2] else None)
@@ -37,7 +37,7 @@ class PlainBackend:
         stats = torch.full((h.shape[0], 4), eps) if keep_stats else None
         return None if y is None else ho.to(h.dtype), None if u is None else u.to(h.dtype), stats
 
-    def norm_residual_bwd(self, gh, gu, stats, h, y, wo, bo, gate, wi, bi, out_kind, in_kind, scale, rpg, want):
+    def norm_residual_bwd(self, gh, gu, stats, h, y, wo, bo, gate, wi, bi, out_kind, in_kind, scale, rpg, want, saved=False):
         src = (h, y, wo, bo, gate, wi, bi)
         args = [None if t is None else t.detach().double().requires_grad_(True) for t in src]
         with torch.enable_grad():
