@@ -1060,8 +1060,17 @@ class HipBackend:
         if rc:
             self._check(rc, op)
 
-    def linear_fwd(self, x, weight, bias=None, act: int = 0, residual=None, keep_z: bool = False):
-        """(y, z): y = act(z) + residual with z = x weight^T + bias; z is handed back (x's dtype) if ``keep_z``."""
+    @staticmethod
+    def _out(t, rows, cols, like):
+        """Memory for a (rows, cols) result: ``t`` (any axis order whose memory is that matrix), or new."""
+        if t is None:
+            return like.new_empty((rows, cols))
+        assert t.numel() == rows * cols and t.dtype == like.dtype and t.device == like.device
+        assert t.is_contiguous() or t.is_contiguous(memory_format=torch.channels_last)
+        return t
+
+    def linear_fwd(self, x, weight, bias=None, act: int = 0, residual=None, keep_z: bool = False, out=None):
+        """(y, z): y = act(z) + residual with z = x weight^T + bias; z is handed back (x's dtype) if ``keep_z``; y is written to ``out`` if given."""
         M, K = x.shape
         N = weight.shape[0]
         dt, dev = x.dtype, x.device
@@ -1069,7 +1078,7 @@ class HipBackend:
         assert x.is_cuda and code is not None, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
         assert self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev) and self._rows_ok(residual, M, N, dt, dev)
         assert bias is None or (bias.shape == (N,) and bias.is_contiguous() and bias.dtype in (dt, torch.float32) and bias.device == dev)
-        y = x.new_empty((M, N))
+        y = self._out(out, M, N, x)
         z = x.new_empty((M, N)) if keep_z else None
         need = self.lib.bc_linear_fwd_workspace(M, N, K, code)
         ws = x.new_empty(need, dtype=torch.uint8) if need else None
@@ -1112,16 +1121,17 @@ class HipBackend:
         return kind == torch.float32
 
     def norm_residual_fwd(self, h, y, out_weight, out_bias, gate, in_weight, in_bias, out_kind: int, in_kind: int, residual_scale: float, eps: float,
-                          rows_per_gate: int = 0, keep_stats: bool = False):
-        """(h_new, u, stats): h_new = residual_scale * h + gate * N_out(y), u = N_in(h_new) (blockcopy/utils/channel_ops.py); None for what is not asked for."""
+                          rows_per_gate: int = 0, keep_stats: bool = False, out=(None, None)):
+        """(h_new, u, stats): h_new = residual_scale * h + gate * N_out(y), u = N_in(h_new) (blockcopy/utils/channel_ops.py); None for what is not asked
+        for; h_new and u are written to the tensors of ``out`` that are given."""
         M, C = h.shape
         dt, dev = h.dtype, h.device
         code = _DTYPE_CODE.get(dt)
         assert h.is_cuda and code is not None, "blockcopy ops need GPU tensors (no CPU path) of float32 / float16 / bfloat16"
         assert self._rows_ok(h, M, C, dt, dev) and self._rows_ok(y, M, C, dt, dev)
         pf32 = self._norm_params((out_weight, out_bias, gate, in_weight, in_bias), C, dt, dev, M // rows_per_gate if rows_per_gate else 0)
-        ho = h.new_empty((M, C)) if y is not None else None
-        u = h.new_empty((M, C)) if in_kind else None
+        ho = self._out(out[0], M, C, h) if y is not None else None
+        u = self._out(out[1], M, C, h) if in_kind else None
         stats = h.new_empty((M, 4), dtype=torch.float32) if keep_stats else None
         self._launch("norm_residual_fwd", self.lib.bc_norm_residual_fwd, dev,
                      (_ptr(ho), _ptr(u), _ptr(stats), h.data_ptr(), _ptr(y), _ptr(out_weight), _ptr(out_bias), _ptr(gate), _ptr(in_weight), _ptr(in_bias), M, C, self._ld(h),

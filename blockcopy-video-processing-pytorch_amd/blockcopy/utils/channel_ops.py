@@ -56,6 +56,11 @@ def _back(t, shape, dim):
     return t.view(shape) if dim == -1 else t.view(shape[0], shape[2], shape[3], shape[1]).permute(0, 3, 1, 2)
 
 
+def _result(x, shape, dim):
+    """Memory for a result of ``shape`` whose features lie together.  Never a view: autograd lets results be modified in place (a ReLU)."""
+    return x.new_empty(shape) if dim == -1 else torch.empty(shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
+
+
 def _rows(x):
     """(rows, features) view of x, or of a contiguous copy where its strides allow none (features apart, overlapping rows)."""
     f = x.shape[-1]
@@ -130,10 +135,11 @@ def _first_order(fn):
 def _linear_rows(be, x, weight, bias, residual, act, dim, keep_z):
     """(y in the axis order of x, z, x's rows, the weight's rows)"""
     xr, wr = _rows(_features(x, dim)), _rows(weight if weight.dim() == 2 else weight.flatten(1))
-    y, z = be.linear_fwd(xr, wr, bias, act, None if residual is None else _rows(_features(residual, dim)), keep_z)
     shape = list(x.shape)
     shape[dim] = wr.shape[0]
-    return _back(y, shape, dim), z, xr, wr
+    y = _result(x, shape, dim)
+    z = be.linear_fwd(xr, wr, bias, act, None if residual is None else _rows(_features(residual, dim)), keep_z, out=y)[1]
+    return y, z, xr, wr
 
 
 class _LinearAct(torch.autograd.Function):
@@ -197,10 +203,10 @@ def _norm_rows(be, h, y, params, kinds, dim, keep_stats):
     """(h', u, stats, h's rows, y's rows); h', u in the axis order of h"""
     hr, yr = _rows(_features(h, dim)), None if y is None else _rows(_features(y, dim))
     wo, bo, gate, wi, bi = params
-    if hr.shape[0] == 0:
-        return None if y is None else h.new_empty(h.shape), h.new_empty(h.shape) if kinds[1] else None, None, hr, yr
-    ho, u, stats = be.norm_residual_fwd(hr, yr, wo, bo, None if gate is None else gate.view(-1), wi, bi, *kinds, keep_stats)
-    return _back(ho, h.shape, dim), _back(u, h.shape, dim), stats, hr, yr
+    ho, u, stats = None if y is None else _result(h, h.shape, dim), _result(h, h.shape, dim) if kinds[1] else None, None
+    if hr.shape[0]:
+        stats = be.norm_residual_fwd(hr, yr, wo, bo, None if gate is None else gate.view(-1), wi, bi, *kinds, keep_stats, out=(ho, u))[2]
+    return ho, u, stats, hr, yr
 
 
 class _NormResidual(torch.autograd.Function):

@@ -15,10 +15,17 @@ class PlainBackend:
 
     name = "plain"
 
-    def linear_fwd(self, x, w, b=None, act=0, res=None, keep_z=False):
+    @staticmethod
+    def _put(out, rows):
+        if out is None or rows is None:
+            return rows
+        (out.permute(0, 2, 3, 1) if out.dim() == 4 and out.numel() and out.stride(1) == 1 else out).view(rows.shape).copy_(rows)
+        return out
+
+    def linear_fwd(self, x, w, b=None, act=0, res=None, keep_z=False, out=None):
         z = x.double() @ w.double().t() + (0 if b is None else b.double())
         y = CO.act(z, CO.ACTS[act])[0] + (0 if res is None else res.double())
-        return y.to(x.dtype), z.to(x.dtype) if keep_z else None
+        return self._put(out, y.to(x.dtype)), z.to(x.dtype) if keep_z else None
 
     def linear_bwd(self, gy, z, x, w, act, want, bias_dtype=None, saved=False):
         dz = gy.double() * (1 if act == 0 else CO.act(z.double(), CO.ACTS[act])[1])
@@ -31,11 +38,11 @@ class PlainBackend:
         gate = gate if gate is None or not rpg else gate.view(-1, h.shape[1])
         return CO.norm_residual(h, y, {"wo": wo, "bo": bo, "wi": wi, "bi": bi}, gate, scale, kinds[out_kind], kinds[in_kind], eps, rpg)
 
-    def norm_residual_fwd(self, h, y, wo, bo, gate, wi, bi, out_kind, in_kind, scale, eps, rpg=0, keep_stats=False):
+    def norm_residual_fwd(self, h, y, wo, bo, gate, wi, bi, out_kind, in_kind, scale, eps, rpg=0, keep_stats=False, out=(None, None)):
         args = [None if t is None else t.double() for t in (h, y, wo, bo, gate, wi, bi)]
         ho, u = self._norm(*args, out_kind, in_kind, scale, eps, rpg)
         stats = torch.full((h.shape[0], 4), eps) if keep_stats else None
-        return None if y is None else ho.to(h.dtype), None if u is None else u.to(h.dtype), stats
+        return None if y is None else self._put(out[0], ho.to(h.dtype)), None if u is None else self._put(out[1], u.to(h.dtype)), stats
 
     def norm_residual_bwd(self, gh, gu, stats, h, y, wo, bo, gate, wi, bi, out_kind, in_kind, scale, rpg, want, saved=False):
         src = (h, y, wo, bo, gate, wi, bi)
@@ -214,6 +221,23 @@ def test_gradient_of_one_output_only(plain_backend):
     (gx,) = torch.autograd.grad(blockcopy.linear_act(x, w, activation="silu").sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError):
         gx.sum().backward()
+
+
+@pytest.mark.parametrize("shape,dim", [((4, 6), -1), ((2, 3, 6), -1), ((2, 6, 3, 5), 1)])
+def test_results_may_be_modified_in_place(plain_backend, shape, dim):
+    """As any other operation's results: y.relu_() and its like, with the gradients of the composition."""
+    import blockcopy
+
+    gen = torch.Generator().manual_seed(3)
+    x, w = torch.randn(shape, generator=gen, requires_grad=True), torch.randn(6, 6, generator=gen, requires_grad=True)
+    y = blockcopy.linear_act(x, w, dim=dim)
+    h, u = blockcopy.norm_residual(x, y, in_norm="rms", dim=dim)
+    got = torch.autograd.grad(h.relu_().sum() + u.mul_(2).pow(2).sum() + blockcopy.linear_act(x, w, dim=dim).add_(1).pow(2).sum(), [x, w])
+    rows = x.permute(0, 2, 3, 1) if dim == 1 else x
+    yr = rows @ w.t()
+    hr, ur = rows + yr, CO.normed(rows + yr, "rms", None, None, 1e-6)
+    want = torch.autograd.grad(hr.relu().sum() + (2 * ur).pow(2).sum() + (yr + 1).pow(2).sum(), [x, w])
+    assert all(torch.allclose(a, b, atol=1e-3, rtol=1e-4) for a, b in zip(got, want))
 
 
 def test_no_rows(plain_backend):
