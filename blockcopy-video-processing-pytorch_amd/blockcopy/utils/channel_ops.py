@@ -255,7 +255,7 @@ def _gate(name, gate, h, C, dim, packed):
         if s[0] == h.shape[0] and not packed:
             if s[0] > 65535:
                 raise ValueError(f"{name}: gates for at most 65535 samples, got {s[0]}")
-            return gate, h.numel() // (C * s[0])
+            return gate, h.numel() // gate.numel() if s[0] else 0
     raise ValueError(f"{name}: gate must hold one value per channel ({C},) or per sample and channel, got {tuple(s)} for {tuple(h.shape)}"
                      + ("; packed tiles are no samples" if packed else ""))
 

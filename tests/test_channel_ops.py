@@ -256,6 +256,11 @@ def test_no_rows(plain_backend):
     ho, u = blockcopy.norm_residual(h, h, gate=g)
     gh, gg = torch.autograd.grad(ho.sum(), [h, g])
     assert u is None and ho.shape == gh.shape == (2, 0, 4) and torch.equal(gg, torch.zeros(2, 1, 4))
+    for h, g, dim in ((torch.empty(0, 3, 4), torch.ones(0, 1, 4), -1), (torch.empty(0, 4, 2, 2), torch.ones(0, 4, 1, 1), 1)):        # no samples: no gates either
+        h.requires_grad_(True), g.requires_grad_(True)
+        ho, u = blockcopy.norm_residual(h, h, gate=g, in_norm="layer", dim=dim)
+        gh, gg = torch.autograd.grad(ho.sum() + u.sum(), [h, g])
+        assert ho.shape == u.shape == gh.shape == h.shape and gg.shape == g.shape
 
 
 # ------------------------------------------------------------------------------------------------ GPU
