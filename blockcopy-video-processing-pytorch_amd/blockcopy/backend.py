@@ -1091,7 +1091,7 @@ class HipBackend:
         """(dx, dw, db) of ``linear_fwd`` for the gradient ``gy`` of y; ``want`` = three truth values, None in the place of the others;
         ``saved``: the other tensors are a forward call's own (checked there)."""
         M, N = gy.shape
-        K = weight.shape[1] if weight is not None else x.shape[1]
+        K = weight.shape[1] if weight is not None else x.shape[1] if x is not None else 1       # (the bias alone: neither is there)
         dt, dev = gy.dtype, gy.device
         code = _DTYPE_CODE.get(dt)
         assert gy.is_cuda and code is not None

@@ -576,6 +576,48 @@ def test_norm_rows_are_independent(dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("M,K,N", [(70, 40, 24), (1100, 1026, 1030)])
+def test_each_linear_gradient_alone(dt, M, K, N):
+    """Frozen arguments (a bias tuned alone, a first layer's input) change no bit of the other gradients."""
+    import blockcopy
+
+    gen = torch.Generator().manual_seed(47)
+    ts = [_rand(gen, M, K, dtype=DT[dt]), _rand(gen, N, K, dtype=DT[dt], std=K ** -0.5), _rand(gen, N, dtype=DT[dt]), _rand(gen, M, N, dtype=DT[dt])]
+    gy = _rand(gen, M, N, dtype=DT[dt])
+    for act in ("none", "gelu"):
+        def grads(live):
+            args = [t.clone().requires_grad_(i in live) for i, t in enumerate(ts)]
+            return torch.autograd.grad(blockcopy.linear_act(args[0], args[1], args[2], act, args[3]), [args[i] for i in live], gy)
+
+        full = grads(range(4))
+        for live in itertools.chain(*(itertools.combinations(range(4), r) for r in (1, 2, 3))):
+            assert all(torch.equal(g, full[i]) for i, g in zip(live, grads(live))), (act, live)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("C", [40, 1030, 9000])
+def test_each_norm_gradient_alone(dt, C):
+    import blockcopy
+
+    gen = torch.Generator().manual_seed(53)
+    M = 60
+    ts = [_rand(gen, M, C, dtype=DT[dt]), _rand(gen, M, C, dtype=DT[dt]), *(_rand(gen, C, dtype=DT[dt], mean=1.0, std=0.2) for _ in range(5))]
+    gs = [_rand(gen, M, C, dtype=DT[dt]) for _ in range(2)]
+
+    def grads(live, use):
+        a = [t.clone().requires_grad_(i in live) for i, t in enumerate(ts)]
+        out = blockcopy.norm_residual(a[0], a[1], out_norm="layer", out_weight=a[2], out_bias=a[3], gate=a[4], in_norm="rms", in_weight=a[5], in_bias=a[6])
+        return torch.autograd.grad([out[i] for i in use], [a[i] for i in live], [gs[i] for i in use])
+
+    for use in ((0, 1), (1,)):
+        full = grads(range(7), use)
+        for i in range(7):
+            assert torch.equal(grads([i], use)[0], full[i]), (use, i)
+
+
+@pytest.mark.gpu
 def test_results_repeat_bit_for_bit():
     import blockcopy
 
