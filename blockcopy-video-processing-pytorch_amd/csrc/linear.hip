@@ -852,7 +852,7 @@ template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, hipStr
 // (32 x 1024 x 1024 4.8 us against 6.0, 32 x 4096 x 4096 14 against 11)
 static bool lin_takes_few(const void *x, const void *w, long long M, int N, int K, long long ldx, long long ldw, int dtype)
 {
-    if (M > 32 || (M > 16 && K > 1024) || (N < 1024 && K > 2048)) return false;
+    if (M > 32 || (M > 16 && K > 1024) || (N < 1024 && K > 2048) || N > 16 * 0x3fffff) return false;       // (the launch: below 2^32 threads)
     return dtype == DT_F32 || ((uintptr_t)x % 4 == 0 && (uintptr_t)w % 4 == 0 && ldx % 2 == 0 && ldw % 2 == 0);
 }
 
@@ -940,7 +940,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
     char *wsp = (char *)workspace, *pack = wsp + s.dz + s.part + s.slices;
     void *slices = wsp + s.dz + s.part;
     LinOperand dz = {gy, ldg, N};
-    const bool store = act != ACT_NONE || (s.order_n && !lin_direct(dz, true, dtype));
+    const bool store = (dx || dw) && (act != ACT_NONE || s.order_n);
     if (store || db) {
         const DactPlan p = lin_dact_plan(M, N, dtype);
         DactArgs a = {};
@@ -962,7 +962,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
     if (dx) {       // dx[m][k] = sum_n dz[m][n] w[n][k]: the weight runs across the summed index
         LinArgs g = {};
         g.a = {w, ldw, K};
-        if (s.order_k && !lin_direct(g.a, true, dtype)) g.a = lin_pack(g.a, N, &pack, dtype, st);
+        if (s.order_k) g.a = lin_pack(g.a, N, &pack, dtype, st);
         g.b = {dz.p, dz.ld, N};
         g.M = (int)M;
         g.N = K;
@@ -974,7 +974,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
     if (dw) {       // dw[n][k] = sum_m dz[m][n] x[m][k]: both run across it
         LinArgs g = {};
         g.a = {x, ldx, K};
-        if (s.order_k && !lin_direct(g.a, true, dtype)) g.a = lin_pack(g.a, M, &pack, dtype, st);
+        if (s.order_k) g.a = lin_pack(g.a, M, &pack, dtype, st);
         g.b = dz;
         g.M = N;
         g.N = K;

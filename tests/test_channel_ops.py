@@ -782,6 +782,20 @@ def test_on_another_stream_and_two_at_once():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 20])
+def test_very_many_columns(M):
+    """One launch of the kernel for few rows has fewer than 2^32 threads: beyond its columns the tiles take over."""
+    import blockcopy
+
+    N = 70_000_003 if M == 1 else 9_000_001
+    w = (torch.arange(N, device="cuda") % 1021).to(torch.float16)[:, None]
+    x = torch.arange(1, M + 1, device="cuda", dtype=torch.float16)[:, None]
+    y = blockcopy.linear_act(x, w)
+    for m in {0, M - 1}:        # (whole numbers: exact up to 2048, rounded once beyond)
+        assert torch.equal(y[m], (w[:, 0].float() * (m + 1)).half())
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits():
     """More than 2^31 elements in one operand: rows at the far end are read and written at their own places."""
     import blockcopy
