@@ -55,45 +55,73 @@ template <int CTRL> __device__ __forceinline__ float nr_dpp(float v)
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
 }
 
+typedef unsigned nr_pair __attribute__((ext_vector_type(2)));
+
+// v + the v of the lane 16 / 32 away, without the LDS
+__device__ __forceinline__ float nr_swap16(float v)
+{
+    const nr_pair p = __builtin_bit_cast(nr_pair, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+__device__ __forceinline__ float nr_swap32(float v)
+{
+    const nr_pair p = __builtin_bit_cast(nr_pair, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
 __device__ __forceinline__ float nr_wave_sum(float v, int g_log)
 {
     if (g_log > 0) v = nr_dpp<0xB1>(v);         // quad_perm 1 0 3 2
     if (g_log > 1) v = nr_dpp<0x4E>(v);         // quad_perm 2 3 0 1
     if (g_log > 2) v = nr_dpp<0x141>(v);        // row_half_mirror
     if (g_log > 3) v = nr_dpp<0x140>(v);        // row_mirror
-    if (g_log > 4) v += __shfl_xor(v, 16);
-    if (g_log > 5) v += __shfl_xor(v, 32);
+    if (g_log > 4) v = nr_swap16(v);
+    if (g_log > 5) v = nr_swap32(v);
     return v;
 }
 
-// WPR waves share a row: the waves' sums meet in `red` (two halves used in turn, so one barrier per exchange is enough)
+// WPR waves share a row: the waves' sums meet in `red` (two halves used in turn, so one barrier per exchange is enough; entries of waves that
+// were not launched stay zeros).  Lane l reads wave l % WPR's and the lanes add up by exchange
 template <int WPR, int NW> struct NrSum {
-    float *red;         // [2][NW][2]
+    static constexpr int LOG = WPR == 16 ? 4 : WPR == 8 ? 3 : WPR == 4 ? 2 : WPR == 2 ? 1 : 0;
+    float2 *red;            // [2][NW]
     int turn, wave, g_log;
+    float n, inv_n;         // channels of wave lane % WPR, and their reciprocal (0: none)
+    __device__ __forceinline__ float2 exchange(float a, float b)
+    {
+        float2 *r = red + turn * NW;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) r[wave] = float2{a, b};
+        __syncthreads();
+        return r[wave / WPR * WPR + (threadIdx.x & (WPR - 1))];
+    }
     __device__ __forceinline__ void operator()(float &a, float &b, bool two)
     {
         a = nr_wave_sum(a, g_log);
         if (two) b = nr_wave_sum(b, g_log);
         if constexpr (WPR > 1) {
-            float *r = red + turn * (2 * NW);
-            turn ^= 1;
-            if ((threadIdx.x & 63) == 0) {
-                r[2 * wave] = a;
-                r[2 * wave + 1] = b;
-            }
-            __syncthreads();
-            const float *q = r + 2 * (wave / WPR * WPR);
-            float sa = 0.f, sb = 0.f;
-#pragma unroll
-            for (int w = 0; w < WPR; ++w) {
-                sa += q[2 * w];
-                sb += q[2 * w + 1];
-            }
-            a = sa;
-            b = sb;
+            const float2 t = exchange(a, b);
+            a = nr_wave_sum(t.x, LOG);
+            if (two) b = nr_wave_sum(t.y, LOG);
         }
     }
 };
+
+template <int WPR, int NW, int V, int NV> __device__ __forceinline__ NrSum<WPR, NW> nr_sum(float2 *red, int wave, int g_log, int G, int C)
+{
+    NrSum<WPR, NW> s = {red, 0, wave, g_log, 0.f, 0.f};
+    if constexpr (WPR > 1) {
+        if (threadIdx.x < 2 * NW) red[threadIdx.x] = float2{0.f, 0.f};
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) n += min(max(C - (i * G + 64 * (int)(threadIdx.x & (WPR - 1))) * V, 0), min(64, max(G - 64 * (int)(threadIdx.x & (WPR - 1)), 0)) * V);
+        s.n = (float)n;
+        s.inv_n = n ? 1.f / s.n : 0.f;
+        __syncthreads();
+    }
+    return s;
+}
 
 // `cnt` of V elements at column `at` of row `base` (in elements).  With the base in scalar registers (whole waves share a row) a lane's address
 // is one 32-bit offset.  Rows of any width and start: the 16-byte accesses ask for the alignment of an element only (the hardware takes
@@ -185,24 +213,39 @@ template <typename S, int V, int NV> __device__ __forceinline__ void nr_params(f
     for (int i = 0; i < NV; ++i) nr_param<S, V>(f + i * V, p, pf32, base, col[i], cnt[i], none);
 }
 
-// x[E] -> normalised in place (0 behind the row's end); mean and 1 / deviation returned.  E = NV vectors of V
-template <int V, int NV, class Sum> __device__ __forceinline__ void nr_normalise(float *x, int kind, const int *cnt, float inv_c, float eps, Sum &sum, float &mean, float &rstd)
+// x[E] -> normalised in place (0 behind the row's end); mean and 1 / deviation returned.  E = NV vectors of V.  Variances are sums of squared
+// distances from the mean.  Of the row where a wave or less holds it; where waves share it, each takes the distances from its own mean, and
+// sum (x - mean)^2 = sum over waves of [sum (x - mean_w)^2 + n_w (mean_w - mean)^2]: one exchange instead of two
+template <int V, int NV, int WPR, int NW>
+__device__ __forceinline__ void nr_normalise(float *x, int kind, const int *cnt, float inv_c, float eps, float own_inv_n, NrSum<WPR, NW> &sum, float &mean, float &rstd)
 {
-    float none = 0.f;
+    float q = 0.f, none = 0.f;
     mean = 0.f;
     if (kind == NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV * V; ++i) s += x[i];
-        sum(s, none, false);
-        mean = s * inv_c;
+        s = nr_wave_sum(s, sum.g_log);
+        mean = s * (WPR > 1 ? own_inv_n : inv_c);
+        if constexpr (WPR > 1) {
+#pragma unroll
+            for (int i = 0; i < NV * V; ++i) {
+                const float d = i % V < cnt[i / V] ? x[i] - mean : 0.f;
+                q += d * d;
+            }
+            const float2 t = sum.exchange(s, nr_wave_sum(q, sum.g_log));
+            mean = nr_wave_sum(t.x, sum.LOG) * inv_c;
+            const float d = t.x * sum.inv_n - mean;
+            q = nr_wave_sum(t.y + sum.n * d * d, sum.LOG);
+        }
 #pragma unroll
         for (int i = 0; i < NV * V; ++i) x[i] = i % V < cnt[i / V] ? x[i] - mean : 0.f;
     }
-    float q = 0.f;
+    if (WPR == 1 || kind != NORM_LAYER) {
 #pragma unroll
-    for (int i = 0; i < NV * V; ++i) q += x[i] * x[i];
-    sum(q, none, false);
+        for (int i = 0; i < NV * V; ++i) q += x[i] * x[i];
+        sum(q, none, false);
+    }
     rstd = 1.f / sqrtf(q * inv_c + eps);
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) x[i] *= rstd;
@@ -213,12 +256,13 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
 {
     typedef typename NrT<DT>::S S;
     constexpr int NT = WPR > 4 ? 64 * WPR : 256, NW = NT / 64, E = V * NV;
-    __shared__ float red[4 * NW];
+    __shared__ float2 red[2 * NW];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int G = WPR > 1 ? 64 * WPR : 1 << a.g_log, lr = WPR > 1 ? tid % (64 * WPR) : tid & (G - 1), RPB = NT / G;
-    const int slot = WPR > 1 ? wave / WPR : tid >> a.g_log;       // (a scalar where whole waves share a row)
+    // (rows of 4 waves and more have a workgroup of their own, of as many waves as hold channels)
+    const int G = WPR > 2 ? (int)blockDim.x : WPR > 1 ? 128 : 1 << a.g_log, lr = tid & (WPR > 2 ? 1023 : G - 1), RPB = WPR > 2 ? 1 : 256 / G;
+    const int slot = WPR > 2 ? 0 : WPR > 1 ? wave >> 1 : tid >> a.g_log;       // (a scalar where whole waves share a row)
     const float inv_c = 1.f / (float)a.C;
-    NrSum<WPR, NW> sum = {red, 0, wave, a.g_log};
+    NrSum<WPR, NW> sum = nr_sum<WPR, NW, V, NV>(red, wave, a.g_log, G, a.C);
     unsigned col[NV];
     int cnt[NV];        // how many of a vector's channels exist
 #pragma unroll
@@ -226,7 +270,8 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
         col[i] = (i * G + lr) * V;
         cnt[i] = a.C - (int)col[i];
     }
-    constexpr bool KEEP = WPR < 16;     // parameters and the next row stay in registers (16 waves leave a lane 128 of them: asked for at their turn)
+    const float own_inv_n = WPR > 1 ? __shfl(sum.inv_n, wave % WPR) : 0.f;
+    constexpr bool KEEP = WPR < 16 || (E == 8 && DT != DT_F32);     // parameters and the next row stay in registers (16 waves leave a lane 128 of them: else asked for at their turn)
     const bool outer = a.y != nullptr && a.out_kind != NORM_NONE, inner = a.in_kind != NORM_NONE;
     float wo[E], bo[E], gate[E], wi[E], bi[E];
     if constexpr (KEEP) {
@@ -265,7 +310,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
         if (a.y) {
             if (!KEEP || a.rows_per_gate) nr_params<S, V, NV>(gate, live ? a.gate : nullptr, a.pf32, live && a.rows_per_gate ? (size_t)(row / a.rows_per_gate) * a.C : 0, col, cnt, 1.f);
             if (outer) {
-                nr_normalise<V, NV>(x, a.out_kind, cnt, inv_c, a.eps, sum, mean_y, rstd_y);
+                nr_normalise<V, NV, WPR, NW>(x, a.out_kind, cnt, inv_c, a.eps, own_inv_n, sum, mean_y, rstd_y);
                 if constexpr (!KEEP) {
                     nr_params<S, V, NV>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
                     nr_params<S, V, NV>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
@@ -282,7 +327,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] = h[i];
         if (inner) {
-            nr_normalise<V, NV>(x, a.in_kind, cnt, inv_c, a.eps, sum, mean_h, rstd_h);
+            nr_normalise<V, NV, WPR, NW>(x, a.in_kind, cnt, inv_c, a.eps, own_inv_n, sum, mean_h, rstd_h);
             if constexpr (!KEEP) {
                 nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
                 nr_params<S, V, NV>(bi, a.bi, a.pf32, 0, col, cnt, 0.f);
@@ -333,13 +378,14 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
 {
     typedef typename NrT<DT>::S S;
     constexpr int NT = WPR > 4 ? 64 * WPR : 256, NW = NT / 64, E = V * NV;
-    __shared__ float red[4 * NW];
+    __shared__ float2 red[2 * NW];
     __shared__ float meet[WPR > 2 ? 1 : 256 * E];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int G = WPR > 1 ? 64 * WPR : 1 << a.g_log, lr = WPR > 1 ? tid % (64 * WPR) : tid & (G - 1), RPB = NT / G;
-    const int slot = WPR > 1 ? wave / WPR : tid >> a.g_log;       // (a scalar where whole waves share a row)
+    // (rows of 4 waves and more have a workgroup of their own, of as many waves as hold channels)
+    const int G = WPR > 2 ? (int)blockDim.x : WPR > 1 ? 128 : 1 << a.g_log, lr = tid & (WPR > 2 ? 1023 : G - 1), RPB = WPR > 2 ? 1 : 256 / G;
+    const int slot = WPR > 2 ? 0 : WPR > 1 ? wave >> 1 : tid >> a.g_log;       // (a scalar where whole waves share a row)
     const float inv_c = 1.f / (float)a.C;
-    NrSum<WPR, NW> sum = {red, 0, wave, a.g_log};
+    NrSum<WPR, NW> sum = nr_sum<WPR, NW, V, NV>(red, wave, a.g_log, G, a.C);
     unsigned col[NV];
     int cnt[NV];        // how many of a vector's channels exist
 #pragma unroll
@@ -574,30 +620,30 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_join(const NormJ
 // ------------------------------------------------------------------------------------------------------------------ host side
 constexpr int NR_MAX_C = 16384;
 
-struct NormShape { int E, WPR, g_log; bool odd; };
+struct NormShape { int E, WPR, waves, g_log; bool odd; };      // waves: those of a row that have channels
 
 // lanes per row so that a lane owns eight channels (sixteen beyond 8192)
 NormShape nr_shape(int C, int dtype)
 {
-    NormShape s = {8, 1, 0, C % (dtype == DT_F32 ? 4 : 8) != 0};
+    NormShape s = {8, 1, 1, 0, C % (dtype == DT_F32 ? 4 : 8) != 0};
     while (s.WPR < 16 && 64 * s.WPR * s.E < C) s.WPR *= 2;
     if (64 * s.WPR * s.E < C) s.E = 16;
     while (s.g_log < 6 && (s.E << s.g_log) < C) ++s.g_log;
+    s.waves = (C + 64 * s.E - 1) / (64 * s.E);
     return s;
 }
 
 inline int nr_rows_per_block(const NormShape &s) { return s.WPR > 1 ? (s.WPR > 4 ? 1 : 4 / s.WPR) : 256 >> s.g_log; }
 
-template <int DT, int V, int NV> int nr_go(bool bwd, const NormArgs &a, int wpr, unsigned grid, hipStream_t st)
+template <int DT, int V, int NV> int nr_go(bool bwd, const NormArgs &a, const NormShape &s, unsigned grid, hipStream_t st)
 {
 #define NR_GO(W)                                                                                       \
-    if (wpr == W) {                                                                                    \
-        constexpr bool can = W < 16;                                                                   \
-        const bool odd = can && a.C % V != 0;                                                          \
-        constexpr int T = W > 4 ? 64 * W : 256;                                                        \
-        if (bwd && odd) k_norm_bwd<DT, V, NV, W, can><<<grid, T, 0, st>>>(a);                          \
+    if (s.WPR == W) {                                                                                  \
+        constexpr bool fwd_odd = W < 16 || (V * NV == 8 && DT != DT_F32), bwd_odd = W < 16;            \
+        const int T = W > 2 ? 64 * s.waves : 256;                                                      \
+        if (bwd && bwd_odd && s.odd) k_norm_bwd<DT, V, NV, W, bwd_odd><<<grid, T, 0, st>>>(a);         \
         else if (bwd) k_norm_bwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                          \
-        else if (odd) k_norm_fwd<DT, V, NV, W, can><<<grid, T, 0, st>>>(a);                            \
+        else if (fwd_odd && s.odd) k_norm_fwd<DT, V, NV, W, fwd_odd><<<grid, T, 0, st>>>(a);           \
         else k_norm_fwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                                   \
         return nr_status();                                                                            \
     }
@@ -615,7 +661,7 @@ template <int DT, int V, int NV> int nr_go(bool bwd, const NormArgs &a, int wpr,
 template <int DT> int nr_launch(bool bwd, const NormArgs &a, const NormShape &s, unsigned grid, hipStream_t st)
 {
     constexpr int V = NrT<DT>::V;
-    return s.E == 8 ? nr_go<DT, V, 8 / V>(bwd, a, s.WPR, grid, st) : nr_go<DT, V, 16 / V>(bwd, a, s.WPR, grid, st);
+    return s.E == 8 ? nr_go<DT, V, 8 / V>(bwd, a, s, grid, st) : nr_go<DT, V, 16 / V>(bwd, a, s, grid, st);
 }
 
 int nr_dispatch(int dtype, bool bwd, const NormArgs &a, const NormShape &s, unsigned grid, hipStream_t st)
