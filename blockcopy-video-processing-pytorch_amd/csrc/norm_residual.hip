@@ -123,67 +123,84 @@ template <int WPR, int NW, int V, int NV> __device__ __forceinline__ NrSum<WPR, 
     return s;
 }
 
-// `cnt` of V elements at column `at` of row `base` (in elements).  With the base in scalar registers (whole waves share a row) a lane's address
-// is one 32-bit offset.  Rows of any width and start: the 16-byte accesses ask for the alignment of an element only (the hardware takes
-// unaligned vectors), the last vector of a row goes element by element.
+// `cnt` of V elements (all of them or none unless ODD) at column `at` of row `base` (in elements).  With the base in scalar registers (whole
+// waves share a row) a lane's address is one 32-bit offset.  Rows of any width and start: the 16-byte accesses ask for the alignment of an
+// element only (the hardware takes unaligned vectors).
 template <typename S, int V> struct NrVec { typedef S T __attribute__((ext_vector_type(V), aligned(sizeof(S)))); };
 
-template <typename S, int V> __device__ __forceinline__ typename NrVec<S, V>::T nr_raw(const void *q, size_t base, unsigned at, int cnt)
+template <bool ODD, int V> __device__ __forceinline__ bool nr_has(int cnt, int e) { return ODD ? e < cnt : cnt > 0; }
+
+template <typename S, int V, bool ODD> __device__ __forceinline__ typename NrVec<S, V>::T nr_raw(const void *q, size_t base, unsigned at, int cnt)
 {
     typedef typename NrVec<S, V>::T SV;
     const S *p = (const S *)q + base + at;
-    if (cnt >= V) return *(const SV *)p;
     SV v;
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = e < cnt ? p[e] : (S)0.f;
+    for (int e = 0; e < V; ++e) v[e] = (S)0.f;
+    if (cnt <= 0) return v;         // (lanes without channels: one branch, nothing else)
+    if (!ODD || cnt >= V) return *(const SV *)p;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (e < cnt) v[e] = p[e];
     return v;
 }
 
-template <typename S, int V> __device__ __forceinline__ void nr_load(float *f, const void *q, size_t base, unsigned at, int cnt)
+template <typename S, int V, bool ODD> __device__ __forceinline__ void nr_load(float *f, const void *q, size_t base, unsigned at, int cnt)
 {
-    const typename NrVec<S, V>::T v = nr_raw<S, V>(q, base, at, cnt);
+    const typename NrVec<S, V>::T v = nr_raw<S, V, ODD>(q, base, at, cnt);
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = (float)v[e];
 }
 
-template <typename S, int V> __device__ __forceinline__ void nr_store(void *q, size_t base, unsigned at, int cnt, const float *f)
+template <typename S, int V, bool ODD> __device__ __forceinline__ void nr_store(void *q, size_t base, unsigned at, int cnt, const float *f)
 {
-    typedef S SV __attribute__((ext_vector_type(V), aligned(sizeof(S))));
+    typedef typename NrVec<S, V>::T SV;
+    if (cnt <= 0) return;
     S *p = (S *)q + base + at;
-    if (cnt >= V) {
-        SV v;
+    SV v;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = (S)f[e];
-        *(SV *)p = v;
-    } else
+    for (int e = 0; e < V; ++e) v[e] = (S)f[e];
+    if (!ODD || cnt >= V) *(SV *)p = v;
+    else {              // the end of a row in pieces of 4, 2 and 1
+        if constexpr (V == 8)
+            if (cnt & 4) {
+                *(typename NrVec<S, 4>::T *)p = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+                p += 4;
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e < cnt) p[e] = (S)f[e];
+                for (int e = 0; e < 4; ++e) v[e] = v[e + 4];
+            }
+        if (cnt & 2) {
+            *(typename NrVec<S, 2>::T *)p = __builtin_shufflevector(v, v, 0, 1);
+            p += 2;
+            v[0] = v[2];
+        }
+        if (cnt & 1) *p = v[0];
+    }
 }
 
 // per-channel parameters; `none` where the pointer is NULL
-template <typename S, int V> __device__ __forceinline__ void nr_param(float *f, const void *p, int pf32, size_t base, unsigned at, int cnt, float none)
+template <typename S, int V, bool ODD> __device__ __forceinline__ void nr_param(float *f, const void *p, int pf32, size_t base, unsigned at, int cnt, float none)
 {
     if (!p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] = none;
     } else if (pf32) {
         if constexpr (V == 8) {
-            nr_load<float, 4>(f, p, base, at, cnt);
-            nr_load<float, 4>(f + 4, p, base, at + 4, cnt - 4);
+            nr_load<float, 4, ODD>(f, p, base, at, cnt);
+            nr_load<float, 4, ODD>(f + 4, p, base, at + 4, ODD ? cnt - 4 : cnt);
         } else
-            nr_load<float, V>(f, p, base, at, cnt);
+            nr_load<float, V, ODD>(f, p, base, at, cnt);
     } else
-        nr_load<S, V>(f, p, base, at, cnt);
+        nr_load<S, V, ODD>(f, p, base, at, cnt);
 }
 
 // one row of a tensor as a lane holds it before its turn: NV vectors as they come from memory (requested a row ahead, so that the latency of
-// memory lies behind the row in hand).  LAST: the last vector of a row is read as the row's last V elements and moved down at its turn by
+// memory lies behind the row in hand).  ODD: the last vector of a row is read as the row's last V elements and moved down at its turn by
 // those that belong to the vector before -- one load like all others; element by element its 16-bit pieces are put together as they arrive,
 // in front of everything behind them
-template <typename S, int V, int NV, bool LAST> struct NrRow {
+template <typename S, int V, int NV, bool ODD> struct NrRow {
     typename NrVec<S, V>::T v[NV];
-    static __device__ __forceinline__ bool last(unsigned col, int cnt) { return LAST && cnt > 0 && cnt < V && (int)col + cnt >= V; }
+    static __device__ __forceinline__ bool last(unsigned col, int cnt) { return ODD && cnt > 0 && cnt < V && (int)col + cnt >= V; }
     __device__ __forceinline__ void ask(const void *q, size_t base, const unsigned *col, const int *cnt, bool live)
     {
 #pragma unroll
@@ -193,7 +210,7 @@ template <typename S, int V, int NV, bool LAST> struct NrRow {
                 for (int e = 0; e < V; ++e) v[i][e] = (S)0.f;
             else {
                 const bool l = last(col[i], cnt[i]);
-                v[i] = nr_raw<S, V>(q, base, l ? col[i] + cnt[i] - V : col[i], l ? V : cnt[i]);
+                v[i] = nr_raw<S, V, ODD>(q, base, l ? col[i] + cnt[i] - V : col[i], l ? V : cnt[i]);
             }
         }
     }
@@ -207,16 +224,16 @@ template <typename S, int V, int NV, bool LAST> struct NrRow {
 };
 
 // a parameter's channels of this lane, in registers for all its rows
-template <typename S, int V, int NV> __device__ __forceinline__ void nr_params(float *f, const void *p, int pf32, size_t base, const unsigned *col, const int *cnt, float none)
+template <typename S, int V, int NV, bool ODD> __device__ __forceinline__ void nr_params(float *f, const void *p, int pf32, size_t base, const unsigned *col, const int *cnt, float none)
 {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) nr_param<S, V>(f + i * V, p, pf32, base, col[i], cnt[i], none);
+    for (int i = 0; i < NV; ++i) nr_param<S, V, ODD>(f + i * V, p, pf32, base, col[i], cnt[i], none);
 }
 
 // x[E] -> normalised in place (0 behind the row's end); mean and 1 / deviation returned.  E = NV vectors of V.  Variances are sums of squared
 // distances from the mean.  Of the row where a wave or less holds it; where waves share it, each takes the distances from its own mean, and
 // sum (x - mean)^2 = sum over waves of [sum (x - mean_w)^2 + n_w (mean_w - mean)^2]: one exchange instead of two
-template <int V, int NV, int WPR, int NW>
+template <int V, int NV, bool ODD, int WPR, int NW>
 __device__ __forceinline__ void nr_normalise(float *x, int kind, const int *cnt, float inv_c, float eps, float own_inv_n, NrSum<WPR, NW> &sum, float &mean, float &rstd)
 {
     float q = 0.f, none = 0.f;
@@ -230,7 +247,7 @@ __device__ __forceinline__ void nr_normalise(float *x, int kind, const int *cnt,
         if constexpr (WPR > 1) {
 #pragma unroll
             for (int i = 0; i < NV * V; ++i) {
-                const float d = i % V < cnt[i / V] ? x[i] - mean : 0.f;
+                const float d = nr_has<ODD, V>(cnt[i / V], i % V) ? x[i] - mean : 0.f;
                 q += d * d;
             }
             const float2 t = sum.exchange(s, nr_wave_sum(q, sum.g_log));
@@ -239,7 +256,7 @@ __device__ __forceinline__ void nr_normalise(float *x, int kind, const int *cnt,
             q = nr_wave_sum(t.y + sum.n * d * d, sum.LOG);
         }
 #pragma unroll
-        for (int i = 0; i < NV * V; ++i) x[i] = i % V < cnt[i / V] ? x[i] - mean : 0.f;
+        for (int i = 0; i < NV * V; ++i) x[i] = nr_has<ODD, V>(cnt[i / V], i % V) ? x[i] - mean : 0.f;
     }
     if (WPR == 1 || kind != NORM_LAYER) {
 #pragma unroll
@@ -275,11 +292,11 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
     const bool outer = a.y != nullptr && a.out_kind != NORM_NONE, inner = a.in_kind != NORM_NONE;
     float wo[E], bo[E], gate[E], wi[E], bi[E];
     if constexpr (KEEP) {
-        nr_params<S, V, NV>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
-        nr_params<S, V, NV>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
-        nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
-        nr_params<S, V, NV>(bi, a.bi, a.pf32, 0, col, cnt, 0.f);
-        if (!a.rows_per_gate) nr_params<S, V, NV>(gate, a.gate, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV, ODD>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV, ODD>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+        nr_params<S, V, NV, ODD>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV, ODD>(bi, a.bi, a.pf32, 0, col, cnt, 0.f);
+        if (!a.rows_per_gate) nr_params<S, V, NV, ODD>(gate, a.gate, a.pf32, 0, col, cnt, 1.f);
     }
     const long long hop = (long long)gridDim.x * RPB;
     NrRow<S, V, NV, ODD> ry, rh;
@@ -308,35 +325,35 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
             rh.ask(a.h, (size_t)next * a.ldh, col, cnt, next < a.M);
         }
         if (a.y) {
-            if (!KEEP || a.rows_per_gate) nr_params<S, V, NV>(gate, live ? a.gate : nullptr, a.pf32, live && a.rows_per_gate ? (size_t)(row / a.rows_per_gate) * a.C : 0, col, cnt, 1.f);
+            if (!KEEP || a.rows_per_gate) nr_params<S, V, NV, ODD>(gate, live ? a.gate : nullptr, a.pf32, live && a.rows_per_gate ? (size_t)(row / a.rows_per_gate) * a.C : 0, col, cnt, 1.f);
             if (outer) {
-                nr_normalise<V, NV, WPR, NW>(x, a.out_kind, cnt, inv_c, a.eps, own_inv_n, sum, mean_y, rstd_y);
+                nr_normalise<V, NV, ODD>(x, a.out_kind, cnt, inv_c, a.eps, own_inv_n, sum, mean_y, rstd_y);
                 if constexpr (!KEEP) {
-                    nr_params<S, V, NV>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
-                    nr_params<S, V, NV>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+                    nr_params<S, V, NV, ODD>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+                    nr_params<S, V, NV, ODD>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
                 }
 #pragma unroll
                 for (int i = 0; i < E; ++i) x[i] = x[i] * wo[i] + bo[i];
             }
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = i % V < cnt[i / V] ? a.alpha * h[i] + gate[i] * x[i] : 0.f;
+            for (int i = 0; i < E; ++i) x[i] = nr_has<ODD, V>(cnt[i / V], i % V) ? a.alpha * h[i] + gate[i] * x[i] : 0.f;
             if (live)
 #pragma unroll
-                for (int i = 0; i < NV; ++i) nr_store<S, V>(a.ho, (size_t)row * a.C, col[i], cnt[i], x + i * V);
+                for (int i = 0; i < NV; ++i) nr_store<S, V, ODD>(a.ho, (size_t)row * a.C, col[i], cnt[i], x + i * V);
         } else
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] = h[i];
         if (inner) {
-            nr_normalise<V, NV, WPR, NW>(x, a.in_kind, cnt, inv_c, a.eps, own_inv_n, sum, mean_h, rstd_h);
+            nr_normalise<V, NV, ODD>(x, a.in_kind, cnt, inv_c, a.eps, own_inv_n, sum, mean_h, rstd_h);
             if constexpr (!KEEP) {
-                nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
-                nr_params<S, V, NV>(bi, a.bi, a.pf32, 0, col, cnt, 0.f);
+                nr_params<S, V, NV, ODD>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+                nr_params<S, V, NV, ODD>(bi, a.bi, a.pf32, 0, col, cnt, 0.f);
             }
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] = x[i] * wi[i] + bi[i];
             if (live)
 #pragma unroll
-                for (int i = 0; i < NV; ++i) nr_store<S, V>(a.u, (size_t)row * a.C, col[i], cnt[i], x + i * V);
+                for (int i = 0; i < NV; ++i) nr_store<S, V, ODD>(a.u, (size_t)row * a.C, col[i], cnt[i], x + i * V);
         }
         if (a.stats && live && lr == 0) *(float4 *)(a.stats + 4 * row) = float4{mean_y, rstd_y, mean_h, rstd_h};
         row = next;
@@ -345,7 +362,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(const Nor
 
 // the five column sums of a workgroup: lanes of a wave that hold the same channels of different rows add up by exchange, the waves' sums meet
 // in the LDS in the order of the waves
-template <int V, int NV, int WPR, int NW> __device__ __forceinline__ void nr_put_sums(float *lds, float *dst, float *acc, const unsigned *col, const int *cnt, int wave, int lr, int g_log)
+template <int V, int NV, bool ODD, int WPR, int NW> __device__ __forceinline__ void nr_put_sums(float *lds, float *dst, float *acc, const unsigned *col, const int *cnt, int wave, int lr, int g_log)
 {
     constexpr int E = V * NV, ROWS = WPR > 4 ? 1 : 4 / WPR;       // groups of waves with rows of their own
     if constexpr (WPR == 1)
@@ -369,7 +386,7 @@ template <int V, int NV, int WPR, int NW> __device__ __forceinline__ void nr_put
     }
 #pragma unroll
     for (int i = 0; i < E; ++i)
-        if (i % V < cnt[i / V]) dst[col[i / V] + i % V] = acc[i];
+        if (nr_has<ODD, V>(cnt[i / V], i % V)) dst[col[i / V] + i % V] = acc[i];
 }
 
 // (rows of more than 8192 channels, 16 per lane: the five sums of each would not fit the 128 registers of a lane; they go to k_norm_cols)
@@ -407,13 +424,13 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
     constexpr bool KEEP = WPR < 16;     // (as in k_norm_fwd)
     float wo[E], bo[E], gate[E], wi[E];
     auto outer = [&]() {
-        nr_params<S, V, NV>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
-        nr_params<S, V, NV>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
-        nr_params<S, V, NV>(gate, a.gate, a.pf32, gate_at, col, cnt, 1.f);
+        nr_params<S, V, NV, ODD>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV, ODD>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+        nr_params<S, V, NV, ODD>(gate, a.gate, a.pf32, gate_at, col, cnt, 1.f);
     };
     if constexpr (KEEP) {
         outer();
-        nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+        nr_params<S, V, NV, ODD>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
     }
 
     NrRow<S, V, NV, ODD> rgh, ry, rh, rgu;
@@ -449,17 +466,17 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
         // (rows and channels that do not exist are zeros from here on: gradients zero, normalised values forced to zero)
         if (a.out_kind != NORM_NONE)
 #pragma unroll
-            for (int i = 0; i < E; ++i) n[i] = i % V < cnt[i / V] ? (n[i] - st.x) * st.y : 0.f;
+            for (int i = 0; i < E; ++i) n[i] = nr_has<ODD, V>(cnt[i / V], i % V) ? (n[i] - st.x) * st.y : 0.f;
         if (a.in_kind != NORM_NONE) {
             float m1 = 0.f, m2 = 0.f;
             if constexpr (!KEEP) {
                 outer();
-                nr_params<S, V, NV>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+                nr_params<S, V, NV, ODD>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
             }
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 if (a.y) hn[i] = a.alpha * hn[i] + gate[i] * (n[i] * wo[i] + bo[i]);
-                hn[i] = i % V < cnt[i / V] ? (hn[i] - st.z) * st.w : 0.f;
+                hn[i] = nr_has<ODD, V>(cnt[i / V], i % V) ? (hn[i] - st.z) * st.w : 0.f;
                 if constexpr (SUMS) {
                     s_wi[i] += p[i] * hn[i];
                     s_bi[i] += p[i];
@@ -481,14 +498,14 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
                 float d[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) d[e] = a.alpha * g[i * V + e];
-                nr_store<S, V>(a.dh, out, col[i], cnt[i], d);
+                nr_store<S, V, ODD>(a.dh, out, col[i], cnt[i], d);
             }
         if (!a.y) continue;
         if constexpr (!KEEP) outer();
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            if (!(live && i % V < cnt[i / V])) g[i] = 0.f;
+            if (!(live && nr_has<ODD, V>(cnt[i / V], i % V))) g[i] = 0.f;
             const float q = g[i] * gate[i];
             if constexpr (SUMS) {
                 s_gate[i] += g[i] * (n[i] * wo[i] + bo[i]);
@@ -508,17 +525,17 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
         }
         if (a.need_dy && live)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) nr_store<S, V>(a.dy, out, col[i], cnt[i], p + i * V);
+            for (int i = 0; i < NV; ++i) nr_store<S, V, ODD>(a.dy, out, col[i], cnt[i], p + i * V);
     }
     if (!SUMS || !a.part) return;
     float *dst = a.part + (size_t)blockIdx.x * 5 * a.C;
     if (a.y) {
-        nr_put_sums<V, NV, WPR, NW>(meet, dst, s_gate, col, cnt, wave, lr, a.g_log);
-        nr_put_sums<V, NV, WPR, NW>(meet, dst + a.C, s_wo, col, cnt, wave, lr, a.g_log);
-        nr_put_sums<V, NV, WPR, NW>(meet, dst + 2 * (size_t)a.C, s_bo, col, cnt, wave, lr, a.g_log);
+        nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst, s_gate, col, cnt, wave, lr, a.g_log);
+        nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + a.C, s_wo, col, cnt, wave, lr, a.g_log);
+        nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + 2 * (size_t)a.C, s_bo, col, cnt, wave, lr, a.g_log);
     }
-    nr_put_sums<V, NV, WPR, NW>(meet, dst + 3 * (size_t)a.C, s_wi, col, cnt, wave, lr, a.g_log);
-    nr_put_sums<V, NV, WPR, NW>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, wave, lr, a.g_log);
+    nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + 3 * (size_t)a.C, s_wi, col, cnt, wave, lr, a.g_log);
+    nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, wave, lr, a.g_log);
 }
 
 // the column sums of wide rows in a second pass: with the rows' statistics and means known everything is element by element.  A lane takes V
@@ -535,10 +552,10 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_cols(const NormA
     const long long base = (long long)group * per_group;
     const int first = chunk * a.span, last = per_group - first < a.span ? per_group : first + a.span;
     float wo[V], bo[V], gate[V], wi[V], s[5 * V];
-    nr_params<S, V, 1>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
-    nr_params<S, V, 1>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
-    nr_params<S, V, 1>(gate, a.gate, a.pf32, a.rows_per_gate ? (size_t)group * a.C : 0, col, cnt, 1.f);
-    nr_params<S, V, 1>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
+    nr_params<S, V, 1, true>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
+    nr_params<S, V, 1, true>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
+    nr_params<S, V, 1, true>(gate, a.gate, a.pf32, a.rows_per_gate ? (size_t)group * a.C : 0, col, cnt, 1.f);
+    nr_params<S, V, 1, true>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
 #pragma unroll
     for (int i = 0; i < 5 * V; ++i) s[i] = 0.f;
     if (cnt[0] > 0)
@@ -618,7 +635,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_join(const NormJ
 }
 
 // ------------------------------------------------------------------------------------------------------------------ host side
-constexpr int NR_MAX_C = 16384;
+constexpr int NR_MAX_C = 16384, NR_CUS = 256;
 
 struct NormShape { int E, WPR, waves, g_log; bool odd; };      // waves: those of a row that have channels
 
@@ -639,11 +656,10 @@ template <int DT, int V, int NV> int nr_go(bool bwd, const NormArgs &a, const No
 {
 #define NR_GO(W)                                                                                       \
     if (s.WPR == W) {                                                                                  \
-        constexpr bool fwd_odd = W < 16 || (V * NV == 8 && DT != DT_F32), bwd_odd = W < 16;            \
         const int T = W > 2 ? 64 * s.waves : 256;                                                      \
-        if (bwd && bwd_odd && s.odd) k_norm_bwd<DT, V, NV, W, bwd_odd><<<grid, T, 0, st>>>(a);         \
+        if (bwd && s.odd) k_norm_bwd<DT, V, NV, W, true><<<grid, T, 0, st>>>(a);                       \
         else if (bwd) k_norm_bwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                          \
-        else if (fwd_odd && s.odd) k_norm_fwd<DT, V, NV, W, fwd_odd><<<grid, T, 0, st>>>(a);           \
+        else if (s.odd) k_norm_fwd<DT, V, NV, W, true><<<grid, T, 0, st>>>(a);                         \
         else k_norm_fwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                                   \
         return nr_status();                                                                            \
     }
@@ -703,10 +719,20 @@ NormChunks nr_split(long long M, long long rows_per_gate, int want, int rows_per
     return c;
 }
 
-// as many workgroups as run at once: three of four waves per CU for 16-bit rows of whole vectors, two for others
+// workgroups of a launch: as many as run at once, so that each asks for its parameters and its first row once.  Forward, 128 MB per tensor, bf16:
+// 16384 x 4096 111 us with two per CU, 129 with sixteen; 22369 x 3000 177 and 239; 8192 x 8192 126 with one, 160 with sixteen; 32768 x 2048 109 with
+// four, 158 with two (fp32: 195 with two, 217 with four).  Backward: 16384 x 4096 225 us with one, 261 with three (1024 x 4096 37 and 58: fewer sums
+// to join); 43690 x 1536 203 with three, 266 with two
+int nr_fill(const NormShape &s, int dtype, bool bwd)
+{
+    if (bwd) return NR_CUS * (s.waves > 4 ? 1 : s.waves == 3 ? 3 : 2);
+    if (s.waves > 4) return NR_CUS * (s.waves > 8 ? 1 : 2);
+    return NR_CUS * (dtype == DT_F32 ? (s.waves == 3 ? 3 : 2) : (s.waves == 3 ? 5 : 4));
+}
+
 NormChunks nr_rows_split(long long M, long long rows_per_gate, int dtype, const NormShape &s)
 {
-    return nr_split(M, rows_per_gate, dtype == DT_F32 || s.WPR > 4 || s.odd ? 512 : 768, nr_rows_per_block(s));
+    return nr_split(M, rows_per_gate, nr_fill(s, dtype, true), nr_rows_per_block(s));
 }
 
 inline unsigned nr_strips(int C, int dtype) { const int v = 64 * 16 / (dtype == DT_F32 ? 4 : 2); return (unsigned)((C + v - 1) / v); }
@@ -750,7 +776,8 @@ BC_EXPORT int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const voi
     const NormShape s = nr_shape(C, dtype);
     a.g_log = s.g_log;
     const long long blocks = (M + nr_rows_per_block(s) - 1) / nr_rows_per_block(s);
-    return nr_dispatch(dtype, false, a, s, (unsigned)(blocks < 4096 ? blocks : 4096), (hipStream_t)stream);
+    const int fill = nr_fill(s, dtype, false);
+    return nr_dispatch(dtype, false, a, s, (unsigned)(blocks < fill ? blocks : fill), (hipStream_t)stream);
 }
 
 BC_EXPORT long long bc_norm_residual_bwd_workspace(long long M, int C, long long rows_per_gate, int dtype)
