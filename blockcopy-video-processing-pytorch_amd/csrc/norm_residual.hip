@@ -418,9 +418,9 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
     const size_t gate_at = a.rows_per_gate ? (size_t)group * a.C : 0;
 
     constexpr bool SUMS = E == 8;
-    float s_gate[E], s_wo[E], s_bo[E], s_wi[E], s_bi[E];
+    float s_g[E], s_gn[E], s_wi[E], s_bi[E];        // sums of g and g n (a workgroup's rows share their gate: three of the five sums follow), p n', p
 #pragma unroll
-    for (int i = 0; i < E; ++i) s_gate[i] = s_wo[i] = s_bo[i] = s_wi[i] = s_bi[i] = 0.f;
+    for (int i = 0; i < E; ++i) s_g[i] = s_gn[i] = s_wi[i] = s_bi[i] = 0.f;
     constexpr bool KEEP = WPR < 16;     // (as in k_norm_fwd)
     float wo[E], bo[E], gate[E], wi[E];
     auto outer = [&]() {
@@ -506,13 +506,11 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             if (!(live && nr_has<ODD, V>(cnt[i / V], i % V))) g[i] = 0.f;
-            const float q = g[i] * gate[i];
             if constexpr (SUMS) {
-                s_gate[i] += g[i] * (n[i] * wo[i] + bo[i]);
-                s_wo[i] += q * n[i];
-                s_bo[i] += q;
+                s_g[i] += g[i];
+                s_gn[i] += g[i] * n[i];
             }
-            p[i] = q * wo[i];
+            p[i] = g[i] * gate[i] * wo[i];
             m1 += p[i] * n[i];
             m2 += p[i];
         }
@@ -530,9 +528,18 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
     if (!SUMS || !a.part) return;
     float *dst = a.part + (size_t)blockIdx.x * 5 * a.C;
     if (a.y) {
-        nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst, s_gate, col, cnt, wave, lr, a.g_log);
-        nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + a.C, s_wo, col, cnt, wave, lr, a.g_log);
-        nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + 2 * (size_t)a.C, s_bo, col, cnt, wave, lr, a.g_log);
+        if constexpr (!KEEP) outer();
+        float t[E];
+        auto put = [&](int which) { nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + which * (size_t)a.C, t, col, cnt, wave, lr, a.g_log); };
+#pragma unroll
+        for (int i = 0; i < E; ++i) t[i] = wo[i] * s_gn[i] + bo[i] * s_g[i];
+        put(0);
+#pragma unroll
+        for (int i = 0; i < E; ++i) t[i] = gate[i] * s_gn[i];
+        put(1);
+#pragma unroll
+        for (int i = 0; i < E; ++i) t[i] = gate[i] * s_g[i];
+        put(2);
     }
     nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + 3 * (size_t)a.C, s_wi, col, cnt, wave, lr, a.g_log);
     nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, wave, lr, a.g_log);
