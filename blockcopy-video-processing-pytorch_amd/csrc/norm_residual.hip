@@ -727,14 +727,15 @@ NormChunks nr_split(long long M, long long rows_per_gate, int want, int rows_per
 }
 
 // workgroups of a launch: as many as run at once, so that each asks for its parameters and its first row once.  Forward, 128 MB per tensor, bf16:
-// 16384 x 4096 111 us with two per CU, 129 with sixteen; 22369 x 3000 177 and 239; 8192 x 8192 126 with one, 160 with sixteen; 32768 x 2048 109 with
-// four, 158 with two (fp32: 195 with two, 217 with four).  Backward: 16384 x 4096 225 us with one, 261 with three (1024 x 4096 37 and 58: fewer sums
-// to join); 43690 x 1536 203 with three, 266 with two
+// 16384 x 4096 107 us with two per CU, 129 with sixteen; 22369 x 3000 129 and 239; 8192 x 8192 126 with one, 160 with sixteen; 32768 x 2048 108 with
+// four, 148 with two.  fp32 rows of whole vectors saturate memory with half as many (32768 x 2048 193 us with two, 211 with four; 65154 x 1030 349
+// with two, 230 with four).  Backward: 16384 x 4096 214 us with one, 232 with three (1024 x 4096 28 and 40: fewer sums to join); 43690 x 1536 200 with
+// three, 238 with two (fp32: 391 and 421 -- but 65154 x 1030 563 and 434)
 int nr_fill(const NormShape &s, int dtype, bool bwd)
 {
-    if (bwd) return NR_CUS * (s.waves > 4 ? 1 : s.waves == 3 ? 3 : 2);
+    if (bwd) return NR_CUS * (s.waves > 4 ? 1 : s.waves == 3 && dtype != DT_F32 ? 3 : 2);
     if (s.waves > 4) return NR_CUS * (s.waves > 8 ? 1 : 2);
-    return NR_CUS * (dtype == DT_F32 ? (s.waves == 3 ? 3 : 2) : (s.waves == 3 ? 5 : 4));
+    return NR_CUS * (dtype == DT_F32 && !s.odd ? (s.waves == 3 ? 3 : 2) : (s.waves == 3 ? 5 : 4));
 }
 
 NormChunks nr_rows_split(long long M, long long rows_per_gate, int dtype, const NormShape &s)
