@@ -313,8 +313,9 @@ __device__ __forceinline__ void lin_meet()
 // while step t is multiplied, step t + 1 travels into the other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel
 // global -> LDS without registers (a partial last step goes through registers, zero-filled); otherwise through registers, requested before
 // the products and stored behind them.
+// (steps of 64 bytes: 128 registers, so that four workgroups share a CU; with three 131072 x 256 x 512 57 us against 51, with five it spills)
 template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C>
-__global__ __launch_bounds__(64 * WM * WN) void k_lin_gemm(const LinArgs g)
+__global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const LinArgs g)
 {
     constexpr int V = LinT<DT>::V, BK = C * V, NT = 64 * WM * WN, ES = 16 / V;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
@@ -689,7 +690,8 @@ LinPlan lin_plan(int dtype, long long M, long long N, long long K)
     // 58, 66), else 128 while that, with a long sum in slices of at least 8 steps, gives every CU one (2048 x 512 x 17408: 50 us, 64: 122), else 64
     // (1024^3 11 us against 17)
     const long long t256 = lin_tiles(M, N, 256), rounds = (t256 + LIN_CUS - 1) / LIN_CUS;
-    const bool full = t256 >= LIN_CUS && 10 * t256 >= 7 * rounds * LIN_CUS;
+    // (rounds filled: 7 tenths pay from 1024 summed indexes on, 9 below: 16384 x 640 x 2560 in 2.5 rounds 92 us, 128: 81; 32768 x 768 x 768 in 1.5 67, 57)
+    const bool full = t256 >= LIN_CUS && 10 * t256 >= (K < 1024 ? 9 : 7) * rounds * LIN_CUS;
     p.edge = dtype == DT_F32 ? 64 : K > 512 && full ? 256 : t128 * (s > 1 ? s : 1) >= LIN_CUS ? 128 : 64;
     p.tm = (unsigned)((M + p.edge - 1) / p.edge);
     p.tn = (unsigned)((N + p.edge - 1) / p.edge);
@@ -748,8 +750,8 @@ template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *
     int r = BC_OK;
     if (p.edge == 64) r = direct ? lin_run<DT, 64, 64, 2, 2, AMC, BMC, true, 8>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false, 8>(g, p, st);
     else if constexpr (DT != DT_F32) {
-        // (a short sum: steps of 64 bytes halve the images, three workgroups share a CU and one's epilogue runs beside another's products:
-        //  17408 x 512 x 2048 58 us against 65; a long one: 128 bytes, half the barriers: 8192 x 768 x 4096 61 us against 67, 2048^3 26 against 32)
+        // (a short sum: steps of 64 bytes halve the images, four workgroups share a CU and one's epilogue runs beside the others' products:
+        //  131072 x 256 x 512 52 us against 63; a long one: 128 bytes, half the barriers: 8192 x 768 x 4096 61 us against 65, 2048^3 26 against 32)
         if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false, 8>(g, p, st);
         else if (p.edge == 256) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true, 8>(g, p, st);
         else if (g.K <= 512) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 4>(g, p, st);
