@@ -313,6 +313,9 @@ __device__ __forceinline__ void lin_meet()
 // while step t is multiplied, step t + 1 travels into the other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel
 // global -> LDS without registers (a partial last step goes through registers, zero-filled); otherwise through registers, requested before
 // the products and stored behind them.
+// Bound: the matrix pipe for long sums (bf16 16384 x 4096 x 8192 with gelu_tanh 884 us = 1243 TFLOP/s, a library product alone 824; its gradients'
+// shapes 1130 - 1180; fp32 17408 x 768 x 256 64 us = 107 TFLOP/s of 136: 4.25 tiles per CU take the time of 5).  Short sums: the epilogue's
+// instructions and the outputs (bf16 17408 x 512 x 2048 53 us, with gelu 61: 25 instructions per output, 40 % of the time, on the vector pipe).
 // (steps of 64 bytes: 128 registers, so that four workgroups share a CU; with three 131072 x 256 x 512 57 us against 51, with five it spills)
 template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C>
 __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const LinArgs g)
@@ -530,8 +533,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_join(const float 
 
 // Few rows (a token, a handful of regions): bound by reading the weight once.  A workgroup takes 16 columns and all rows, its waves a share of the
 // sum each (slices of 64 bytes per weight row, four at a time: 256 bytes in a row), straight from memory into the matrix instruction, four
-// slices ahead; the waves' sums meet in the LDS in their order -- one launch, no partial sums in memory (1 x 4096 x 4096 bf16: the tile kernel
-// with 8 slices and their join 11.1 us).  MB x 16 rows
+// slices ahead; the waves' sums meet in the LDS in their order -- one launch, no partial sums in memory (1 x 4096 x 4096 bf16: 8.1 us = 4.1 TB/s, the
+// tile kernel with 8 slices and their join 11.1).  MB x 16 rows
 template <int DT, int MB, int NW> __global__ __launch_bounds__(64 * NW) void k_lin_few(const LinArgs g)
 {
     constexpr int V = LinT<DT>::V, SL = 4 * V, UN = 4;          // summed indexes of a slice, slices at a time
@@ -581,7 +584,8 @@ template <int DT, int MB, int NW> __global__ __launch_bounds__(64 * NW) void k_l
     lin_epilogue<DT, 4>(g.ep, g.N, m, n, v, bias, res);
 }
 
-// dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.
+// dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.  Bound: memory, two
+// reads and a write (fp16 131072 x 512 with gelu 95 us = 4.2 TB/s; the instructions of gelu' are half of that time)
 struct DactArgs {
     const void *gy, *z;         // z NULL: no activation, dz = gy
     void *dz;                   // NULL: not stored
