@@ -11,7 +11,7 @@ DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
 
 class PlainBackend:
-    """Host logic's checker: the backend's channel operators in 64 bits with torch."""
+    """What the host logic is tested with: the backend's channel operators in 64 bits with torch."""
 
     name = "plain"
 
