@@ -13,8 +13,8 @@ bfloat16; sums, statistics, activations and everything between input and output 
 
 Both are differentiable once with respect to every tensor argument.  Gradients of a captured graph follow torch's rule for captured
 backward passes: warm up on the capturing stream, with no eager graph over the same leaves alive.  A small training step spends most of its
-time on the host: capture it, or run it under ``torch.autograd.set_multithreading_enabled(False)`` (half the time uncaptured).  No call waits for the device, and every
-result is run-to-run identical (sums are split and joined in a fixed order, no atomics)."""
+time on the host: capture it, or run it under ``torch.autograd.set_multithreading_enabled(False)`` (half the time uncaptured).  No call waits
+for the device, and every result is run-to-run identical (sums are split and joined in a fixed order, no atomics)."""
 from __future__ import annotations
 
 import torch
