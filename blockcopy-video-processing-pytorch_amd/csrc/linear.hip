@@ -679,31 +679,38 @@ struct LinPlan { int slices, kspan, edge; unsigned tm, tn; };
 
 inline int lin_bk(int dtype) { return dtype == DT_F32 ? 32 : 64; }
 inline long long lin_round(long long v, long long to) { return (v + to - 1) / to * to; }
+inline long long lin_min(long long a, long long b) { return a < b ? a : b; }
 inline long long lin_tiles(long long M, long long N, int edge) { return ((M + edge - 1) / edge) * ((N + edge - 1) / edge); }
 
 LinPlan lin_plan(int dtype, long long M, long long N, long long K)
 {
     LinPlan p;
     const int bk = lin_bk(dtype);
-    const long long steps = (K + bk - 1) / bk, t128 = lin_tiles(M, N, 128);
-    long long s = t128 >= LIN_CUS ? 1 : 2 * LIN_CUS / t128;
-    s = s < steps / 8 ? s : steps / 8;
-    // fp32: 64 (the matrix instructions take so long that a small tile's operands arrive in time: 17408 x 768 x 256 72 us against 105 with 128,
-    // 1024^3 24 against 34).  16 bits: 256 once that fills the chip's rounds and the sum is long enough to pay for an epilogue that nothing overlaps
-    // (16384 x 4096 x 8192: 845 us, 128: 970, 64: 1512; 8192 x 2048 x 8192: 225, 250, 345; 8192 x 768 x 4096: 54, 61, 76 -- but 17408 x 512 x 2048: 73,
-    // 58, 66), else 128 while that, with a long sum in slices of at least 8 steps, gives every CU one (2048 x 512 x 17408: 50 us, 64: 122), else 64
-    // (1024^3 11 us against 17)
-    const long long t256 = lin_tiles(M, N, 256), rounds = (t256 + LIN_CUS - 1) / LIN_CUS;
-    // (rounds filled: 7 tenths pay from 1024 summed indexes on, 9 below: 16384 x 640 x 2560 in 2.5 rounds 92 us, 128: 81; 32768 x 768 x 768 in 1.5 67, 57)
-    const bool full = t256 >= LIN_CUS && 10 * t256 >= (K < 1024 ? 9 : 7) * rounds * LIN_CUS;
-    p.edge = dtype == DT_F32 ? 64 : K > 512 && full ? 256 : t128 * (s > 1 ? s : 1) >= LIN_CUS ? 128 : 64;
+    const long long steps = (K + bk - 1) / bk, t64 = lin_tiles(M, N, 64), t128 = lin_tiles(M, N, 128), t256 = lin_tiles(M, N, 256);
+    long long s;
+    if (dtype == DT_F32) {
+        // 64 (the matrix instructions take so long that a small tile's operands arrive in time: 17408 x 768 x 256 72 us against 105 with 128, 1024^3
+        // 24 against 34).  Slices until every CU has a tile, of 2 steps at least (128 x 512 x 512 8 slices 8.2 us, one 12.9), or two or three, of 24
+        // steps at least (256 x 768 x 17408 16 slices 62 us, 8: 80; but 512 x 1024 x 1024 2 slices 17 us, 4: 19; 256 x 4096 x 1024 4: 28, 5: 35)
+        p.edge = 64;
+        s = lin_min(LIN_CUS / t64, steps / 2);
+        for (int per_cu = 2; per_cu <= 3; ++per_cu)
+            if (per_cu * LIN_CUS / t64 <= steps / 24) s = per_cu * LIN_CUS / t64;
+    } else {
+        // 256 once that fills the chip's rounds and the sum is long enough to pay for an epilogue that nothing overlaps
+        // (16384 x 4096 x 8192: 845 us, 128: 970, 64: 1512; 8192 x 2048 x 8192: 225, 250, 345; 8192 x 768 x 4096: 54, 61, 76 -- but 17408 x 512 x 2048: 73,
+        // 53, 66; rounds filled: 7 tenths pay from 1024 summed indexes on, 9 below: 16384 x 640 x 2560 in 2.5 rounds 92 us, 128: 81; 32768 x 768 x 768
+        // in 1.5 67, 57), else 128 while that, with a long sum in slices of at least 16 steps, gives every CU one (2048 x 512 x 17408 in 8 slices 47 us,
+        // 64: 66; 256 x 4096 x 4096 in 4: 23.2, 8: 25.3; but 512 x 4096 x 1024 in 8 of 8 steps 21 us, 64: 15.7), else 64 (1024^3 11 us against 17),
+        // in slices of at least 8 steps of a sum of more than 16 (64 x 4096 x 4096 8 slices 12.9 us, 16: 16; 100 x 1024 x 4096 one 6.7, 4: 10.3), 64
+        // slices at most (256 x 64 x 65536 64: 18.8, 128: 22.5)
+        const long long rounds = (t256 + LIN_CUS - 1) / LIN_CUS, s128 = t128 >= LIN_CUS ? 1 : lin_min(2 * LIN_CUS / t128, steps / 16);
+        const bool full = t256 >= LIN_CUS && 10 * t256 >= (K < 1024 ? 9 : 7) * rounds * LIN_CUS;
+        p.edge = K > 512 && full ? 256 : t128 * (s128 > 1 ? s128 : 1) >= LIN_CUS ? 128 : 64;
+        s = p.edge == 256 ? 1 : p.edge == 128 ? s128 : t64 >= LIN_CUS || steps <= 16 ? 1 : lin_min(lin_min(2 * LIN_CUS / t64, 64), steps / 8);
+    }
     p.tm = (unsigned)((M + p.edge - 1) / p.edge);
     p.tn = (unsigned)((N + p.edge - 1) / p.edge);
-    const long long tiles = (long long)p.tm * p.tn;
-    if (p.edge != 128) {        // (64: a slice of at least 4 steps)
-        s = tiles >= LIN_CUS ? 1 : 2 * LIN_CUS / tiles;
-        s = s < steps / 4 ? s : steps / 4;
-    }
     if (s < 1) s = 1;
     const long long per = (steps + s - 1) / s;
     p.kspan = (int)(per * bk);
