@@ -762,10 +762,14 @@ template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *
     if (p.edge == 64) r = direct ? lin_run<DT, 64, 64, 2, 2, AMC, BMC, true, 8>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false, 8>(g, p, st);
     else if constexpr (DT != DT_F32) {
         // (a short sum: steps of 64 bytes halve the images, four workgroups share a CU and one's epilogue runs beside the others' products:
-        //  131072 x 256 x 512 52 us against 63; a long one: 128 bytes, half the barriers: 8192 x 768 x 4096 61 us against 65, 2048^3 26 against 32)
+        //  131072 x 256 x 512 52 us against 63; a long one: 128 bytes, half the barriers: 8192 x 768 x 4096 61 us against 65)
         if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false, 8>(g, p, st);
         else if (p.edge == 256) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true, 8>(g, p, st);
         else if (g.K <= 512) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 4>(g, p, st);
+        // (one workgroup per CU, or up to two with a whole sum each and operands along it: eight waves hide each other's waits, 4096 x 1024 x 1024
+        //  13.5 us against 16.3, 2048^3 24.7 against 27.4, 3000 x 768 x 2304 16.6 against 18.1; else four waves, whose larger tiles read less from
+        //  the LDS, 2048 x 512 x 17408 45 against 51, the data gradient of 2048 x 4096 x 4096 60 against 66)
+        else if (p.tm * p.tn * (unsigned)p.slices <= LIN_CUS || (!AMC && !BMC && p.slices == 1 && p.tm * p.tn <= 2 * LIN_CUS)) r = lin_run<DT, 128, 128, 2, 4, AMC, BMC, true, 8>(g, p, st);
         else r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 8>(g, p, st);
     }
     if (r != BC_OK || p.slices == 1) return r;

@@ -385,6 +385,15 @@ def test_linear_large_tiles_are_exact(dt, M, K, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("M,K,N", [(2048, 1024, 2048), (2040, 1000, 2024), (3000, 768, 2304), (4000, 600, 4000), (4000, 4000, 600), (600, 4000, 4000), (4099, 33, 4101), (4099, 4101, 33),
+                                   (33, 4101, 4099), (512, 4096, 1000), (100, 1032, 4096), (16384, 136, 264)])
+def test_linear_every_tile_is_exact(dt, M, K, N):
+    """Every tile, wave and slice shape (partial tiles and steps among them) in each product it is used for."""
+    test_linear_large_tiles_are_exact(dt, M, K, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_linear_infinities_stay_in_their_rows(dt, M):
     """An infinity or NaN in a row of x reaches that row's outputs only, one in a row of w that column's; large finite pre-activations keep
