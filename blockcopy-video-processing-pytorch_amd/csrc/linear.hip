@@ -313,7 +313,7 @@ __device__ __forceinline__ void lin_meet()
 // while step t is multiplied, step t + 1 travels into the other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel
 // global -> LDS without registers (a partial last step goes through registers, zero-filled); otherwise through registers, requested before
 // the products and stored behind them.
-// Bound: the matrix pipe for long sums (bf16 16384 x 4096 x 8192 with gelu_tanh 884 us = 1243 TFLOP/s, a library product alone 824; its gradients'
+// Bound: the matrix pipe for long sums (bf16 16384 x 4096 x 8192 with gelu_tanh 890 us = 1235 TFLOP/s, a library product alone 824; its gradients'
 // shapes 1130 - 1180; fp32 17408 x 768 x 256 64 us = 107 TFLOP/s of 136: 4.25 tiles per CU take the time of 5).  Short sums: the epilogue's
 // instructions and the outputs (bf16 17408 x 512 x 2048 53 us, with gelu 61: 25 instructions per output, 40 % of the time, on the vector pipe).
 // (steps of 64 bytes: 128 registers, so that four workgroups share a CU; with three 131072 x 256 x 512 57 us against 51, with five it spills)
