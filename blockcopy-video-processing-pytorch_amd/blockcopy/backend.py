@@ -1069,8 +1069,13 @@ class HipBackend:
         assert t.is_contiguous() or t.is_contiguous(memory_format=torch.channels_last)
         return t
 
+    @staticmethod
+    def _z_dtype(act, dtype):
+        return torch.float32 if act > 1 else dtype
+
     def linear_fwd(self, x, weight, bias=None, act: int = 0, residual=None, keep_z: bool = False, out=None):
-        """(y, z): y = act(z) + residual with z = x weight^T + bias; z is handed back (x's dtype) if ``keep_z``; y is written to ``out`` if given."""
+        """(y, z): y = act(z) + residual with z = x weight^T + bias; z is handed back if ``keep_z`` (float32 for an activation with a curve, else x's
+        dtype); y is written to ``out`` if given."""
         M, K = x.shape
         N = weight.shape[0]
         dt, dev = x.dtype, x.device
@@ -1079,7 +1084,7 @@ class HipBackend:
         assert self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev) and self._rows_ok(residual, M, N, dt, dev)
         assert bias is None or (bias.shape == (N,) and bias.is_contiguous() and bias.dtype in (dt, torch.float32) and bias.device == dev)
         y = self._out(out, M, N, x)
-        z = x.new_empty((M, N)) if keep_z else None
+        z = x.new_empty((M, N), dtype=self._z_dtype(act, dt)) if keep_z else None
         need = self.lib.bc_linear_fwd_workspace(M, N, K, code)
         ws = x.new_empty(need, dtype=torch.uint8) if need else None
         self._launch("linear_fwd", self.lib.bc_linear_fwd, dev,
@@ -1096,7 +1101,7 @@ class HipBackend:
         code = _DTYPE_CODE.get(dt)
         assert gy.is_cuda and code is not None
         assert self._rows_ok(gy, M, N, dt, dev)
-        assert saved or (self._rows_ok(z, M, N, dt, dev) and self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev) and (z is None or z.is_contiguous()))
+        assert saved or (self._rows_ok(z, M, N, self._z_dtype(act, dt), dev) and self._rows_ok(x, M, K, dt, dev) and self._rows_ok(weight, N, K, dt, dev) and (z is None or z.is_contiguous()))
         dx = gy.new_empty((M, K)) if want[0] else None
         dw = gy.new_empty((N, K)) if want[1] else None
         db = gy.new_empty((N,), dtype=bias_dtype or dt) if want[2] else None

@@ -171,7 +171,8 @@ def linear_act(x, weight, bias=None, activation: str = "none", residual=None, di
 
     weight (out, in), or (out, in, 1, 1) as a 1x1 conv keeps it, in x's dtype; bias (out,) in x's dtype or float32; activation one of
     ``none relu gelu gelu_tanh silu``; residual of the result's shape.  Any number of rows (none among them), any sizes, row strides as they
-    come.  Under autograd the pre-activations are kept in x's dtype for the backward pass."""
+    come.  Under autograd the pre-activations are kept for the backward pass, in float32 for gelu, gelu_tanh and silu, and only the gradients
+    themselves are rounded to x's dtype."""
     name = "linear_act"
     act = ACTIVATIONS.get(activation)
     if act is None:

@@ -5,12 +5,14 @@
 //
 // A row is one pixel of a channels-last map (or one token), its features are the map's channels; bc_conv1x1_nhwc is the inference form of the
 // same product for packed channel counts, with per-channel affine records around it.  The three products are ONE kernel (k_lin_gemm) over
-// operands that either run along the summed index (KC) or across it (MC).  Sums, pre-activations and epilogue are fp32; z and dz are
-// rounded to the tensors' type once where they are stored.
+// operands that either run along the summed index (KC) or across it (MC).  Sums, pre-activations and epilogue are fp32.  Nothing but results
+// is rounded to the tensors' type: z is stored in fp32, and a 16-bit dz as two numbers of the type, one after the other through the same
+// product (LinParts).  With one number each, z's and dz's roundings made the gradients' error 1.45 times that of rounding the result alone.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/blockcopy_hip.h"
 
@@ -136,11 +138,20 @@ struct LinOperand {
 };
 
 struct LinEpi {
-    void *y, *z;                // z: the pre-activations in the tensors' type (NULL: not kept)
+    void *y, *z;                // z: the pre-activations (NULL: not kept), in fp32 for an activation with a curve, else in the tensors' type
     const void *bias, *res;
     long long ldr;
     int bias_f32, act;
 };
+
+// relu' asks for z's sign alone, and without an activation nothing is asked: the tensors' type will do.  Other derivatives take all of z
+__host__ __device__ constexpr bool lin_curved(int act) { return act > ACT_RELU; }
+
+// dz = gy act'(z) of a curved activation in 16 bits: hi + lo.  PRE dz = hi + what is left, lo = LO times that; the sum of products is (hi's + lo's / LO) / PRE.
+// Two numbers hold twice the type's bits of any dz: of float16 LO = 2^11 keeps what is left of small values above the subnormal numbers, PRE = 1/2 keeps
+// dz (up to 1.13 gy) below the type's end; bfloat16 has float's range and needs neither
+template <int DT> struct LinParts { static constexpr float PRE = 1.f, LO = 1.f; };
+template <> struct LinParts<DT_F16> { static constexpr float PRE = 0.5f, LO = 2048.f; };
 
 struct LinArgs {
     LinOperand a, b;            // a: the operand of the output's columns (n), b: of its rows (m)
@@ -148,6 +159,7 @@ struct LinArgs {
     int kspan;                  // summed indexes of one slice (a multiple of BK): slice s takes [s kspan, (s + 1) kspan)
     unsigned tiles_m, tiles_n;
     float *part;                // [slices][M][N] sums of the slices, or NULL: one slice, epilogue in place
+    size_t b_lo;                // bytes from b's data to its lower part (LinParts); 0: one part
     LinEpi ep;
 };
 
@@ -274,6 +286,9 @@ template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_bias(
     else lin_load<S, W>(b, (const S *)ep.bias + n, N - n);
 }
 
+// the smallest number above zero
+template <int DT> __device__ constexpr float lin_least() { return DT == DT_F16 ? 0x1p-24f : DT == DT_BF16 ? 0x1p-133f : 0x1p-149f; }
+
 template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_epilogue(const LinEpi &ep, int N, int m, int n, float *v, const float *b, const float *r)
 {
     typedef typename LinT<DT>::S S;
@@ -281,7 +296,15 @@ template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_epilo
     const size_t at = (size_t)m * N + n;
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] += b[e];
-    if (ep.z) lin_save<S, W>((S *)ep.z + at, v, cnt);
+    if (ep.z) {
+        if (DT == DT_F32 || lin_curved(ep.act)) lin_save<float, W>((float *)ep.z + at, v, cnt);
+        else {
+            float s[W];         // (a positive z that rounds to 0 stays positive: relu's derivative)
+#pragma unroll
+            for (int e = 0; e < W; ++e) s[e] = v[e] > 0.f && v[e] < lin_least<DT>() ? lin_least<DT>() : v[e];
+            lin_save<S, W>((S *)ep.z + at, s, cnt);
+        }
+    }
     lin_acts<DT, W>(v, ep.act);
     if (ep.res)
 #pragma unroll
@@ -295,11 +318,23 @@ template <int DT, int W = LinT<DT>::V> __device__ __forceinline__ void lin_epilo
 // LDS read once it sees one; the kernel waits itself (lin_arrived), and there is no register that a copy in flight could overwrite.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void lin_copy16(const void *base, unsigned off, unsigned lds)
+// N (1, 2 or 4) of them, STEP bytes apart in the LDS.  The waits are part of the block, the compiler sees none of its instructions: a buffer access
+// may come 5 states after a vector instruction wrote one of its scalar registers (a lane read, a reload), and one state after m0 was written
+template <int N, int STEP> __device__ __forceinline__ void lin_copy16(const void *base, const unsigned *off, unsigned lds)
 {
+    static_assert(N == 1 || N == 2 || N == 4, "copies of a block");
     const unsigned long long b = (unsigned long long)base;
     const i32x4 r = {(int)(unsigned)b, (int)(unsigned)(b >> 32) & 0xffff, -1, 0x00027000};
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(off), "s"(r) : "memory", "m0");
+#define LIN_NEXT(V) "\n\ts_add_u32 m0, m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 " V ", %1, 0 offen lds"
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %3, %1, 0 offen lds" : : "s"(lds), "s"(r), "i"(STEP), "v"(off[0]) : "memory", "m0", "scc");
+    else if constexpr (N == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %3, %1, 0 offen lds" LIN_NEXT("%4")
+                     : : "s"(lds), "s"(r), "i"(STEP), "v"(off[0]), "v"(off[1]) : "memory", "m0", "scc");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %3, %1, 0 offen lds" LIN_NEXT("%4") LIN_NEXT("%5") LIN_NEXT("%6")
+                     : : "s"(lds), "s"(r), "i"(STEP), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory", "m0", "scc");
+#undef LIN_NEXT
 }
 
 // everything this wave copied is in the LDS and everything it read from there in registers, then all waves meet
@@ -312,12 +347,12 @@ __device__ __forceinline__ void lin_meet()
 // one, so a lane ends up with four consecutive columns of one row.  Two LDS images of a step's operands, C vectors (16 C bytes) of every row:
 // while step t is multiplied, step t + 1 travels into the other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel
 // global -> LDS without registers (a partial last step goes through registers, zero-filled); otherwise through registers, requested before
-// the products and stored behind them.
+// the products and stored behind them.  TWO: the row operand's two parts (LinParts), the sum run over twice, the lower part first.
 // Bound: the matrix pipe for long sums (bf16 16384 x 4096 x 8192 with gelu_tanh 890 us = 1235 TFLOP/s, a library product alone 824; its gradients'
 // shapes 1130 - 1180; fp32 17408 x 768 x 256 64 us = 107 TFLOP/s of 136: 4.25 tiles per CU take the time of 5).  Short sums: the epilogue's
 // instructions and the outputs (bf16 17408 x 512 x 2048 53 us, with gelu 61: 25 instructions per output, 40 % of the time, on the vector pipe).
 // (steps of 64 bytes: 128 registers, so that four workgroups share a CU; with three 131072 x 256 x 512 57 us against 51, with five it spills)
-template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C>
+template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C, bool TWO>
 __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const LinArgs g)
 {
     constexpr int V = LinT<DT>::V, BK = C * V, NT = 64 * WM * WN, ES = 16 / V;
@@ -336,19 +371,23 @@ __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const
     const int m0 = (int)(b0 * 8 + in % rows_in_band) * BM, n0 = (int)(in / rows_in_band) * BN;
     const int kbeg = (int)slice * g.kspan, kend = g.K - kbeg < g.kspan ? g.K : kbeg + g.kspan;
 
+    LinOperand rows = g.b;      // (TWO: of the part in hand)
+
     uint4 ra[NA], rb[NB];
     auto fetch = [&](int k0) {
+        int t = tid;
+        if constexpr (TWO) asm("" : "+v"(t), "+s"(k0));      // (each part forms its own addresses: kept from part to part they cost a workgroup per CU)
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-            const int v = tid + NT * i;
+            const int v = t + NT * i;
             if constexpr (AMC) ra[i] = lin_fetch<DT, true>(g.a, g.N, kend, n0 + v % (BN / V) * V, k0 + v / (BN / V));
             else ra[i] = lin_fetch<DT, false>(g.a, g.N, kend, n0 + v / C, k0 + v % C * V);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int v = tid + NT * i;
-            if constexpr (BMC) rb[i] = lin_fetch<DT, true>(g.b, g.M, kend, m0 + v % (BM / V) * V, k0 + v / (BM / V));
-            else rb[i] = lin_fetch<DT, false>(g.b, g.M, kend, m0 + v / C, k0 + v % C * V);
+            const int v = t + NT * i;
+            if constexpr (BMC) rb[i] = lin_fetch<DT, true>(rows, g.M, kend, m0 + v % (BM / V) * V, k0 + v / (BM / V));
+            else rb[i] = lin_fetch<DT, false>(rows, g.M, kend, m0 + v / C, k0 + v % C * V);
         }
     };
     auto stage = [&](uint4 *img) {
@@ -364,6 +403,8 @@ __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const
     const char *pa = nullptr, *pb = nullptr;
     const size_t stepa = AMC ? (size_t)BK * g.a.ld * ES : 16 * C, stepb = BMC ? (size_t)BK * g.b.ld * ES : 16 * C;
     if constexpr (DIRECT) {
+        pa = (const char *)g.a.p + ((AMC ? (size_t)kbeg * g.a.ld + n0 : (size_t)n0 * g.a.ld + kbeg)) * ES;
+        pb = (const char *)g.b.p + ((BMC ? (size_t)kbeg * g.b.ld + m0 : (size_t)m0 * g.b.ld + kbeg)) * ES;
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
             const int v = lin_place<DT, AMC, BN, C>(tid + NT * i);
@@ -386,15 +427,11 @@ __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const
                 ob[i] = (unsigned)((long long)row * g.b.ld) * ES + (unsigned)(v % C) * 16;
             }
         }
-        pa = (const char *)g.a.p + ((AMC ? (size_t)kbeg * g.a.ld + n0 : (size_t)n0 * g.a.ld + kbeg)) * ES;
-        pb = (const char *)g.b.p + ((BMC ? (size_t)kbeg * g.b.ld + m0 : (size_t)m0 * g.b.ld + kbeg)) * ES;
     }
     const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lin_lds + wave * 1024;
     auto copy = [&](int img) {      // the next step's operands into image `img`
-#pragma unroll
-        for (int i = 0; i < NA; ++i) lin_copy16(pa, oa[i], lds0 + (img * IMG + NT * i) * 16);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) lin_copy16(pb, ob[i], lds0 + (img * IMG + BN * C + NT * i) * 16);
+        lin_copy16<NA, NT * 16>(pa, oa, lds0 + img * IMG * 16);
+        lin_copy16<NB, NT * 16>(pb, ob, lds0 + (img * IMG + BN * C) * 16);
         pa += stepa;
         pb += stepb;
     };
@@ -420,34 +457,57 @@ __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const
         }
     };
 
-    if constexpr (DIRECT) {
-        const int full = (kend - kbeg) / BK;
-        if (full > 0) copy(0);
-        for (int t = 0; t < full; ++t) {
-            lin_meet();
-            if (t + 1 < full) copy((t + 1) & 1);
-            multiply(lin_lds + (t & 1) * IMG);
-        }
-        if (kbeg + full * BK < kend) {
-            fetch(kbeg + full * BK);
-            stage(lin_lds + (full & 1) * IMG);      // (last read two steps ago, before the previous barrier)
+    int img = 0;        // (images in turn, also from part to part: the one that is written was last read before the previous barrier)
+    auto sum = [&]() {
+        if constexpr (DIRECT) {
+            const int full = (kend - kbeg) / BK;
+            if (full > 0) copy(img);
+            for (int t = 0; t < full; ++t) {
+                lin_meet();
+                if (t + 1 < full) copy(img ^ 1);
+                multiply(lin_lds + img * IMG);
+                img ^= 1;
+            }
+            if (kbeg + full * BK < kend) {
+                fetch(kbeg + full * BK);
+                stage(lin_lds + img * IMG);
+                __syncthreads();
+                multiply(lin_lds + img * IMG);
+                img ^= 1;
+            }
+        } else {
+            fetch(kbeg);
+            stage(lin_lds + img * IMG);
             __syncthreads();
-            multiply(lin_lds + (full & 1) * IMG);
+            for (int k0 = kbeg; k0 < kend; k0 += BK) {
+                const bool more = k0 + BK < kend;
+                if (more) fetch(k0 + BK);
+                multiply(lin_lds + img * IMG);
+                if (more) stage(lin_lds + (img ^ 1) * IMG);
+                __syncthreads();
+                img ^= 1;
+            }
         }
-    } else {
-        fetch(kbeg);
-        stage(lin_lds);
-        __syncthreads();
-        int cur = 0;
-        for (int k0 = kbeg; k0 < kend; k0 += BK) {
-            const bool more = k0 + BK < kend;
-            if (more) fetch(k0 + BK);
-            multiply(lin_lds + cur * IMG);
-            if (more) stage(lin_lds + (cur ^ 1) * IMG);
-            __syncthreads();
-            cur ^= 1;
+    };
+    if constexpr (!TWO) sum();
+    else
+#pragma nounroll
+        for (int part = 1; part >= 0; --part) {
+            const size_t lo = part ? g.b_lo : 0;
+            rows.p = (const char *)g.b.p + lo;
+            if constexpr (DIRECT) {
+                pa = (const char *)g.a.p + ((AMC ? (size_t)kbeg * g.a.ld + n0 : (size_t)n0 * g.a.ld + kbeg)) * ES;
+                pb = (const char *)rows.p + ((BMC ? (size_t)kbeg * g.b.ld + m0 : (size_t)m0 * g.b.ld + kbeg)) * ES;
+            }
+            sum();
+            if constexpr (LinParts<DT>::LO != 1.f) {
+                const float f = part ? 1.f / LinParts<DT>::LO : 1.f / LinParts<DT>::PRE;
+#pragma unroll
+                for (int i = 0; i < FN; ++i)
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) acc[i][j] *= f;
+            }
         }
-    }
 
     // the sums meet their epilogue through the LDS: a wave lays RH rows of them (16-byte vector c of row r at c ^ (r & its mask)) into its own
     // part of the images and takes them back row by row, so that every access to memory is a whole 16-byte vector
@@ -584,20 +644,21 @@ template <int DT, int MB, int NW> __global__ __launch_bounds__(64 * NW) void k_l
     lin_epilogue<DT, 4>(g.ep, g.N, m, n, v, bias, res);
 }
 
-// dz = dy * act'(z) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.  Bound: memory, two
+// dz = dy * act'(z) (CURVED, 16 bits: its two parts) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.  Bound: memory, two
 // reads and a write (fp16 131072 x 512 with gelu 95 us = 4.2 TB/s; the instructions of gelu' are half of that time)
 struct DactArgs {
     const void *gy, *z;         // z NULL: no activation, dz = gy
-    void *dz;                   // NULL: not stored
+    void *dz, *lo;              // NULL: not stored; lo: the lower part (CURVED in 16 bits)
     float *part;                // [gridDim.y][N] (one run of rows: not used, the sums go to db)
     void *db;                   // NULL: no sums asked for
     long long ldg, ldz;         // ldz: elements between the rows of dz
     int M, N, span, act, tpr_log, db_f32;
 };
 
-template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactArgs a)
+template <int DT, bool CURVED> __global__ __launch_bounds__(256) void k_lin_dact(const DactArgs a)
 {
     typedef typename LinT<DT>::S S;
+    typedef std::conditional_t<CURVED, float, S> Z;
     constexpr int W = LinT<DT>::V;
     __shared__ float red[256 * W];
     const int tpr = 1 << a.tpr_log, tid = threadIdx.x, c = tid & (tpr - 1), r = tid >> a.tpr_log, rows = 256 >> a.tpr_log;
@@ -612,12 +673,24 @@ template <int DT> __global__ __launch_bounds__(256) void k_lin_dact(const DactAr
             float d[W], z[W];
             lin_load<S, W>(d, (const S *)a.gy + (size_t)m * a.ldg + n, cnt);
             if (a.z) {
-                lin_load<S, W>(z, (const S *)a.z + (size_t)m * a.N + n, cnt);
+                lin_load<Z, W>(z, (const Z *)a.z + (size_t)m * a.N + n, cnt);
                 lin_dacts<DT, W>(d, z, a.act);
             }
-            if (a.dz) lin_save<S, W>((S *)a.dz + (size_t)m * a.ldz + n, d, cnt);
 #pragma unroll
             for (int e = 0; e < W; ++e) sum[e] += d[e];
+            if (!a.dz) continue;
+            const size_t at = (size_t)m * a.ldz + n;
+            if constexpr (CURVED && DT != DT_F32) {
+                float lo[W];
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    d[e] *= LinParts<DT>::PRE;
+                    const float hi = (float)(S)d[e];
+                    lo[e] = __builtin_isfinite(hi) ? (d[e] - hi) * LinParts<DT>::LO : 0.f;
+                }
+                lin_save<S, W>((S *)a.lo + at, lo, cnt);
+            }
+            lin_save<S, W>((S *)a.dz + at, d, cnt);
         }
     if (!a.db) return;
 #pragma unroll
@@ -729,7 +802,7 @@ inline bool lin_direct(const LinOperand &o, bool mc, int dtype)
     return (uintptr_t)o.p % 16 == 0 && o.ld % v == 0 && (!mc || o.run % v == 0) && o.ld * e * 256 < 0x7fffffffll;
 }
 
-template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C> int lin_run(LinArgs &g, const LinPlan &p, hipStream_t st)
+template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C, bool TWO> int lin_run(LinArgs &g, const LinPlan &p, hipStream_t st)
 {
     const size_t lds = (size_t)2 * (BM + BN) * C * sizeof(uint4);
     if (lds > 64 * 1024) {      // (asked for once per device)
@@ -737,16 +810,16 @@ template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIREC
         int dev = 0;
         hipError_t e = hipGetDevice(&dev);
         if (e == hipSuccess && !(asked.load() >> (dev & 63) & 1)) {
-            e = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            e = hipFuncSetAttribute((const void *)k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C, TWO>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             if (e == hipSuccess) asked.fetch_or(1ull << (dev & 63));
         }
         if (e != hipSuccess) return (int)e;
     }
-    k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C><<<p.tm * p.tn * (unsigned)p.slices, 64 * WM * WN, lds, st>>>(g);
+    k_lin_gemm<DT, BM, BN, WM, WN, AMC, BMC, DIRECT, C, TWO><<<p.tm * p.tn * (unsigned)p.slices, 64 * WM * WN, lds, st>>>(g);
     return lin_status();
 }
 
-template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *ws, hipStream_t st)
+template <int DT, bool AMC, bool BMC, bool TWO> int lin_pick(LinArgs &g, LinPlan p, void *ws, hipStream_t st)
 {
     g.part = p.slices > 1 ? (float *)ws : nullptr;
     const bool direct = lin_direct(g.a, AMC, DT) && lin_direct(g.b, BMC, DT);
@@ -759,18 +832,18 @@ template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *
     g.tiles_m = p.tm;
     g.tiles_n = p.tn;
     int r = BC_OK;
-    if (p.edge == 64) r = direct ? lin_run<DT, 64, 64, 2, 2, AMC, BMC, true, 8>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false, 8>(g, p, st);
+    if (p.edge == 64) r = direct ? lin_run<DT, 64, 64, 2, 2, AMC, BMC, true, 8, TWO>(g, p, st) : lin_run<DT, 64, 64, 2, 2, AMC, BMC, false, 8, TWO>(g, p, st);
     else if constexpr (DT != DT_F32) {
         // (a short sum: steps of 64 bytes halve the images, four workgroups share a CU and one's epilogue runs beside the others' products:
         //  131072 x 256 x 512 52 us against 63; a long one: 128 bytes, half the barriers: 8192 x 768 x 4096 61 us against 65)
-        if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false, 8>(g, p, st);
-        else if (p.edge == 256) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true, 8>(g, p, st);
-        else if (g.K <= 512) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 4>(g, p, st);
+        if (!direct) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, false, 8, TWO>(g, p, st);
+        else if (p.edge == 256) r = lin_run<DT, 256, 256, 2, 4, AMC, BMC, true, 8, TWO>(g, p, st);
+        else if (g.K <= 512) r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 4, TWO>(g, p, st);
         // (one workgroup per CU, or up to two with a whole sum each and operands along it: eight waves hide each other's waits, 4096 x 1024 x 1024
         //  13.5 us against 16.3, 2048^3 24.7 against 27.4, 3000 x 768 x 2304 16.6 against 18.1; else four waves, whose larger tiles read less from
         //  the LDS, 2048 x 512 x 17408 45 against 51, the data gradient of 2048 x 4096 x 4096 60 against 66)
-        else if (p.tm * p.tn * (unsigned)p.slices <= LIN_CUS || (!AMC && !BMC && p.slices == 1 && p.tm * p.tn <= 2 * LIN_CUS)) r = lin_run<DT, 128, 128, 2, 4, AMC, BMC, true, 8>(g, p, st);
-        else r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 8>(g, p, st);
+        else if (p.tm * p.tn * (unsigned)p.slices <= LIN_CUS || (!AMC && !BMC && p.slices == 1 && p.tm * p.tn <= 2 * LIN_CUS)) r = lin_run<DT, 128, 128, 2, 4, AMC, BMC, true, 8, TWO>(g, p, st);
+        else r = lin_run<DT, 128, 128, 2, 2, AMC, BMC, true, 8, TWO>(g, p, st);
     }
     if (r != BC_OK || p.slices == 1) return r;
     const long long units = (long long)g.M * ((g.N + LinT<DT>::V - 1) / LinT<DT>::V);
@@ -781,9 +854,15 @@ template <int DT, bool AMC, bool BMC> int lin_pick(LinArgs &g, LinPlan p, void *
 template <bool AMC, bool BMC> int lin_product(int dtype, LinArgs &g, const LinPlan &p, void *ws, hipStream_t st)
 {
     switch (dtype) {
-    case DT_F32: return lin_pick<DT_F32, AMC, BMC>(g, p, ws, st);
-    case DT_F16: return lin_pick<DT_F16, AMC, BMC>(g, p, ws, st);
-    default: return lin_pick<DT_BF16, AMC, BMC>(g, p, ws, st);
+    case DT_F32: return lin_pick<DT_F32, AMC, BMC, false>(g, p, ws, st);
+    case DT_F16:
+        if constexpr (AMC)      // (dz is the row operand of both gradients, whose other operand runs across the summed index)
+            if (g.b_lo) return lin_pick<DT_F16, AMC, BMC, true>(g, p, ws, st);
+        return lin_pick<DT_F16, AMC, BMC, false>(g, p, ws, st);
+    default:
+        if constexpr (AMC)
+            if (g.b_lo) return lin_pick<DT_BF16, AMC, BMC, true>(g, p, ws, st);
+        return lin_pick<DT_BF16, AMC, BMC, false>(g, p, ws, st);
     }
 }
 
@@ -799,6 +878,8 @@ template <int DT> int lin_few(const LinArgs &g, hipStream_t st)
 }
 
 inline bool lin_aligned(const void *p, int dtype) { return (uintptr_t)p % lin_esize(dtype) == 0; }
+inline bool lin_z_aligned(const void *z, int act, int dtype) { return (uintptr_t)z % (lin_curved(act) ? 4 : lin_esize(dtype)) == 0; }
+inline bool lin_two_parts(int act, int dtype) { return dtype != DT_F32 && lin_curved(act); }
 
 int lin_sizes(long long M, int N, int K, int dtype)
 {
@@ -857,7 +938,8 @@ template <int DT> int lin_dact_run(const DactArgs &a0, const DactPlan &p, hipStr
     DactArgs a = a0;
     a.span = p.span;
     a.tpr_log = p.tpr_log;
-    k_lin_dact<DT><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
+    if (a.z && lin_curved(a.act)) k_lin_dact<DT, true><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
+    else k_lin_dact<DT, false><<<dim3(p.gx, p.gy), 256, 0, st>>>(a);
     if (a.db && p.gy > 1) k_lin_colsum<DT><<<(a.N + 15) / 16, 256, 0, st>>>(a.db, a.db_f32, a.part, (int)p.gy, a.N);
     return lin_status();
 }
@@ -888,7 +970,7 @@ BC_EXPORT int bc_linear_fwd(void *y, void *z, const void *x, const void *w, cons
     if (act < 0 || act >= ACT_COUNT || ldx < K || ldw < K || (residual && ldr < N)) return BC_ERR_SHAPE;
     if (M == 0) return BC_OK;
     if (!y || !x || !w) return BC_ERR_NULL;
-    if (!lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(y, dtype) || !lin_aligned(z, dtype) || !lin_aligned(residual, dtype)) return BC_ERR_ALIGN;
+    if (!lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(y, dtype) || !lin_z_aligned(z, act, dtype) || !lin_aligned(residual, dtype)) return BC_ERR_ALIGN;
     if (bias && (uintptr_t)bias % (bias_f32 ? 4 : lin_esize(dtype))) return BC_ERR_ALIGN;
     const long long need = bc_linear_fwd_workspace(M, N, K, dtype);
     if (need > 0 && !workspace) return BC_ERR_NULL;
@@ -923,7 +1005,7 @@ static LinBwdSpace lin_bwd_space(long long M, int N, int K, int act, int dtype)
     const bool worth = lin_worth(M, N, K);
     s.order_n = N % v && worth;
     s.order_k = K % v && worth;
-    s.dz = act != ACT_NONE || s.order_n ? lin_pack_bytes(M, N, dtype) : 0;
+    s.dz = act != ACT_NONE || s.order_n ? lin_pack_bytes(M, N, dtype) * (lin_two_parts(act, dtype) ? 2 : 1) : 0;
     s.part = lin_round(4ll * N * lin_dact_plan(M, N, dtype).gy, 256);
     const long long x = lin_part_bytes(lin_plan(dtype, M, K, N), M, K), w = lin_part_bytes(lin_plan(dtype, N, K, M), N, K);
     s.slices = x > w ? x : w;
@@ -946,7 +1028,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
     if (act < 0 || act >= ACT_COUNT || ldg < N || (dw && ldx < K) || (dx && ldw < K)) return BC_ERR_SHAPE;
     if (M == 0) return BC_ERR_SHAPE;        // (no rows: the caller's gradients are zeros, nothing to launch)
     if (!gy || (act != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return BC_ERR_NULL;
-    if (!lin_aligned(gy, dtype) || !lin_aligned(z, dtype) || !lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(dx, dtype) || !lin_aligned(dw, dtype))
+    if (!lin_aligned(gy, dtype) || !lin_z_aligned(z, act, dtype) || !lin_aligned(x, dtype) || !lin_aligned(w, dtype) || !lin_aligned(dx, dtype) || !lin_aligned(dw, dtype))
         return BC_ERR_ALIGN;
     if (db && (uintptr_t)db % (bias_f32 ? 4 : lin_esize(dtype))) return BC_ERR_ALIGN;
     const LinBwdSpace s = lin_bwd_space(M, N, K, act, dtype);
@@ -957,6 +1039,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
     char *wsp = (char *)workspace, *pack = wsp + s.dz + s.part + s.slices;
     void *slices = wsp + s.dz + s.part;
     LinOperand dz = {gy, ldg, N};
+    const size_t lo = lin_two_parts(act, dtype) ? (size_t)lin_pack_bytes(M, N, dtype) : 0;
     const bool store = (dx || dw) && (act != ACT_NONE || s.order_n);
     if (store || db) {
         const DactPlan p = lin_dact_plan(M, N, dtype);
@@ -964,6 +1047,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
         a.gy = gy;
         a.z = act != ACT_NONE ? z : nullptr;
         a.dz = store ? wsp : nullptr;
+        a.lo = store && lo ? wsp + lo : nullptr;
         a.part = (float *)(wsp + s.dz);
         a.db = db;
         a.db_f32 = bias_f32;
@@ -981,6 +1065,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
         g.a = {w, ldw, K};
         if (s.order_k) g.a = lin_pack(g.a, N, &pack, dtype, st);
         g.b = {dz.p, dz.ld, N};
+        g.b_lo = lo;
         g.M = (int)M;
         g.N = K;
         g.K = N;
@@ -993,6 +1078,7 @@ BC_EXPORT int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const 
         g.a = {x, ldx, K};
         if (s.order_k) g.a = lin_pack(g.a, M, &pack, dtype, st);
         g.b = dz;
+        g.b_lo = lo;
         g.M = N;
         g.N = K;
         g.K = (int)M;

@@ -615,13 +615,13 @@ int bc_pn_features_nhwc(float *out, int N, int h, int w, int Cpad, const void *c
  * ------------------------------------------------------------------------------------------- */
 
 /* y[m][n] = act(z[m][n]) + residual[m][n],  z[m][n] = sum_k x[m][k] w[n][k] + bias[n].  x (M, K), w (N, K), y and residual (M, N); bias, residual and
- * z may be NULL; bias in fp32 (bias_f32) or dtype; act 0 none, 1 relu, 2 gelu (erf), 3 gelu (tanh), 4 silu.  z: the pre-activations rounded to dtype,
- * which the backward pass of an activation needs. */
+ * z may be NULL; bias in fp32 (bias_f32) or dtype; act 0 none, 1 relu, 2 gelu (erf), 3 gelu (tanh), 4 silu.  z: the pre-activations, which the
+ * backward pass of an activation needs: fp32 for act 2, 3, 4; in dtype for 0, 1 (where a positive one that rounds to zero is stored as dtype's smallest number). */
 int bc_linear_fwd(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, long long M, int N, int K, long long ldx,
                   long long ldw, long long ldr, int act, int dtype, int bias_f32, void *workspace, long long workspace_bytes, void *stream);
 long long bc_linear_fwd_workspace(long long M, int N, int K, int dtype);
 /* gradients for gy = d loss / d y (the residual's gradient is gy itself): dz = gy * act'(z), dx (M, K) = dz w, dw (N, K) = dz^T x, db (N) = column sums
- * of dz (fp32 sums, taken before dz is rounded to dtype; stored in fp32 if bias_f32).  dx, dw, db may each be NULL; z only with an activation,
+ * of dz (stored in fp32 if bias_f32); z as bc_linear_fwd stores it.  A 16-bit dz enters both products with twice dtype's bits: only results are rounded to dtype.  dx, dw, db may each be NULL; z only with an activation,
  * w only for dx, x only for dw. */
 int bc_linear_bwd(void *dx, void *dw, void *db, const void *gy, const void *z, const void *x, const void *w, long long M, int N, int K, long long ldg,
                   long long ldx, long long ldw, int act, int dtype, int bias_f32, void *workspace, long long workspace_bytes, void *stream);

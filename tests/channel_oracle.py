@@ -73,6 +73,25 @@ def linear(x, w, b, r, name, gy=None):
     return out
 
 
+def linear_gradients(x, w, b, name, gy):
+    """{name: (value, bound)} of dx, dw, db where nothing but the result is rounded to the tensors' type: z in float32, dz = dy act'(z) as two numbers
+    of the type (the second holds what the first leaves: off by half_eps^2 of dz)."""
+    he, dtype = half_eps(x.dtype), x.dtype
+    x, w, g = x.double(), w.double(), gy.double()
+    K, N, M = w.shape[1], w.shape[0], x.shape[0]
+    z = x @ w.t() + b.double()
+    z_err = (K + 2) * U * (x.abs() @ w.abs().t() + b.double().abs())
+    d = act(z, name)[1]
+    # (the derivative's own evaluation: at most 32 U, as in linear())
+    e = g.abs() * (CURVE[name] * z_err + 32 * U)
+    dz = g * d
+    out = {"db": (dz.sum(0), e.sum(0) + (M + 1) * U * (dz.abs() + e).sum(0))}
+    e = e + he * he * (dz.abs() + e) + 2.0 ** -34 * he
+    out["dx"] = (dz @ w, e @ w.abs() + 2 * N * U * ((dz.abs() + e) @ w.abs()))
+    out["dw"] = (dz.t() @ x, e.t() @ x.abs() + 2 * M * U * ((dz.abs() + e).t() @ x.abs()))
+    return {k: (v, rounded(v, err, b.dtype if k == "db" else dtype)) for k, (v, err) in out.items()}
+
+
 def normed(x, kind, w, b, eps):
     if kind == "none":
         return x

@@ -1,0 +1,93 @@
+"""linear_act and norm_residual where their roundings, ranges and resources end."""
+import itertools
+
+import pytest
+import torch
+
+import channel_oracle as CO
+from test_channel_ops import DT, _close, _norm_case, _rand, plain_backend  # noqa: F401  (a fixture)
+
+SMOOTH = ("gelu", "gelu_tanh", "silu")
+
+
+# ------------------------------------------------------------------------------------------------ gradients in 16 bits
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("name", SMOOTH)
+@pytest.mark.parametrize("M,K,N,size", [(130, 96, 72, 1.0), (513, 264, 200, 1.0), (1, 515, 1001, 1.0), (2049, 19, 130, 1.0), (33, 1000, 7, 1.0), (300, 512, 512, 2.0 ** -13),
+                                        (1100, 1003, 1001, 1.0), (4100, 128, 1032, 2.0 ** 12)])
+def test_gradients_round_once(dt, name, M, K, N, size):
+    """Pre-activations and dz = dy act'(z) keep their bits until the gradient itself is rounded (``size``: of dy -- small ones lie among float16's
+    subnormal numbers, large ones near its end)."""
+    import blockcopy
+
+    gen = torch.Generator().manual_seed(61)
+    dtype = DT[dt]
+    x, w, b = _rand(gen, M, K, dtype=dtype), _rand(gen, N, K, dtype=dtype, std=K ** -0.5), _rand(gen, N, dtype=dtype, std=0.3)
+    gy = _rand(gen, M, N, dtype=dtype, std=size)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = blockcopy.linear_act(x, w, b, activation=name)
+    want = CO.linear_gradients(x.detach(), w.detach(), b.detach(), name, gy)
+    for k, got in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, gy)):
+        v, bound = (t.cpu() for t in want[k])
+        # (a value beyond the type's largest number rounds to an infinity of its sign; at the border, within the bound, either is right)
+        over = v.abs() + bound > torch.finfo(dtype).max
+        _close(torch.where(over, v, got.double().cpu()), v, bound, (dt, M, K, N, name, k))
+        assert bool((got.double().cpu() * v.sign() >= v.abs() - bound)[over].all()), (dt, M, K, N, name, k)
+
+
+@pytest.mark.gpu
+def test_gradients_round_once_in_every_product_shape():
+    """The large tiles, slices and partial steps of both products: the share of the error that is not the result's own rounding (which alone
+    gives the ratio 1) is at most a tenth."""
+    import blockcopy
+
+    sizes = [(8192, 1032, 2056, 1.0), (4100, 4104, 72, 1.0), (72, 4104, 4104, 1.0), (600, 4000, 4000, 1.0), (16384, 136, 264, 1.0), (1500, 1002, 1004, 1.0),
+             (16384, 136, 264, 2.0 ** -18)]        # (the last: dy and dz among float16's subnormal numbers)
+    for dtype, (M, K, N, size), name in itertools.product((torch.float16, torch.bfloat16), sizes, ("gelu", "silu")):
+        gen = torch.Generator(device="cuda").manual_seed(62)
+        r = lambda *s, std=1.0: (torch.randn(s, generator=gen, device="cuda") * std).to(dtype)
+        x, w, b, gy = r(M, K).requires_grad_(True), r(N, K, std=K ** -0.5).requires_grad_(True), r(N).requires_grad_(True), r(M, N, std=size)
+        got = torch.autograd.grad(blockcopy.linear_act(x, w, b, activation=name), [x, w, b], gy)
+        d = lambda t: t.detach().double()
+        dz = d(gy) * CO.act(d(x) @ d(w).t() + d(b), name)[1]
+        for k, g, e in zip(("dx", "dw", "db"), got, (dz @ d(w), dz.t() @ d(x), dz.sum(0))):
+            own = float((e.to(dtype).double() - e).norm())
+            assert float((g.double() - e).norm()) <= 1.1 * own, (dtype, M, K, N, name, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+def test_relu_passes_what_is_above_zero(dt):
+    """A pre-activation above zero that is too small for the tensors' type still passes its gradient; one below or at zero none."""
+    import blockcopy
+
+    tiny = 2.0 ** -14 if dt == "f16" else 2.0 ** -40
+    x = torch.tensor([[tiny], [-tiny], [0.0]], dtype=DT[dt], device="cuda").requires_grad_(True)
+    w = torch.full((9, 1), tiny, dtype=DT[dt], device="cuda").requires_grad_(True)
+    (gx,) = torch.autograd.grad(blockcopy.linear_act(x, w, activation="relu"), [x], torch.ones(3, 9, dtype=DT[dt], device="cuda"))
+    assert torch.equal(gx, torch.tensor([[9 * tiny], [0.0], [0.0]], dtype=DT[dt], device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+def test_infinite_gradients_keep_their_sign(dt):
+    """An infinity or NaN in dy reaches its own row of dx and its own column's row of dw, as such."""
+    import blockcopy
+
+    gen = torch.Generator().manual_seed(63)
+    x, w = _rand(gen, 40, 24, dtype=DT[dt]), _rand(gen, 16, 24, dtype=DT[dt]).abs() + 0.5
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    gy = _rand(gen, 40, 16, dtype=DT[dt])
+    run = lambda g: torch.autograd.grad(blockcopy.linear_act(x, w, activation="silu"), [x, w], g)
+    clean = run(gy)
+    gy = gy.clone()
+    with torch.no_grad():
+        z = x.double() @ w.double().t()
+    gy[3, 5], gy[9, 7] = float("inf"), float("nan")
+    dx, dw = run(gy)
+    sign = CO.act(z[3, 5], "silu")[1].sign()
+    assert bool((dx[3] == float("inf") * sign).all()) and bool(dx[9].isnan().all())
+    keep, cols = [i for i in range(40) if i not in (3, 9)], [i for i in range(16) if i not in (5, 7)]
+    assert torch.equal(dx[keep], clean[0][keep]) and torch.equal(dw[cols], clean[1][cols])
+    assert bool((dw[5] == float("inf") * sign * x[3].sign()).all()) and bool(dw[7].isnan().all())
