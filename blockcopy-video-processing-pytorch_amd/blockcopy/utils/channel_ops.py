@@ -11,13 +11,14 @@ are independent of each other, so no halo, no transfer and no cache is involved,
 combined (in a frame sized for a ceiling of tiles every row is computed, the surplus ones out of whatever they hold).  float32, float16 and
 bfloat16; sums, statistics, activations and everything between input and output in float32.  GPU tensors only.
 
-Both are differentiable once with respect to every tensor argument.  Gradients of a captured graph follow torch's rule for captured
+Both are differentiable once with respect to every tensor argument, backward (a forward-mode tangent is refused).  Gradients of a captured graph follow torch's rule for captured
 backward passes: warm up on the capturing stream, with no eager graph over the same leaves alive.  A small training step spends most of its
 time on the host: capture it, or run it under ``torch.autograd.set_multithreading_enabled(False)`` (half the time uncaptured).  No call waits
 for the device, and every result is run-to-run identical (sums are split and joined in a fixed order, no atomics)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from blockcopy.backend import BlockCopyBackendError, get_backend
@@ -121,6 +122,20 @@ def _wrapped(out, wrapper):
     return out if out is None or wrapper is None else TensorWrapper._wrap_like(out, wrapper, wrapper.is_blocks)
 
 
+def _watched(*tensors):
+    """Whether the call has to go through autograd: for a backward pass, or because an argument carries a forward-mode tangent (which autograd
+    refuses there: there is no forward-mode derivative, and a result without a tangent would say that it is zero)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
+
+
 def _first_order(fn):
     """``once_differentiable`` where a second derivative could be asked for at all (create_graph), else the function itself: its guard costs as
     much host time as a small product's launch."""
@@ -193,7 +208,7 @@ def linear_act(x, weight, bias=None, activation: str = "none", residual=None, di
         shape[dim] = weight.shape[0]
         _matching(name, residual, torch.Size(shape), x, "residual")
     be = _backend(x)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
+    if _watched(x, weight, bias, residual):
         y = _LinearAct.apply(x, weight, bias, residual, act, dim, be)
     else:
         y = _linear_rows(be, x, weight, bias, residual, act, dim, False)[0]
@@ -293,10 +308,9 @@ def norm_residual(h, y=None, *, out_norm: str = "none", out_weight=None, out_bia
         gate, rows_per_gate = _gate(name, gate, h, C, dim, wrapper is not None and wrapper.is_blocks)
     params = (_vector(name, out_weight, C, h, "out_weight"), _vector(name, out_bias, C, h, "out_bias"), gate, _vector(name, in_weight, C, h, "in_weight"),
               _vector(name, in_bias, C, h, "in_bias"))
-    kind, grad = None, h.requires_grad or (y is not None and y.requires_grad)
+    kind = None
     for p in params:
         if p is not None:
-            grad = grad or p.requires_grad
             if kind is None:
                 kind = p.dtype
             elif p.dtype != kind:
@@ -305,7 +319,7 @@ def norm_residual(h, y=None, *, out_norm: str = "none", out_weight=None, out_bia
         params = tuple(None if p is None else p.float() for p in params)
     be = _backend(h)
     kinds = (out_kind, in_kind, scale, eps, rows_per_gate)
-    if grad and torch.is_grad_enabled():
+    if _watched(h, y, *params):
         out = _NormResidual.apply(h, y, *params, kinds, dim, be)
         ho, u = out if isinstance(out, tuple) else ((out, None) if y is not None else (None, out))
     else:

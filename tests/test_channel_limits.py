@@ -91,3 +91,39 @@ def test_infinite_gradients_keep_their_sign(dt):
     keep, cols = [i for i in range(40) if i not in (3, 9)], [i for i in range(16) if i not in (5, 7)]
     assert torch.equal(dx[keep], clean[0][keep]) and torch.equal(dw[cols], clean[1][cols])
     assert bool((dw[5] == float("inf") * sign * x[3].sign()).all()) and bool(dw[7].isnan().all())
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused_by_linear_act(plain_backend, which, grad):  # noqa: F811
+    """There is no forward-mode derivative: a dual argument raises, whichever it is, instead of losing its tangent."""
+    import blockcopy
+    import torch.autograd.forward_ad as fw
+
+    args = [torch.randn(3, 4), torch.randn(5, 4), torch.randn(5), torch.randn(3, 5)]
+    call = lambda a: blockcopy.linear_act(a[0], a[1], a[2], activation="silu", residual=a[3])
+    with torch.set_grad_enabled(grad):
+        with fw.dual_level():
+            assert torch.equal(call(args), call(args))       # (no tangent: as ever)
+            args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call(args)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            plain = [fw.unpack_dual(a).primal if isinstance(a, torch.Tensor) else a for a in args]
+            torch.func.jvp(lambda t: call([t if i == which else p for i, p in enumerate(plain)]), (plain[which],), (torch.ones_like(plain[which]),))
+
+
+@pytest.mark.parametrize("which", range(7))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused_by_norm_residual(plain_backend, which, grad):  # noqa: F811
+    import blockcopy
+    import torch.autograd.forward_ad as fw
+
+    args = [torch.randn(3, 4), torch.randn(3, 4), *(torch.randn(4) for _ in range(5))]
+    call = lambda a: blockcopy.norm_residual(a[0], a[1], out_norm="rms", out_weight=a[2], out_bias=a[3], gate=a[4], in_norm="layer", in_weight=a[5], in_bias=a[6])
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        call(args)
+        args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call(args)
