@@ -8,7 +8,7 @@ API: an addition).
 Both work on rows of features: the last axis of a tensor (``dim=-1``, tokens), or axis 1 of a (N, C, H, W) map (``dim=1``, pixels), for which
 channels-last memory is the free layout.  A packed or dense ``TensorWrapper`` is always read along axis 1 and gives a ``TensorWrapper``: rows
 are independent of each other, so no halo, no transfer and no cache is involved, and skipped tiles keep their values when the result is
-combined (in a frame sized for a ceiling of tiles every row is computed, the surplus ones out of whatever they hold).  float32, float16 and
+combined (in a frame sized for a ceiling of tiles every row is computed, the surplus ones out of whatever they hold, and gradients of parameters are refused).  float32, float16 and
 bfloat16; sums, statistics, activations and everything between input and output in float32.  GPU tensors only.
 
 Both are differentiable once with respect to every tensor argument, backward (a forward-mode tangent is refused).  Gradients of a captured graph follow torch's rule for captured
@@ -118,6 +118,16 @@ def _argument(x, dim, name):
     return x, x.shape[dim], wrapper, dim
 
 
+def _surplus(wrapper):
+    """Whether rows behind the executed tiles are there (a frame sized for a ceiling of tiles)."""
+    return wrapper is not None and wrapper._dyn() is not None
+
+
+def _refuse_sums(surplus, want, name):
+    if surplus and any(want):
+        raise NotImplementedError(f"{name}: gradients of parameters are sums over the executed tiles' rows, whose count only the device knows in this frame (block_graph=2)")
+
+
 def _wrapped(out, wrapper):
     return out if out is None or wrapper is None else TensorWrapper._wrap_like(out, wrapper, wrapper.is_blocks)
 
@@ -161,24 +171,25 @@ def _linear_rows(be, x, weight, bias, residual, act, dim, keep_z):
 class _LinearAct(torch.autograd.Function):
     # (one node from argument to result: axis order, rows and their way back are inside)
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, dim, be):
+    def forward(ctx, x, weight, bias, residual, act, dim, be, surplus):
         want = ctx.needs_input_grad
         y, z, xr, wr = _linear_rows(be, x, weight, bias, residual, act, dim, act != 0 and (want[0] or want[1] or want[2]))
         ctx.save_for_backward(xr if want[1] else None, wr if want[0] else None, z)
-        ctx.meta = act, dim, be, x.shape, weight.shape, None if bias is None else bias.dtype
+        ctx.meta = act, dim, be, x.shape, weight.shape, None if bias is None else bias.dtype, surplus
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, gy):
         xr, wr, z = ctx.saved_tensors
-        act, dim, be, x_shape, w_shape, bias_dtype = ctx.meta
+        act, dim, be, x_shape, w_shape, bias_dtype, surplus = ctx.meta
         want = ctx.needs_input_grad
+        _refuse_sums(surplus, want[1:3], "linear_act")
         dx = dw = db = None
         if want[0] or want[1] or want[2]:
             dx, dw, db = be.linear_bwd(_rows(_features(gy, dim)), z, xr, wr, act, want, bias_dtype, saved=True)
             dx, dw = _back(dx, x_shape, dim), None if dw is None else dw.view(w_shape)
-        return dx, dw, db, gy if want[3] else None, None, None, None
+        return dx, dw, db, gy if want[3] else None, None, None, None, None
 
 
 def linear_act(x, weight, bias=None, activation: str = "none", residual=None, dim: int = -1):
@@ -209,7 +220,7 @@ def linear_act(x, weight, bias=None, activation: str = "none", residual=None, di
         _matching(name, residual, torch.Size(shape), x, "residual")
     be = _backend(x)
     if _watched(x, weight, bias, residual):
-        y = _LinearAct.apply(x, weight, bias, residual, act, dim, be)
+        y = _LinearAct.apply(x, weight, bias, residual, act, dim, be, _surplus(wrapper))
     else:
         y = _linear_rows(be, x, weight, bias, residual, act, dim, False)[0]
     return _wrapped(y, wrapper)
@@ -228,23 +239,24 @@ def _norm_rows(be, h, y, params, kinds, dim, keep_stats):
 
 class _NormResidual(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, y, out_weight, out_bias, gate, in_weight, in_bias, kinds, dim, be):
+    def forward(ctx, h, y, out_weight, out_bias, gate, in_weight, in_bias, kinds, dim, be, surplus):
         ctx.set_materialize_grads(False)
         ho, u, stats, hr, yr = _norm_rows(be, h, y, (out_weight, out_bias, gate, in_weight, in_bias), kinds, dim, True)
         ctx.save_for_backward(hr, yr, out_weight, out_bias, gate, in_weight, in_bias, stats)
-        ctx.meta = kinds, dim, be, h.shape
+        ctx.meta = kinds, dim, be, h.shape, surplus
         return (ho, u) if ho is not None and u is not None else (ho if ho is not None else u)
 
     @staticmethod
     @_first_order
     def backward(ctx, *grads):
         h, y, out_weight, out_bias, gate, in_weight, in_bias, stats = ctx.saved_tensors
-        (out_kind, in_kind, scale, _, rows_per_gate), dim, be, shape = ctx.meta
+        (out_kind, in_kind, scale, _, rows_per_gate), dim, be, shape, surplus = ctx.meta
         gh = grads[0] if y is not None else None
         gu = grads[-1] if in_kind else None
         want = ctx.needs_input_grad[:7]
         if gh is None and gu is None:
-            return (None,) * 10
+            return (None,) * 11
+        _refuse_sums(surplus, want[2:], "norm_residual")
         flat = None if gate is None else gate.view(-1)
         if h.shape[0] == 0:
             out = [torch.zeros_like(t) if w else None for t, w in zip((h, y, out_weight, out_bias, flat, in_weight, in_bias), want)]
@@ -252,7 +264,7 @@ class _NormResidual(torch.autograd.Function):
             out = be.norm_residual_bwd(None if gh is None else _rows(_features(gh, dim)), None if gu is None else _rows(_features(gu, dim)), stats, h, y, out_weight, out_bias,
                                        flat, in_weight, in_bias, out_kind, in_kind, scale, rows_per_gate, want, saved=True)
         dh, dy, dwo, dbo, dg, dwi, dbi = out
-        return (_back(dh, shape, dim), _back(dy, shape, dim), dwo, dbo, None if dg is None else dg.view(gate.shape), dwi, dbi, None, None, None)
+        return (_back(dh, shape, dim), _back(dy, shape, dim), dwo, dbo, None if dg is None else dg.view(gate.shape), dwi, dbi, None, None, None, None)
 
 
 def _gate(name, gate, h, C, dim, packed):
@@ -320,7 +332,7 @@ def norm_residual(h, y=None, *, out_norm: str = "none", out_weight=None, out_bia
     be = _backend(h)
     kinds = (out_kind, in_kind, scale, eps, rows_per_gate)
     if _watched(h, y, *params):
-        out = _NormResidual.apply(h, y, *params, kinds, dim, be)
+        out = _NormResidual.apply(h, y, *params, kinds, dim, be, _surplus(wrapper))
         ho, u = out if isinstance(out, tuple) else ((out, None) if y is not None else (None, out))
     else:
         ho, u = _norm_rows(be, h, y, params, kinds, dim, False)[:2]

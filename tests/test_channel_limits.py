@@ -127,3 +127,28 @@ def test_forward_mode_is_refused_by_norm_residual(plain_backend, which, grad):  
         args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
         with pytest.raises((RuntimeError, NotImplementedError)):
             call(args)
+
+
+def test_parameter_gradients_of_a_frame_with_surplus_tiles_are_refused(plain_backend):  # noqa: F811
+    """In a frame sized for a ceiling of tiles the rows behind the executed ones hold anything: a sum over all rows is no gradient.  The data
+    gradients, row by row, are those of the rows."""
+    import blockcopy
+
+    def frame(dyn):
+        t = blockcopy.to_tensorwrapper(torch.randn(2, 6, 8, 8).contiguous(memory_format=torch.channels_last))
+        t.process_temporal_features(None)
+        t._is_blocks = True
+        t._features.dyn = (torch.tensor([1]), 2) if dyn else None
+        return t
+
+    w, v = torch.randn(6, 6, requires_grad=True), torch.randn(6, requires_grad=True)
+    for dyn in (False, True):
+        calls = [lambda: blockcopy.linear_act(frame(dyn), w), lambda: blockcopy.linear_act(frame(dyn), w.detach(), v), lambda: blockcopy.norm_residual(frame(dyn), frame(dyn), gate=v)[0],
+                 lambda: blockcopy.norm_residual(frame(dyn), in_norm="rms", in_weight=v)[1]]
+        for call in calls:
+            out = call()._plain()
+            if dyn:
+                with pytest.raises(NotImplementedError):
+                    out.sum().backward()
+            else:
+                out.sum().backward()
