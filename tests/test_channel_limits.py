@@ -93,6 +93,27 @@ def test_infinite_gradients_keep_their_sign(dt):
     assert bool((dw[5] == float("inf") * sign * x[3].sign()).all()) and bool(dw[7].isnan().all())
 
 
+# ------------------------------------------------------------------------------------------------ activations far out
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("name", CO.ACTS)
+def test_derivatives_far_out(dt, name):
+    """act'(z) beyond the range that the exponentials cover.  One input, one weight of 1, dy = 1: the data gradient is act'(z), rounded once.  32
+    roundings of its own, (z^2 + 2 |z|) U from the exponent's roundings, and where a sigmoid or exponential lies below float32's smallest normal
+    number 2^-126 it may be 0: an error of 2^-126 times what it is multiplied by, at most (1 + |z|)^3."""
+    import blockcopy
+
+    z = torch.tensor([s * v for v in (0.5, 20.0, 40.0, 63.0, 64.0, 65.0, 80.0, 86.0, 90.0, 110.0, 127.0, 128.0, 130.0, 200.0, 1000.0, 60000.0) for s in (1, -1)], dtype=torch.float64)
+    x = z.to(DT[dt]).cuda()[:, None].requires_grad_(True)
+    w = torch.ones(1, 1, dtype=DT[dt], device="cuda")
+    (gx,) = torch.autograd.grad(blockcopy.linear_act(x, w, activation=name), [x], torch.ones(len(z), 1, dtype=DT[dt], device="cuda"))
+    z = x.detach().double().cpu()
+    d = CO.act(z, name)[1]
+    inner = {"gelu": z * z, "gelu_tanh": 1.6 * z.abs() * (1 + 0.045 * z * z)}.get(name, z.abs())
+    err = 32 * CO.U * d.abs() + 2 * inner.clamp_max(200) * CO.U * d.abs() + 2.0 ** -126 * (1 + z.abs().clamp_max(128)) ** 3 + 32 * CO.U * (z.abs() < 10)
+    _close(gx, d, CO.rounded(d, err, DT[dt]), (dt, name))
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 @pytest.mark.parametrize("which", range(4))
 @pytest.mark.parametrize("grad", [True, False])
