@@ -114,6 +114,22 @@ def test_derivatives_far_out(dt, name):
     _close(gx, d, CO.rounded(d, err, DT[dt]), (dt, name))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+def test_tails_of_gelu(dt):
+    """gelu(z) = z Phi(z) keeps its relative precision where Phi is small: Phi's own error (2^-19 in 16-bit types, 64 U in float32, besides the
+    exponent's: z^2 / 2 off by at most 4 roundings) times the value, never 1 - (1 - Phi)."""
+    import blockcopy
+
+    z = -torch.linspace(0.01, 12.9, 700, dtype=torch.float64)
+    x = z.to(DT[dt]).cuda()[:, None]
+    y = blockcopy.linear_act(x, torch.ones(1, 1, dtype=DT[dt], device="cuda"), activation="gelu")
+    z = x.double().cpu()
+    a = CO.act(z, "gelu")[0]
+    err = a.abs() * ((64 * CO.U if dt == "f32" else 2.0 ** -19) + 2 * z * z * CO.U)
+    _close(y, a, CO.rounded(a, err, DT[dt]), dt)
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 @pytest.mark.parametrize("which", range(4))
 @pytest.mark.parametrize("grad", [True, False])
