@@ -47,11 +47,13 @@ struct NormArgs {
     const void *gh, *gu;                        // gradients of h' and u (NULL: zeros)
     void *dh, *dy;
     float *part;                                // [workgroups][5][C]: column sums of gate, wo, bo, wi, bi
-    float *means;                               // [M][2]: mean(p n), mean(p) of the inner norm's backward (rows of more than 8192 channels)
+    float *means;                               // [M][2]: mean(p n), mean(p) of the inner norm's backward (column sums in a second pass)
     long long ldh, ldy, ldgh, ldgu;
     int M, C, g_log, rows_per_gate, span, chunks;
     int out_kind, in_kind, pf32, need_dh, need_dy;
     float alpha, eps;
+    void *d_gate;                               // the gate's gradient where k_norm_cols writes it itself
+    int gate_every;                             // backward: rows per gate where a workgroup's rows have several (rows_per_gate is 0 then)
 };
 
 // ---- sums over the G lanes of a row; every lane of the row gets the same bits
@@ -399,8 +401,9 @@ template <int V, int NV, bool ODD, int WPR, int NW> __device__ __forceinline__ v
 // Backward, p = du * wi, n and n' the normalised y and h':
 //   g = dh' + (p - mean(p) - n' mean(p n')) / dev'   (rms: without mean(p))     dh = scale * g     q = g * gate * wo
 //   dy = (q - mean(q) - n mean(q n)) / dev           d gate = sum g (n wo + bo)   d wo = gate sum g n   d bo = gate sum g   d wi = sum du n'   d bi = sum du
-// (rows of more than 8192 channels, 16 per lane: four sums of each would not fit the 128 registers of a lane; they go to k_norm_cols)
-template <int DT, int V, int NV, int WPR, bool ODD>
+// (rows of more than 8192 channels, 16 per lane: four sums of each would not fit the 128 registers of a lane; they go to k_norm_cols.  GATES: so do
+// those of many gates, and a row takes its own)
+template <int DT, int V, int NV, int WPR, bool ODD, bool GATES>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 || ODD ? 1 : 3) void k_norm_bwd(const NormArgs a)
 {
     typedef typename NrT<DT>::S S;
@@ -425,9 +428,9 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
     const int per_group = a.rows_per_gate ? a.rows_per_gate : a.M;
     const long long base = (long long)group * per_group;
     const int first = chunk * a.span, last = per_group - first < a.span ? per_group : first + a.span;
-    const size_t gate_at = a.rows_per_gate ? (size_t)group * a.C : 0;
+    size_t gate_at = a.rows_per_gate ? (size_t)group * a.C : 0;
 
-    constexpr bool SUMS = E == 8;
+    constexpr bool SUMS = E == 8 && !GATES;
     float s_g[E], s_gn[E], s_wi[E], s_bi[E];        // sums of g and g n (a workgroup's rows share their gate: three of the five sums follow), p n', p
 #pragma unroll
     for (int i = 0; i < E; ++i) s_g[i] = s_gn[i] = s_wi[i] = s_bi[i] = 0.f;
@@ -445,6 +448,10 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
 
     NrRow<S, V, NV, ODD> rgh, ry, rh, rgu;
     float4 rst;
+    auto own_gate = [&](int r) {        // of a row (a gate of its own, or of few rows)
+        gate_at = (size_t)((unsigned)(r < last ? r : last - 1) / (unsigned)a.gate_every) * a.C;
+        if constexpr (KEEP) nr_params<S, V, NV, ODD>(gate, a.gate, a.pf32, gate_at, col, cnt, 1.f);
+    };
     auto ask = [&](int r) {
         const bool live = r < last;
         const long long row = base + r;
@@ -458,6 +465,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
     for (int r0 = first; r0 < last; r0 += RPB) {
         const bool live = r0 + slot < last;
         const size_t out = (size_t)(base + r0 + slot) * a.C;
+        if constexpr (GATES) own_gate(r0 + slot);
         if constexpr (!KEEP) ask(r0 + slot);
         float n[E], g[E], p[E], hn[E];      // normalised y; gradient of h'; working row; normalised h'
         const float4 st = rst;
@@ -555,9 +563,10 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 |
     nr_put_sums<V, NV, ODD, WPR, NW>(meet, dst + 4 * (size_t)a.C, s_bi, col, cnt, wave, lr, a.g_log);
 }
 
-// the column sums of wide rows in a second pass: with the rows' statistics and means known everything is element by element.  A lane takes V
-// channels, a workgroup a strip of 64 V of them and a run of rows, its four waves every fourth
-template <int DT> __global__ __launch_bounds__(256) void k_norm_cols(const NormArgs a)
+// the column sums of wide rows, or of many gates, in a second pass: with the rows' statistics and means known everything is element by element.
+// A lane takes V channels, a workgroup a strip of 64 V of them and a run of rows, its four waves every fourth.  GATES: a run of gates (whole groups of
+// rows), a wave a quarter of it: a gate's gradient is complete where its rows end, the four other sums go on
+template <int DT, bool GATES> __global__ __launch_bounds__(256) void k_norm_cols(const NormArgs a)
 {
     typedef typename NrT<DT>::S S;
     constexpr int V = NrT<DT>::V;
@@ -565,47 +574,66 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_cols(const NormA
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const unsigned col[1] = {(blockIdx.x * 64 + lane) * V};
     const int cnt[1] = {a.C - (int)col[0]};
-    const int group = (int)blockIdx.y / a.chunks, chunk = (int)blockIdx.y % a.chunks, per_group = a.rows_per_gate ? a.rows_per_gate : a.M;
-    const long long base = (long long)group * per_group;
-    const int first = chunk * a.span, last = per_group - first < a.span ? per_group : first + a.span;
     float wo[V], bo[V], gate[V], wi[V], s[5 * V];
     nr_params<S, V, 1, true>(wo, a.wo, a.pf32, 0, col, cnt, 1.f);
     nr_params<S, V, 1, true>(bo, a.bo, a.pf32, 0, col, cnt, 0.f);
-    nr_params<S, V, 1, true>(gate, a.gate, a.pf32, a.rows_per_gate ? (size_t)group * a.C : 0, col, cnt, 1.f);
     nr_params<S, V, 1, true>(wi, a.wi, a.pf32, 0, col, cnt, 1.f);
 #pragma unroll
     for (int i = 0; i < 5 * V; ++i) s[i] = 0.f;
-    if (cnt[0] > 0)
-#pragma unroll 2
-        for (int r = first + wave; r < last; r += 4) {
-            const long long row = base + r;
-            const float4 st = *(const float4 *)(a.stats + 4 * row);
-            const float2 mean = a.in_kind != NORM_NONE ? *(const float2 *)(a.means + 2 * row) : float2{0.f, 0.f};
-            NrRow<S, V, 1, true> ry, rh, rgu, rgh;
-            ry.ask(a.y, (size_t)row * a.ldy, col, cnt, true);
-            rh.ask(a.in_kind != NORM_NONE ? a.h : nullptr, (size_t)row * a.ldh, col, cnt, true);
-            rgu.ask(a.gu, (size_t)row * a.ldgu, col, cnt, true);
-            rgh.ask(a.gh, (size_t)row * a.ldgh, col, cnt, true);
-            ry.settle(col, cnt);
-            rh.settle(col, cnt);
-            rgu.settle(col, cnt);
-            rgh.settle(col, cnt);
+    auto add = [&](long long row) {
+        const float4 st = *(const float4 *)(a.stats + 4 * row);
+        const float2 mean = a.in_kind != NORM_NONE ? *(const float2 *)(a.means + 2 * row) : float2{0.f, 0.f};
+        NrRow<S, V, 1, true> ry, rh, rgu, rgh;
+        ry.ask(a.y, (size_t)row * a.ldy, col, cnt, true);
+        rh.ask(a.in_kind != NORM_NONE ? a.h : nullptr, (size_t)row * a.ldh, col, cnt, true);
+        rgu.ask(a.gu, (size_t)row * a.ldgu, col, cnt, true);
+        rgh.ask(a.gh, (size_t)row * a.ldgh, col, cnt, true);
+        ry.settle(col, cnt);
+        rh.settle(col, cnt);
+        rgu.settle(col, cnt);
+        rgh.settle(col, cnt);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float n = a.out_kind != NORM_NONE ? (ry.at(e) - st.x) * st.y : ry.at(e);
-                float g = rgh.at(e);
-                if (a.in_kind != NORM_NONE) {
-                    const float h = a.y ? a.alpha * rh.at(e) + gate[e] * (n * wo[e] + bo[e]) : rh.at(e);
-                    const float hn = (h - st.z) * st.w, u = rgu.at(e);
-                    s[3 * V + e] += u * hn;
-                    s[4 * V + e] += u;
-                    g += st.w * (u * wi[e] - mean.y - hn * mean.x);
-                }
-                s[e] += g * (n * wo[e] + bo[e]);
-                s[V + e] += g * gate[e] * n;
-                s[2 * V + e] += g * gate[e];
+        for (int e = 0; e < V; ++e) {
+            const float n = a.out_kind != NORM_NONE ? (ry.at(e) - st.x) * st.y : ry.at(e);
+            float g = rgh.at(e);
+            if (a.in_kind != NORM_NONE) {
+                const float h = a.y ? a.alpha * rh.at(e) + gate[e] * (n * wo[e] + bo[e]) : rh.at(e);
+                const float hn = (h - st.z) * st.w, u = rgu.at(e);
+                s[3 * V + e] += u * hn;
+                s[4 * V + e] += u;
+                g += st.w * (u * wi[e] - mean.y - hn * mean.x);
             }
+            s[e] += g * (n * wo[e] + bo[e]);
+            s[V + e] += g * gate[e] * n;
+            s[2 * V + e] += g * gate[e];
         }
+    };
+    if constexpr (GATES) {
+        const int groups = a.M / a.gate_every, g0 = ((int)blockIdx.y * 4 + wave) * a.span;
+        const int g1 = groups - g0 < a.span ? groups : g0 + a.span;
+        if (cnt[0] > 0)
+            for (int group = g0; group < g1; ++group) {
+                const size_t at = (size_t)group * a.C;
+                nr_params<S, V, 1, true>(gate, a.gate, a.pf32, at, col, cnt, 1.f);
+                for (int r = 0; r < a.gate_every; ++r) add((long long)group * a.gate_every + r);
+                if (a.d_gate) {
+                    if (a.pf32)
+#pragma unroll
+                        for (int p = 0; p < V; p += 4) nr_store<float, 4, true>(a.d_gate, at, col[0] + p, cnt[0] - p, s + p);
+                    else nr_store<S, V, true>(a.d_gate, at, col[0], cnt[0], s);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[e] = 0.f;
+            }
+    } else {
+        const int group = (int)blockIdx.y / a.chunks, chunk = (int)blockIdx.y % a.chunks, per_group = a.rows_per_gate ? a.rows_per_gate : a.M;
+        const long long base = (long long)group * per_group;
+        const int first = chunk * a.span, last = per_group - first < a.span ? per_group : first + a.span;
+        nr_params<S, V, 1, true>(gate, a.gate, a.pf32, a.rows_per_gate ? (size_t)group * a.C : 0, col, cnt, 1.f);
+        if (cnt[0] > 0)
+#pragma unroll 2
+            for (int r = first + wave; r < last; r += 4) add(base + r);
+    }
     if (wave)
 #pragma unroll
         for (int i = 0; i < 5 * V; ++i) meet[wave - 1][i][lane] = s[i];
@@ -619,8 +647,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_cols(const NormA
     }
 }
 
-// column sums of the workgroups: 16 columns x 16 runs of workgroups per launch block, joined in a fixed order.  blockIdx.y: which of the five
-// (the gate's sums run over its own group's workgroups, blockIdx.z)
+// column sums of the workgroups: 16 columns x 16 runs of workgroups per launch block, joined in a fixed order.  blockIdx.x: which of the four that
+// run over all workgroups, behind them the gate's, each over its own group's workgroups
 struct NormJoin {
     const float *part;
     void *out[5];
@@ -631,10 +659,10 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_join(const NormJ
 {
     typedef typename NrT<DT>::S S;
     __shared__ float red[256];
-    const int which = blockIdx.y, c = (int)blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
-    if (!a.out[which] || (which > 0 && blockIdx.z > 0)) return;
+    const int which = blockIdx.x < 4 ? (int)blockIdx.x + 1 : 0, c = (int)blockIdx.y * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
+    if (!a.out[which]) return;
     const bool per_group = which == 0;
-    const int b0 = per_group ? (int)blockIdx.z * a.chunks : 0, nb = per_group ? a.chunks : a.blocks;
+    const int group = per_group ? (int)blockIdx.x - 4 : 0, b0 = group * a.chunks, nb = per_group ? a.chunks : a.blocks;
     float s = 0.f;
     if (c < a.C)
 #pragma unroll 8
@@ -645,7 +673,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_join(const NormJ
         float t = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) t += red[16 * r + threadIdx.x];
-        const size_t at = (per_group ? (size_t)blockIdx.z * a.C : 0) + c;
+        const size_t at = (size_t)group * a.C + c;
         if (a.f32) ((float *)a.out[which])[at] = t;
         else ((S *)a.out[which])[at] = (S)t;
     }
@@ -674,8 +702,9 @@ template <int DT, int V, int NV> int nr_go(bool bwd, const NormArgs &a, const No
 #define NR_GO(W)                                                                                       \
     if (s.WPR == W) {                                                                                  \
         const int T = W > 2 ? 64 * s.waves : 256;                                                      \
-        if (bwd && s.odd) k_norm_bwd<DT, V, NV, W, true><<<grid, T, 0, st>>>(a);                       \
-        else if (bwd) k_norm_bwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                          \
+        if (bwd && a.gate_every) k_norm_bwd<DT, V, NV, W, true, true><<<grid, T, 0, st>>>(a);          \
+        else if (bwd && s.odd) k_norm_bwd<DT, V, NV, W, true, false><<<grid, T, 0, st>>>(a);           \
+        else if (bwd) k_norm_bwd<DT, V, NV, W, false, false><<<grid, T, 0, st>>>(a);                   \
         else if (s.odd) k_norm_fwd<DT, V, NV, W, true><<<grid, T, 0, st>>>(a);                         \
         else k_norm_fwd<DT, V, NV, W, false><<<grid, T, 0, st>>>(a);                                   \
         return nr_status();                                                                            \
@@ -755,17 +784,39 @@ NormChunks nr_rows_split(long long M, long long rows_per_gate, int dtype, const 
 
 inline unsigned nr_strips(int C, int dtype) { const int v = 64 * 16 / (dtype == DT_F32 ? 4 : 2); return (unsigned)((C + v - 1) / v); }
 
-// the workgroups that leave column sums: those of the rows, or (wide rows) about 1024 of k_norm_cols
-NormChunks nr_sums_split(long long M, long long rows_per_gate, int C, int dtype, const NormShape &s)
+// the backward pass's plan.  A workgroup of the rows' kernel keeps the sums of one gate, and leaves five fp32 numbers per channel.  Gates of so few rows
+// that this is more than a tensor of the call holds (and more than the L2s do) take their sums in the second pass instead, a run of gates per
+// wave: backward of 65535 x 4096 bf16 with a gate per row 11 MB of workspace and 1.7 ms, sums per gate 5.4 GB and 21 ms; 65528 x 1024 with a gate per 8
+// rows 11 MB and 398 us, 168 MB and 758
+struct NormPlan {
+    NormChunks rows, sums;      // the workgroups of the rows' kernel, and those that leave column sums (GATES: span counts gates, of a wave)
+    bool second, gates;
+};
+
+NormPlan nr_plan(long long M, long long rows_per_gate, int C, int dtype, const NormShape &s)
 {
-    return s.E == 8 ? nr_rows_split(M, rows_per_gate, dtype, s) : nr_split(M, rows_per_gate, (int)(1024 / nr_strips(C, dtype)), 4);
+    NormPlan p;
+    const long long groups = rows_per_gate ? M / rows_per_gate : 1, left = 20ll * C * groups;
+    p.gates = left > (16ll << 20) && left > M * C * (dtype == DT_F32 ? 4 : 2);
+    p.second = p.gates || s.E != 8;
+    p.rows = nr_rows_split(M, p.gates ? 0 : rows_per_gate, dtype, s);
+    const int want = (int)(1024 / nr_strips(C, dtype));
+    if (p.gates) {
+        p.sums.span = (int)((groups + 4 * want - 1) / (4 * want));
+        p.sums.chunks = (int)((groups + 4ll * p.sums.span - 1) / (4ll * p.sums.span));
+        p.sums.groups = 1;
+    } else
+        p.sums = p.second ? nr_split(M, rows_per_gate, want, 4) : p.rows;
+    return p;
 }
 
-long long nr_bwd_space(long long M, int C, long long rows_per_gate, int dtype)
+// (the rows' means first: whatever the sums' size, they start on 256 bytes)
+long long nr_bwd_space(long long M, int C, const NormPlan &p) { return (p.second ? (8 * M + 255) / 256 * 256 : 0) + 20ll * C * p.sums.chunks * p.sums.groups; }
+
+template <int DT> void nr_cols(const NormArgs &a, bool gates, dim3 grid, hipStream_t st)
 {
-    const NormShape s = nr_shape(C, dtype);
-    const NormChunks c = nr_sums_split(M, rows_per_gate, C, dtype, s);
-    return 20ll * C * c.chunks * c.groups + (s.E == 8 ? 0 : 8 * M);
+    if (gates) k_norm_cols<DT, true><<<grid, 256, 0, st>>>(a);
+    else k_norm_cols<DT, false><<<grid, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -801,7 +852,7 @@ BC_EXPORT int bc_norm_residual_fwd(void *h_out, void *u, float *stats, const voi
 BC_EXPORT long long bc_norm_residual_bwd_workspace(long long M, int C, long long rows_per_gate, int dtype)
 {
     if (M < 1 || C < 1 || C > NR_MAX_C || dtype < 0 || dtype > 2 || rows_per_gate < 0 || (rows_per_gate && M % rows_per_gate)) return 0;
-    return nr_bwd_space(M, C, rows_per_gate, dtype);
+    return nr_bwd_space(M, C, nr_plan(M, rows_per_gate, C, dtype, nr_shape(C, dtype)));
 }
 
 BC_EXPORT int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void *d_out_bias, void *d_gate, void *d_in_weight, void *d_in_bias, const void *gh, const void *gu,
@@ -821,40 +872,48 @@ BC_EXPORT int bc_norm_residual_bwd(void *dh, void *dy, void *d_out_weight, void 
         if (ps[i] && (uintptr_t)ps[i] % pe) return BC_ERR_ALIGN;
     if ((uintptr_t)stats % 16) return BC_ERR_ALIGN;
     const NormShape s = nr_shape(C, dtype);
-    const NormChunks c = nr_rows_split(M, rows_per_gate, dtype, s), q = nr_sums_split(M, rows_per_gate, C, dtype, s);
+    const NormPlan p = nr_plan(M, rows_per_gate, C, dtype, s);
+    const NormChunks &c = p.rows, &q = p.sums;
     const bool sums = d_out_weight || d_out_bias || d_gate || d_in_weight || d_in_bias;
     if (sums && !workspace) return BC_ERR_NULL;
-    if (sums && workspace_bytes < nr_bwd_space(M, C, rows_per_gate, dtype)) return BC_ERR_SHAPE;
+    if (sums && workspace_bytes < nr_bwd_space(M, C, p)) return BC_ERR_SHAPE;
     if (sums && (uintptr_t)workspace % 256) return BC_ERR_ALIGN;
     NormArgs a = {};
     a.h = h; a.y = y; a.wo = out_weight; a.bo = out_bias; a.gate = gate; a.wi = in_weight;
-    a.stats = (float *)stats; a.gh = gh; a.gu = gu; a.dh = dh; a.dy = dy; a.part = sums ? (float *)workspace : nullptr;
-    a.means = sums && s.E != 8 ? (float *)((char *)workspace + 20ll * C * q.chunks * q.groups) : nullptr;
-    a.ldh = ldh; a.ldy = ldy; a.ldgh = ldgh; a.ldgu = ldgu; a.M = (int)M; a.C = C; a.rows_per_gate = (int)rows_per_gate;
+    a.stats = (float *)stats; a.gh = gh; a.gu = gu; a.dh = dh; a.dy = dy;
+    a.means = sums && p.second ? (float *)workspace : nullptr;
+    float *part = sums ? (float *)((char *)workspace + nr_bwd_space(M, C, p) - 20ll * C * q.chunks * q.groups) : nullptr;
+    a.part = p.second ? nullptr : part;
+    a.ldh = ldh; a.ldy = ldy; a.ldgh = ldgh; a.ldgu = ldgu; a.M = (int)M; a.C = C;
+    a.rows_per_gate = p.gates ? 0 : (int)rows_per_gate;
+    a.gate_every = p.gates ? (int)rows_per_gate : 0;
     a.out_kind = out_kind; a.in_kind = in_kind; a.pf32 = params_f32; a.alpha = residual_scale;
     a.need_dh = dh != nullptr; a.need_dy = dy != nullptr;
     a.g_log = s.g_log; a.span = c.span; a.chunks = c.chunks;
-    const int r = nr_dispatch(dtype, true, a, s, (unsigned)(c.chunks * c.groups), (hipStream_t)stream);
+    const hipStream_t st = (hipStream_t)stream;
+    const int r = nr_dispatch(dtype, true, a, s, (unsigned)(c.chunks * c.groups), st);
     if (r != BC_OK || !sums) return r;
-    if (s.E != 8) {
+    if (p.second) {
+        a.part = part;
         a.span = q.span;
         a.chunks = q.chunks;
+        a.d_gate = d_gate;
         const dim3 grid(nr_strips(C, dtype), (unsigned)(q.chunks * q.groups));
         switch (dtype) {
-        case DT_F32: k_norm_cols<DT_F32><<<grid, 256, 0, (hipStream_t)stream>>>(a); break;
-        case DT_F16: k_norm_cols<DT_F16><<<grid, 256, 0, (hipStream_t)stream>>>(a); break;
-        default: k_norm_cols<DT_BF16><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        case DT_F32: nr_cols<DT_F32>(a, p.gates, grid, st); break;
+        case DT_F16: nr_cols<DT_F16>(a, p.gates, grid, st); break;
+        default: nr_cols<DT_BF16>(a, p.gates, grid, st);
         }
     }
     NormJoin j = {};
-    j.part = (const float *)workspace;
-    j.out[0] = d_gate; j.out[1] = d_out_weight; j.out[2] = d_out_bias; j.out[3] = d_in_weight; j.out[4] = d_in_bias;
+    j.part = part;
+    j.out[0] = p.gates ? nullptr : d_gate; j.out[1] = d_out_weight; j.out[2] = d_out_bias; j.out[3] = d_in_weight; j.out[4] = d_in_bias;
     j.C = C; j.blocks = q.chunks * q.groups; j.chunks = q.chunks; j.groups = q.groups; j.f32 = params_f32;
-    const dim3 grid((unsigned)((C + 15) / 16), 5, (unsigned)q.groups);
+    const dim3 grid(4 + (j.out[0] ? (unsigned)q.groups : 0), (unsigned)((C + 15) / 16));
     switch (dtype) {
-    case DT_F32: k_norm_join<DT_F32><<<grid, 256, 0, (hipStream_t)stream>>>(j); break;
-    case DT_F16: k_norm_join<DT_F16><<<grid, 256, 0, (hipStream_t)stream>>>(j); break;
-    default: k_norm_join<DT_BF16><<<grid, 256, 0, (hipStream_t)stream>>>(j);
+    case DT_F32: k_norm_join<DT_F32><<<grid, 256, 0, st>>>(j); break;
+    case DT_F16: k_norm_join<DT_F16><<<grid, 256, 0, st>>>(j); break;
+    default: k_norm_join<DT_BF16><<<grid, 256, 0, st>>>(j);
     }
     return nr_status();
 }

@@ -189,3 +189,45 @@ def test_parameter_gradients_of_a_frame_with_surplus_tiles_are_refused(plain_bac
                     out.sum().backward()
             else:
                 out.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------------ many gates
+@pytest.mark.parametrize("M,C,rpg", [(65535, 4096, 1), (65535 * 2, 1024, 2), (65528, 1024, 8), (65535, 16384, 1), (65535, 16, 1), (60000, 9000, 3), (4200, 48, 2)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_workspace_of_many_gates(M, C, rpg, dtype):
+    """The backward pass asks for no more than the size of one of its tensors, or 32 MB."""
+    import blockcopy.backend as bk
+
+    assert bk.load_library().bc_norm_residual_bwd_workspace(M, C, rpg, dtype) <= max(M * C * (4 if dtype == 0 else 2), 32 << 20) + 8 * M
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("M,C,groups", [(20000, 64, 20000), (30003, 33, 30003), (9000, 200, 4500), (9002, 201, 4501), (2400, 1030, 1200), (900, 4096, 450), (600, 8192, 300), (300, 9000, 100),
+                                        (60, 16384, 60), (6000, 520, 2000)])
+def test_many_gates(dt, M, C, groups):
+    """Gates of few rows each: every gradient."""
+    _norm_case(dt, M, C, "layer", "rms", gate="sample", groups=groups, seed=71)
+    _norm_case(dt, M, C, "none", "layer", gate="sample", groups=groups, seed=72, bias=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,C,groups", [(20000, 64, 20000), (300, 9000, 100), (9002, 201, 4501)])
+def test_many_gates_each_gradient_alone(M, C, groups):
+    import blockcopy
+
+    gen = torch.Generator().manual_seed(73)
+    dtype, R = torch.bfloat16, M // groups
+    ts = [_rand(gen, groups, R, C, dtype=dtype), _rand(gen, groups, R, C, dtype=dtype), *(_rand(gen, C, dtype=dtype, mean=1.0, std=0.2) for _ in range(2)),
+          _rand(gen, groups, 1, C, dtype=dtype), *(_rand(gen, C, dtype=dtype, mean=1.0, std=0.2) for _ in range(2))]
+    gs = [_rand(gen, groups, R, C, dtype=dtype) for _ in range(2)]
+
+    def grads(live):
+        a = [t.clone().requires_grad_(i in live) for i, t in enumerate(ts)]
+        out = blockcopy.norm_residual(a[0], a[1], out_norm="layer", out_weight=a[2], out_bias=a[3], gate=a[4], in_norm="rms", in_weight=a[5], in_bias=a[6])
+        return torch.autograd.grad(out, [a[i] for i in live], gs)
+
+    full = grads(range(7))
+    for i in range(7):
+        assert torch.equal(grads([i])[0], full[i]), i
+    assert all(torch.equal(p, q) for p, q in zip(full, grads(range(7))))
