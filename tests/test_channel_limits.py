@@ -231,3 +231,78 @@ def test_many_gates_each_gradient_alone(M, C, groups):
     for i in range(7):
         assert torch.equal(grads([i])[0], full[i]), i
     assert all(torch.equal(p, q) for p, q in zip(full, grads(range(7))))
+
+
+# ------------------------------------------------------------------------------------------------ more rows than one step of every workgroup
+def _rows_at_once(C):
+    """Rows that one step of a whole launch takes at most, and rows that any launch of the backward pass takes in one step: a row of up to 512
+    channels is a power of two of lanes with eight channels each, 256 lanes a workgroup; up to 1024 two rows share a workgroup; beyond one."""
+    lanes = 1
+    while lanes < 64 and 8 * lanes < C:
+        lanes *= 2
+    per = 256 // lanes if C <= 512 else 2 if C <= 1024 else 1
+    return (1280 if C <= 2048 else 512) * per, 256 * per
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("C", [5, 40, 200, 500, 1001, 1024, 1500, 2048, 2100, 4096, 4100, 8192, 8200, 9001])
+def test_norm_rows_of_later_steps(dt, C):
+    """Workgroups that take four rows and more, the last step ragged: every row's results and gradients have the bits that the same row has in a
+    call where each workgroup takes one step, and the column sums are those of all rows."""
+    import blockcopy
+
+    most, once = _rows_at_once(C)
+    M = 3 * most + most // 3 + 1
+    assert M > 3 * most
+    gen = torch.Generator(device="cuda").manual_seed(81)
+    dtype = DT[dt]
+    r = lambda *s, std=1.0, mean=0.0, t=dtype: (torch.randn(s, generator=gen, device="cuda") * std + mean).to(t)
+    h, y, gh, gu = r(M, C, mean=0.3), r(M, C, std=0.7), r(M, C), torch.randint(-3, 4, (M, C), generator=gen, device="cuda").to(dtype)
+    ps = [r(C, std=0.2, mean=1.0, t=torch.float32) for _ in range(5)]
+    names = ("out_weight", "out_bias", "gate", "in_weight", "in_bias")
+
+    def run(rows):
+        a = [t[rows].clone().requires_grad_(True) for t in (h, y)] + [p.clone().requires_grad_(True) for p in ps]
+        out = blockcopy.norm_residual(a[0], a[1], out_norm="layer", in_norm="layer", **dict(zip(names, a[2:])))
+        return [*(o.detach() for o in out), *torch.autograd.grad(out, a, (gh[rows], gu[rows]))]
+
+    whole = run(slice(0, M))
+    sums = [torch.zeros(C, dtype=torch.float64, device="cuda") for _ in range(5)]
+    for m in range(0, M, once):
+        part = run(slice(m, min(M, m + once)))
+        for k in range(4):
+            assert torch.equal(whole[k][m:m + once], part[k]), (C, k, m)
+        for s, p in zip(sums, part[4:]):
+            s += p.double()
+    assert torch.equal(whole[8].double(), gu.double().sum(0))       # (whole numbers: d in_bias is exact)
+    # the other sums: both sides add at most 200 partial results of a column in a row, of terms no larger than these
+    n = lambda x: (x - x.mean(-1, keepdim=True)) / (x.var(-1, keepdim=True, unbiased=False) + 1e-6).sqrt() if C > 1 else x * 0
+    ny, nh = n(y.double()).abs(), n(whole[0].double()).abs() * 1.02 + 0.02
+    sd = whole[0].double().std(-1, keepdim=True)
+    q = gu.double().abs() * ps[3].double().abs()
+    g = gh.double().abs() + (q + q.mean(-1, keepdim=True) + nh * (q * nh).mean(-1, keepdim=True)) / sd.clamp_min(1e-3) * 1.02
+    gate = ps[2].double().abs()
+    sizes = [(g * gate * ny).sum(0), (g * gate).sum(0), (g * (ny * ps[0].double().abs() + ps[1].double().abs())).sum(0), (gu.double().abs() * nh).sum(0)]
+    for k, (s, size) in enumerate(zip(sums, sizes)):
+        over = (whole[4 + k].double() - s).abs() - 2 * 200 * CO.U * size
+        assert bool((over <= 0).all()), (C, names[k], float(over.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("C,groups", [(40, 3), (500, 2), (1001, 3), (2048, 5), (4100, 2), (9001, 3)])
+def test_norm_long_gate_groups(dt, C, groups):
+    """A gate per sample of many rows: whole numbers without norms, so that every gradient is exact."""
+    import blockcopy
+
+    R = 3 * _rows_at_once(C)[0] // groups + 7
+    gen = torch.Generator(device="cuda").manual_seed(83)
+    pick = lambda *s: torch.randint(-2, 3, s, generator=gen, device="cuda").to(DT[dt])
+    h, y, gh = pick(groups, R, C).requires_grad_(True), pick(groups, R, C).requires_grad_(True), pick(groups, R, C)
+    gate = torch.randint(-2, 3, (groups, 1, C), generator=gen, device="cuda").float().requires_grad_(True)
+    ho, _ = blockcopy.norm_residual(h, y, gate=gate, residual_scale=2.0)
+    assert torch.equal(ho.double(), 2 * h.double() + gate.double() * y.double())
+    dh, dy, dg = torch.autograd.grad(ho, [h, y, gate], gh)
+    assert torch.equal(dh.double(), 2 * gh.double()) and torch.equal(dy.double(), gate.double() * gh.double())
+    assert torch.equal(dg.double(), (gh.double() * y.double()).sum(1, keepdim=True))
