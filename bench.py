@@ -75,7 +75,8 @@ def parse_args(argv=None):
                          "scenario (configs/swiftnet_rn18/swiftnet_rn18_rl05_speed.sh: rl_semseg, target 0.5, --half, batch 2, train-interval 3), "
                          "C4 = SwiftNet-RN50 2048x4096 block 64 target 0.25, C5 = CSP-ResNet50 pedestrian detector 1024x2048 block 128 target 0.3 "
                          "(one stream per GPU)")
-    ap.add_argument("--upload-variant", type=int, default=1, help="1 (default, N=1): also report the PCIe-inclusive fps of the reference's full loop")
+    # (off by default: harness.measure_fps_with_upload ended one run of its test with exit status 134 in the warm-up clip, for a cause not found yet)
+    ap.add_argument("--upload-variant", type=int, default=0, help="1 (N=1): also report the PCIe-inclusive fps of the reference's full loop")
     ap.add_argument("--stub-cpu", action="store_true",
                     help="(tests only) replace the GPU workload by a tiny CPU stand-in so that the launcher, the per-rank "
                          "environment and the clock bracket can be exercised on a machine without a GPU")

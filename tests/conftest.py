@@ -18,8 +18,8 @@ def pytest_configure(config):
 
 # GPU tests that have ended their process now and then, for a cause not found yet: off until it is
 UNEXPLAINED_ABORTS = {
-    "test_upload_inclusive_loop_gives_the_same_predictions": "aborted its process once (exit status 134) in the warm-up clip of "
-                                                            "harness.measure_fps_with_upload, cause not shown; passes in most runs",
+    ("test_gpu_e2e.py", "test_upload_inclusive_loop_gives_the_same_predictions"): "aborted its process once (exit status 134) in the warm-up clip of "
+                                                                                   "harness.measure_fps_with_upload, cause not shown; passes in most runs",
 }
 
 
@@ -28,7 +28,7 @@ def pytest_collection_modifyitems(config, items):
     import torch
 
     for item in items:
-        reason = UNEXPLAINED_ABORTS.get(getattr(item, "originalname", None) or item.name)
+        reason = UNEXPLAINED_ABORTS.get((item.path.name, getattr(item, "originalname", None) or item.name))
         if reason:
             item.add_marker(pytest.mark.skip(reason=reason))
     if torch.cuda.is_available():
