@@ -306,3 +306,27 @@ def test_norm_long_gate_groups(dt, C, groups):
     dh, dy, dg = torch.autograd.grad(ho, [h, y, gate], gh)
     assert torch.equal(dh.double(), 2 * gh.double()) and torch.equal(dy.double(), gate.double() * gh.double())
     assert torch.equal(dg.double(), (gh.double() * y.double()).sum(1, keepdim=True))
+
+
+@pytest.mark.gpu
+def test_gradient_offsets_beyond_32_bits():
+    """More than 2^31 elements of dz: the far rows' pre-activations and both parts of dz lie at their own places."""
+    import blockcopy
+
+    K, N, far = 24, 1032, 300
+    M = (1 << 31) // N + far
+    gen = torch.Generator().manual_seed(91)
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    x[-far:] = _rand(gen, far, K, dtype=torch.bfloat16)
+    w, b = _rand(gen, N, K, dtype=torch.bfloat16, std=K ** -0.5), _rand(gen, N, dtype=torch.bfloat16, std=0.3)
+    gy = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    gy[-far:] = _rand(gen, far, N, dtype=torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = blockcopy.linear_act(x, w, b, activation="silu")
+    dx, dw, db = torch.autograd.grad(y, leaves, gy)
+    # (the other rows' terms are zeros: they change no bound)
+    want = CO.linear_gradients(x.detach()[-far:], w.detach(), b.detach(), "silu", gy[-far:])
+    _close(dx[-far:], *want["dx"], "dx")
+    _close(dw, *want["dw"], "dw")
+    _close(db, *want["db"], "db")
+    assert not bool(dx[:-far].any())
