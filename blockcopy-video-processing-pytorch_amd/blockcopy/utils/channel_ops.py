@@ -8,11 +8,12 @@ API: an addition).
 Both work on rows of features: the last axis of a tensor (``dim=-1``, tokens), or axis 1 of a (N, C, H, W) map (``dim=1``, pixels), for which
 channels-last memory is the free layout.  A packed or dense ``TensorWrapper`` is always read along axis 1 and gives a ``TensorWrapper``: rows
 are independent of each other, so no halo, no transfer and no cache is involved, and skipped tiles keep their values when the result is
-combined (in a frame sized for a ceiling of tiles every row is computed, the surplus ones out of whatever they hold, and gradients of parameters are refused).  float32, float16 and
-bfloat16; sums, statistics, activations and everything between input and output in float32.  GPU tensors only.
+combined (in a frame sized for a ceiling of tiles every row is computed, the surplus ones out of whatever they hold, and gradients of
+parameters are refused).  float32, float16 and bfloat16; sums, statistics, activations and everything between input and output in float32,
+gradients too: nothing but a result is rounded to the tensors' type.  GPU tensors only.
 
-Both are differentiable once with respect to every tensor argument, backward (a forward-mode tangent is refused).  Gradients of a captured graph follow torch's rule for captured
-backward passes: warm up on the capturing stream, with no eager graph over the same leaves alive.  A small training step spends most of its
+Both are differentiable once with respect to every tensor argument, backward (a forward-mode tangent is refused).  Gradients of a captured
+graph follow torch's rule for captured backward passes: warm up on the capturing stream, with no eager graph over the same leaves alive.  A small training step spends most of its
 time on the host: capture it, or run it under ``torch.autograd.set_multithreading_enabled(False)`` (half the time uncaptured).  No call waits
 for the device, and every result is run-to-run identical (sums are split and joined in a fixed order, no atomics)."""
 from __future__ import annotations

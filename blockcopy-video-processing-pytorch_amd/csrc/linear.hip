@@ -53,7 +53,8 @@ template <int DT> __device__ __forceinline__ float lin_sigmoid(float v)
 // Phi(z) = erfc(-z / sqrt 2) / 2 and e = exp(-z^2 / 2), to float's relative precision in the lower tail too (1 + erf would cancel there).  16-bit
 // tensors: with x = |z| / sqrt 2 and t = 1 / (1 + p x), exp(x^2) erfc(x) / 2 = t Q(t) for 0 <= t <= 1; Q of degree 7 and p = 0.46 by a weighted minimax fit
 // (linear program over 1200 Chebyshev points), off by at most 7e-7 of the value, 1e-6 as evaluated -- 17 instructions, and the derivative needs
-// the same exponential.  erfcf is several times that: an epilogue of 256 x 256 outputs spent 17 us on erff, more than eight steps of products
+// the same exponential (a 5-term form of absolute precision, off by 1 % at z = -8: 62.4 us against 63.6 for bf16 17408 x 512 x 2048).  The library's functions are
+// several times that: an epilogue of 256 x 256 outputs spent 17 us on erff, more than eight steps of products
 template <int DT> __device__ __forceinline__ float lin_phi(float z, float &e)
 {
     if constexpr (DT == DT_F32) {
@@ -356,9 +357,10 @@ __device__ __forceinline__ void lin_meet()
 // while step t is multiplied, step t + 1 travels into the other one, one barrier per step.  DIRECT: operands whose vectors are aligned travel
 // global -> LDS without registers (a partial last step goes through registers, zero-filled); otherwise through registers, requested before
 // the products and stored behind them.  TWO: the row operand's two parts (LinParts), the sum run over twice, the lower part first.
-// Bound: the matrix pipe for long sums (bf16 16384 x 4096 x 8192 with gelu_tanh 890 us = 1235 TFLOP/s, a library product alone 824; its gradients'
-// shapes 1130 - 1180; fp32 17408 x 768 x 256 64 us = 107 TFLOP/s of 136: 4.25 tiles per CU take the time of 5).  Short sums: the epilogue's
-// instructions and the outputs (bf16 17408 x 512 x 2048 53 us, with gelu 61: 25 instructions per output, 40 % of the time, on the vector pipe).
+// Bound: the matrix pipe for long sums (bf16 16384 x 4096 x 8192 with gelu_tanh 880 us = 1250 TFLOP/s, a library product alone 824; the two gradients
+// of 8192 x 2048 x 8192 with two parts each 492 and 502 us = 1095 - 1117; fp32 17408 x 768 x 256 64 us = 107 TFLOP/s of 136: 4.25 tiles per CU take the
+// time of 5).  Short sums: products, epilogue and stores of a tile follow each other, only the CU's other workgroups overlap them (bf16 17408 x
+// 512 x 2048 54 us, with gelu 63.5: vector pipe 43 % of the time, matrix pipe 23 %, waves wait 39 % of theirs for memory and barriers).
 // (steps of 64 bytes: 128 registers, so that four workgroups share a CU; with three 131072 x 256 x 512 57 us against 51, with five it spills)
 template <int DT, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool DIRECT, int C, bool TWO>
 __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const LinArgs g)
@@ -653,7 +655,7 @@ template <int DT, int MB, int NW> __global__ __launch_bounds__(64 * NW) void k_l
 }
 
 // dz = dy * act'(z) (CURVED, 16 bits: its two parts) and the column sums of dz over a run of rows.  tpr threads (a power of two) take W columns each of a row.  Bound: memory, two
-// reads and a write (fp16 131072 x 512 with gelu 95 us = 4.2 TB/s; the instructions of gelu' are half of that time)
+// reads and a write (fp16 131072 x 512 with gelu, 671 MB with z in fp32 and two parts of dz: 150 us = 4.5 TB/s)
 struct DactArgs {
     const void *gy, *z;         // z NULL: no activation, dz = gy
     void *dz, *lo;              // NULL: not stored; lo: the lower part (CURVED in 16 bits)
@@ -770,8 +772,8 @@ LinPlan lin_plan(int dtype, long long M, long long N, long long K)
     const long long steps = (K + bk - 1) / bk, t64 = lin_tiles(M, N, 64), t128 = lin_tiles(M, N, 128), t256 = lin_tiles(M, N, 256);
     long long s;
     if (dtype == DT_F32) {
-        // 64 (the matrix instructions take so long that a small tile's operands arrive in time: 17408 x 768 x 256 72 us against 105 with 128, 1024^3
-        // 24 against 34).  Slices until every CU has a tile, of 2 steps at least (128 x 512 x 512 8 slices 8.2 us, one 12.9), or two or three, of 24
+        // 64 (the matrix instructions take so long that a small tile's operands arrive in time: 17408 x 768 x 256 and 1024^3 in 0.7 of the time that
+        // 128 takes).  Slices until every CU has a tile, of 2 steps at least (128 x 512 x 512 8 slices 8.2 us, one 12.9), or two or three, of 24
         // steps at least (256 x 768 x 17408 16 slices 62 us, 8: 80; but 512 x 1024 x 1024 2 slices 17 us, 4: 19; 256 x 4096 x 1024 4: 28, 5: 35)
         p.edge = 64;
         s = lin_min(LIN_CUS / t64, steps / 2);

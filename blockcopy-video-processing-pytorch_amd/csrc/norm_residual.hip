@@ -401,7 +401,8 @@ template <int V, int NV, bool ODD, int WPR, int NW> __device__ __forceinline__ v
 // Backward, p = du * wi, n and n' the normalised y and h':
 //   g = dh' + (p - mean(p) - n' mean(p n')) / dev'   (rms: without mean(p))     dh = scale * g     q = g * gate * wo
 //   dy = (q - mean(q) - n mean(q n)) / dev           d gate = sum g (n wo + bo)   d wo = gate sum g n   d bo = gate sum g   d wi = sum du n'   d bi = sum du
-// (rows of more than 8192 channels, 16 per lane: four sums of each would not fit the 128 registers of a lane; they go to k_norm_cols.  GATES: so do
+// (rows of more than 8192 channels, 16 per lane: four sums of each would not fit the 128 registers of a lane; they go to k_norm_cols, and what is left
+// still spills 184 - 356 bytes per lane, rows of any width of 4097 .. 8192 channels 44 - 116: their rates in the table above are those of spilling code.  GATES: so do
 // those of many gates, and a row takes its own)
 template <int DT, int V, int NV, int WPR, bool ODD, bool GATES>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, DT == DT_F32 || WPR > 4 || ODD ? 1 : 3) void k_norm_bwd(const NormArgs a)
@@ -768,8 +769,8 @@ NormChunks nr_split(long long M, long long rows_per_gate, int want, int rows_per
 // workgroups of a launch: as many as run at once, so that each asks for its parameters and its first row once.  Forward, 128 MB per tensor, bf16:
 // 16384 x 4096 107 us with two per CU, 129 with sixteen; 22369 x 3000 129 and 239; 8192 x 8192 126 with one, 160 with sixteen; 32768 x 2048 108 with
 // four, 148 with two.  fp32 rows of whole vectors saturate memory with half as many (32768 x 2048 193 us with two, 211 with four; 65154 x 1030 349
-// with two, 230 with four).  Backward: 16384 x 4096 214 us with one, 232 with three (1024 x 4096 28 and 40: fewer sums to join); 43690 x 1536 200 with
-// three, 238 with two (fp32: 391 and 421 -- but 65154 x 1030 563 and 434)
+// with two, 230 with four).  Backward (ratios of times as the rule was made): 16384 x 4096 one per CU 0.92 of three (1024 x 4096 0.70: fewer sums to join);
+// 43690 x 1536 three 0.84 of two (fp32 0.93 -- but 65154 x 1030 1.30)
 int nr_fill(const NormShape &s, int dtype, bool bwd)
 {
     if (bwd) return NR_CUS * (s.waves > 4 ? 1 : s.waves == 3 && dtype != DT_F32 ? 3 : 2);
