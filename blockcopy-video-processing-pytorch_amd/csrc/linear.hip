@@ -510,13 +510,14 @@ __global__ __launch_bounds__(64 * WM * WN, C == 4 ? 4 : 1) void k_lin_gemm(const
                 pb = (const char *)rows.p + ((BMC ? (size_t)kbeg * g.b.ld + m0 : (size_t)m0 * g.b.ld + kbeg)) * ES;
             }
             sum();
-            if constexpr (LinParts<DT>::LO != 1.f) {
-                const float f = part ? 1.f / LinParts<DT>::LO : 1.f / LinParts<DT>::PRE;
+            // (an infinity or NaN among the operands is the upper part's to answer for: what is left of dz may be 0 or of the other sign)
+            const float f = part ? 1.f / LinParts<DT>::LO : 1.f / LinParts<DT>::PRE;
 #pragma unroll
-                for (int i = 0; i < FN; ++i)
+            for (int i = 0; i < FN; ++i)
 #pragma unroll
-                    for (int j = 0; j < FM; ++j) acc[i][j] *= f;
-            }
+                for (int j = 0; j < FM; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = part && !__builtin_isfinite(acc[i][j][e]) ? 0.f : acc[i][j][e] * f;
         }
 
     // the sums meet their epilogue through the LDS: a wave lays RH rows of them (16-byte vector c of row r at c ^ (r & its mask)) into its own

@@ -330,3 +330,32 @@ def test_gradient_offsets_beyond_32_bits():
     _close(dw, *want["dw"], "dw")
     _close(db, *want["db"], "db")
     assert not bool(dx[:-far].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("name", SMOOTH)
+def test_infinite_operands_of_gradients(dt, name):
+    """An infinity in a row of x or w makes the gradients that it is multiplied into what the products say: infinite with the sign of dz, NaN where dz
+    is zero -- in those places only."""
+    import blockcopy
+
+    gen = torch.Generator().manual_seed(93)
+    x, w = _rand(gen, 70, 40, dtype=DT[dt]), _rand(gen, 24, 40, dtype=DT[dt])
+    gy = _rand(gen, 70, 24, dtype=DT[dt])
+    x[9, 3] = float("inf")
+    run = lambda a, b: torch.autograd.grad(blockcopy.linear_act(a.requires_grad_(True), b.requires_grad_(True), activation=name), [a, b], gy)
+    dx, dw = run(x.clone(), w.clone())
+    # row 9: z = +-inf, act' = 1 or 0, dz = gy or +-0
+    up = w[:, 3] > 0
+    want = torch.where(up, gy[9].sign() * float("inf"), torch.full_like(gy[9], float("nan")))
+    assert torch.equal(dw[up, 3], want[up]) and bool(dw[~up, 3].isnan().all())
+    keep = [i for i in range(40) if i != 3]
+    assert bool(dw[:, keep].isfinite().all()) and bool(dx.isfinite().all())
+    x[9, 3], w[7, 5] = 0.0, float("inf")
+    dx, dw = run(x.clone(), w.clone())
+    # column 7 of z = +-inf by the sign of x[:, 5]
+    up = x[:, 5] > 0
+    assert torch.equal(dx[up, 5], gy[up, 7].sign() * float("inf")) and bool(dx[~up, 5].isnan().all())
+    keep = [i for i in range(40) if i != 5]
+    assert bool(dx[:, keep].isfinite().all()) and bool(dw.isfinite().all())
